@@ -16,9 +16,11 @@ ERR_NAMES = {1: "FG_ERR_INVALID", 2: "FG_ERR_CUDA", 3: "FG_ERR_COMPILE", 4: "FG_
              5: "FG_ERR_DEVICE", 6: "FG_ERR_UNSUPPORTED"}
 
 F32, I32, BOOL = 0, 1, 2
+BF16, F16 = 3, 4  # layer operators only
 REDUCE_SUM, REDUCE_MAX = 0, 1
 EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_RELU_MASK = 0, 1, 2, 3
 GEMM_A_MN_MAJOR, GEMM_B_MN_MAJOR, GEMM_1XTF32 = 1, 2, 4
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4
 ARG_BUFFER, ARG_I32, ARG_F32, ARG_BOOL = 0, 1, 2, 3
 UNIQUE_ID_BYTES = 128
 PEER_HANDLE_BYTES = 96
@@ -40,6 +42,40 @@ class _ArgValue(ctypes.Union):
 
 class KernelArgC(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int32), ("v", _ArgValue)]
+
+
+class DropoutC(ctypes.Structure):
+    """fg_dropout_spec."""
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64)]
+
+
+class LinearArgsC(ctypes.Structure):
+    """fg_linear_args."""
+    _fields_ = [("dtype", ctypes.c_int32), ("M", ctypes.c_int32), ("N", ctypes.c_int32),
+                ("K", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("x_row", ctypes.c_int64), ("x_col", ctypes.c_int64),
+                ("w", ctypes.c_void_p), ("w_row", ctypes.c_int64), ("w_col", ctypes.c_int64),
+                ("bias", ctypes.c_void_p),
+                ("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64),
+                ("act", ctypes.c_int32), ("reserved", ctypes.c_int32), ("drop", DropoutC),
+                ("pre", ctypes.c_void_p), ("ld_pre", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("ld_out", ctypes.c_int64),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class LinearGradArgsC(ctypes.Structure):
+    """fg_linear_grad_args."""
+    _fields_ = [("dtype", ctypes.c_int32), ("M", ctypes.c_int32), ("N", ctypes.c_int32),
+                ("K", ctypes.c_int32),
+                ("dy", ctypes.c_void_p), ("dy_row", ctypes.c_int64), ("dy_col", ctypes.c_int64),
+                ("x", ctypes.c_void_p), ("x_row", ctypes.c_int64), ("x_col", ctypes.c_int64),
+                ("w", ctypes.c_void_p), ("w_row", ctypes.c_int64), ("w_col", ctypes.c_int64),
+                ("pre", ctypes.c_void_p), ("ld_pre", ctypes.c_int64),
+                ("act", ctypes.c_int32), ("reserved", ctypes.c_int32), ("drop", DropoutC),
+                ("dx", ctypes.c_void_p), ("ld_dx", ctypes.c_int64),
+                ("dw", ctypes.c_void_p), ("ld_dw", ctypes.c_int64),
+                ("db", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 # (name, restype, argtypes) for every exported entry point in include/ferro_cuda.h.
@@ -76,6 +112,12 @@ SIGNATURES = [
     ("fg_one_hot_u8", _i, [_vp, _vp, _sz, _i, _vp]),
     ("fg_gemm_3xtf32", _i, [_i, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp,
                             _i, _vp]),
+    ("fg_linear_workspace", _i, [ctypes.POINTER(LinearArgsC), ctypes.POINTER(_sz)]),
+    ("fg_linear", _i, [ctypes.POINTER(LinearArgsC), _vp]),
+    ("fg_linear_grad_workspace", _i, [ctypes.POINTER(LinearGradArgsC), ctypes.POINTER(_sz)]),
+    ("fg_linear_grad", _i, [ctypes.POINTER(LinearGradArgsC), _vp]),
+    ("fg_dropout", _i, [_i, _sz, _sz, _vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp,
+                        ctypes.c_int64, ctypes.POINTER(DropoutC), _vp]),
     ("fg_mlp_create", _i, [_vp, _i, ctypes.POINTER(_i), _i, _f, _pp]),
     ("fg_mlp_destroy", _i, [_vp]),
     ("fg_mlp_set_params", _i, [_vp, _i, _vp, _vp]),

@@ -1,0 +1,529 @@
+// The linear layer with a fused epilogue, its gradient and dropout.
+//
+//   z = x w^T + bias;  out = residual + D(act(z))            fg_linear
+//   dz = D(dy) act'(z);  dx = dz w;  dw = dz^T x;  db = sum dz  fg_linear_grad
+//   out = residual + D(x)                                    fg_dropout
+//
+// D is dropout by a counter-based generator (fg_layer.cuh): the mask is
+// computed where it is used, forwards and backwards, and never stored.
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "fg_internal.h"
+#include "fg_layer.cuh"
+
+namespace fg {
+namespace layer {
+
+// ---------------------------------------------------------------------------
+// C[m, n] = sum_k A(m, k) B(n, k), any strides and sizes (K = 0 included),
+// on the CUDA cores in f32: 64 x 64 tiles, 16-deep steps through shared
+// memory, 2 rows x 8 columns a thread.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_linear_tile(const T *__restrict__ a, int64_t ar, int64_t ac, const T *__restrict__ b,
+                  int64_t br, int64_t bc, int K, const Epilogue e) {
+  __shared__ float sa[16][64 + 4], sb[16][64 + 4];
+  const int m0 = blockIdx.x * 64;
+  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+  for (int n0 = blockIdx.y * 64; n0 < e.N; n0 += gridDim.y * 64) {
+    float acc[2][8] = {};
+    for (int k0 = 0; k0 < K; k0 += 16) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+        // neighbouring threads walk the operand's contiguous direction
+        const int ak = ac == 1 ? i & 15 : i >> 6, am = ac == 1 ? i >> 4 : i & 63;
+        const int bk = bc == 1 ? i & 15 : i >> 6, bn = bc == 1 ? i >> 4 : i & 63;
+        sa[ak][am] = m0 + am < e.M && k0 + ak < K
+                         ? to_f32<T>(a[(m0 + am) * ar + (k0 + ak) * ac]) : 0.0f;
+        sb[bk][bn] = n0 + bn < e.N && k0 + bk < K
+                         ? to_f32<T>(b[(n0 + bn) * br + (k0 + bk) * bc]) : 0.0f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 16; k++) {
+        const float a0 = sa[k][ty], a1 = sa[k][ty + 32];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float bj = sb[k][tx * 8 + j];
+          acc[0][j] = fmaf(a0, bj, acc[0][j]);
+          acc[1][j] = fmaf(a1, bj, acc[1][j]);
+        }
+      }
+    }
+    const int col = n0 + tx * 8;
+    if (col < e.N) {
+      if (m0 + ty < e.M) epilogue8<T>(e, m0 + ty, col, acc[0]);
+      if (m0 + ty + 32 < e.M) epilogue8<T>(e, m0 + ty + 32, col, acc[1]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dz = D(dy) * act'(pre), and the column sums of dz over this block's rows
+// (f32, one row of `part` a block; k_bias_grad adds them up in order).
+// A block takes 256 columns and `rows` rows: 32 lanes x 8 columns, 8 warps
+// over the rows.  dz may be null (only the sums are wanted).
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_layer_dz(const T *__restrict__ dy, int64_t yr, int64_t yc, const T *__restrict__ pre,
+               int64_t ldp, int act, const DropParams drop, T *__restrict__ dz, int64_t ldz,
+               float *__restrict__ part, int M, int N, int rows, int vec) {
+  __shared__ float red[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = blockIdx.x * 256 + lane * 8;
+  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
+  const bool whole = vec && col + 8 <= N;
+  float sum[8] = {};
+  if (col < N)
+    for (int r = r0 + warp; r < r1; r += 8) {
+      float v[8], z[8];
+      if (whole) {
+        load8<T>(dy + r * yr + col, v);
+        if (act != FG_ACT_NONE) load8<T>(pre + r * ldp + col, z);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          v[i] = col + i < N ? to_f32<T>(dy[r * yr + (col + i) * yc]) : 0.0f;
+          z[i] = act != FG_ACT_NONE && col + i < N ? to_f32<T>(pre[r * ldp + col + i]) : 0.0f;
+        }
+      }
+      if (drop.threshold) drop8(drop, r, col, v);
+      if (act == FG_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = 0.0f < z[i] ? v[i] : 0.0f;
+      } else if (act != FG_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= act_slope(z[i], act);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) sum[i] += v[i];
+      if (dz) {
+        if (whole) {
+          store8<T>(dz + r * ldz + col, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (col + i < N) dz[r * ldz + col + i] = from_f32<T>(v[i]);
+        }
+      }
+    }
+  if (!part) return;
+#pragma unroll
+  for (int i = 0; i < 8; i++) red[warp][lane * 8 + i] = sum[i];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < N) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) s += red[w][threadIdx.x];
+    part[(size_t)blockIdx.y * N + c] = s;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_bias_grad(const float *__restrict__ part, int chunks, int N, T *__restrict__ db) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= N) return;
+  float s = 0.0f;
+  for (int i = 0; i < chunks; i++) s += part[(size_t)i * N + c];
+  db[c] = from_f32<T>(s);
+}
+
+// ---------------------------------------------------------------------------
+// out = residual + D(x): eight columns of a row a step.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_dropout(const T *x, int64_t ldx, const T *residual, int64_t ldr, T *out,
+              int64_t ldo, const DropParams drop, int64_t rows, int cols, int vec) {
+  const int64_t groups = (cols + 7) / 8, all = rows * groups;
+  for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < all;
+       g += (int64_t)gridDim.x * 256) {
+    const int64_t r = g / groups;
+    const int col = (int)(g - r * groups) * 8;
+    const bool whole = vec && col + 8 <= cols;
+    float v[8], t[8];
+    if (whole) {
+      load8<T>(x + r * ldx + col, v);
+      if (residual) load8<T>(residual + r * ldr + col, t);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        v[i] = col + i < cols ? to_f32<T>(x[r * ldx + col + i]) : 0.0f;
+        t[i] = residual && col + i < cols ? to_f32<T>(residual[r * ldr + col + i]) : 0.0f;
+      }
+    }
+    if (drop.threshold) drop8(drop, (uint32_t)r, col, v);
+    if (residual) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] += t[i];
+    }
+    if (whole) {
+      store8<T>(out + r * ldo + col, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (col + i < cols) out[r * ldo + col + i] = from_f32<T>(v[i]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+static int elem_size(int dtype) {
+  return dtype == FG_F32 ? 4 : dtype == FG_BF16 || dtype == FG_F16 ? 2 : 0;
+}
+
+static int make_drop(const char *who, const fg_dropout_spec *s, DropParams *d) {
+  *d = DropParams{};
+  if (!s) return FG_OK;
+  FG_REQUIRE(s->p >= 0.0 && s->p <= 1.0, "%s: dropout probability %g is not in [0, 1]", who, s->p);
+  d->threshold = (uint32_t)floor(s->p * 65536.0 + 0.5);
+  d->scale = d->threshold < 65536 ? (float)(65536.0 / (65536 - d->threshold)) : 0.0f;
+  d->k0 = (uint32_t)s->seed;
+  d->k1 = (uint32_t)(s->seed >> 32);
+  d->c2 = (uint32_t)s->offset;
+  d->c3 = (uint32_t)(s->offset >> 32);
+  return FG_OK;
+}
+
+// Rows that start on 16-byte boundaries (or an absent array).
+static bool rows16(const void *p, int64_t ld, int es) {
+  return !p || ((uintptr_t)p % 16 == 0 && ld * es % 16 == 0);
+}
+
+// A rows x cols array's bytes [lo, hi), strides of either sign included.
+struct Span {
+  uintptr_t lo, hi;
+};
+static Span span(const void *p, int64_t rows, int64_t cols, int64_t rs, int64_t cs, int es) {
+  int64_t lo = 0, hi = 0;
+  if (rows > 0 && cols > 0) {
+    (rs < 0 ? lo : hi) += (rows - 1) * rs;
+    (cs < 0 ? lo : hi) += (cols - 1) * cs;
+    hi += 1;
+  }
+  return {(uintptr_t)p + lo * es, (uintptr_t)p + hi * es};
+}
+// Whether a written array may share bytes with another.  Two column ranges of
+// one pitched buffer (equal pitch, disjoint columns) do not.
+static bool overlap(const void *w, int64_t rows, int64_t cols, int64_t ld, const void *q,
+                    int64_t qrows, int64_t qcols, int64_t qrs, int64_t qcs, int es) {
+  if (!w || !q) return false;
+  const Span a = span(w, rows, cols, ld, 1, es), b = span(q, qrows, qcols, qrs, qcs, es);
+  if (a.lo >= b.hi || b.lo >= a.hi) return false;
+  if (ld == qrs && qcs == 1 && ld > 0) {
+    const int64_t pitch = ld * es;
+    int64_t d = (int64_t)((uintptr_t)q - (uintptr_t)w) % pitch;
+    if (d < 0) d += pitch;
+    if (d >= cols * es && d + qcols * es <= pitch) return false;
+  }
+  return true;
+}
+
+template <typename T>
+static int run_tile(const Mat &a, const Mat &b, int K, const Epilogue &e, cudaStream_t st) {
+  const unsigned gx = (unsigned)((e.M + 63LL) / 64), ny = (unsigned)((e.N + 63LL) / 64);
+  k_linear_tile<T><<<dim3(gx, ny < 65535 ? ny : 65535), 256, 0, st>>>(
+      static_cast<const T *>(a.ptr), a.row, a.col, static_cast<const T *>(b.ptr), b.row, b.col, K,
+      e);
+  FG_LAUNCH_TRY();
+  return FG_OK;
+}
+
+// C = A B^T with an epilogue, by the kernel that fits.
+static int run_product(int dtype, const Mat &a, const Mat &b, int K, const Epilogue &e,
+                       cudaStream_t st) {
+  switch (dtype) {
+    case FG_F32:
+      return run_tile<float>(a, b, K, e, st);
+    case FG_BF16:
+      return run_tile<__nv_bfloat16>(a, b, K, e, st);
+    default:
+      return run_tile<__half>(a, b, K, e, st);
+  }
+}
+
+static int check_common(const char *who, int dtype, int M, int N, int K, int act) {
+  FG_REQUIRE(elem_size(dtype) > 0, "%s: dtype %d is not f32, bf16 or f16", who, dtype);
+  const int most = 0x7fffff00;  // tile and column arithmetic stays within an int
+  FG_REQUIRE(M >= 0 && N >= 0 && K >= 0 && M <= most && N <= most && K <= most,
+             "%s: M, N, K must lie in [0, %d] (got %d, %d, %d)", who, most, M, N, K);
+  FG_REQUIRE(act >= FG_ACT_NONE && act <= FG_ACT_SILU, "%s: unknown activation %d", who, act);
+  return FG_OK;
+}
+
+static int linear(const fg_linear_args *g, cudaStream_t st) {
+  const char *who = "fg_linear";
+  FG_REQUIRE(g, "%s: null arguments", who);
+  int rc = check_common(who, g->dtype, g->M, g->N, g->K, g->act);
+  if (rc) return rc;
+  Epilogue e{};
+  if ((rc = make_drop(who, &g->drop, &e.drop))) return rc;
+  if (g->M == 0 || g->N == 0) return FG_OK;
+  const int es = elem_size(g->dtype);
+  FG_REQUIRE(g->out && (g->K == 0 || (g->x && g->w)), "%s: null operand", who);
+  FG_REQUIRE(g->ld_out >= g->N && (!g->pre || g->ld_pre >= g->N), "%s: output pitch too small",
+             who);
+  for (int i = 0; i < 2; i++) {
+    const void *w = i ? g->pre : g->out;
+    const int64_t ld = i ? g->ld_pre : g->ld_out;
+    FG_REQUIRE(!overlap(w, g->M, g->N, ld, g->x, g->M, g->K, g->x_row, g->x_col, es) &&
+                   !overlap(w, g->M, g->N, ld, g->w, g->N, g->K, g->w_row, g->w_col, es) &&
+                   !overlap(w, g->M, g->N, ld, g->bias, 1, g->N, g->N, 1, es),
+               "%s: %s overlaps an operand", who, i ? "pre" : "out");
+    const bool same = !i && g->residual == g->out && g->ld_residual == g->ld_out;
+    FG_REQUIRE(same || !overlap(w, g->M, g->N, ld, g->residual, g->M, g->N, g->ld_residual, 1, es),
+               "%s: %s overlaps the residual (only out may, and only be all of it)", who,
+               i ? "pre" : "out");
+  }
+  FG_REQUIRE(!overlap(g->out, g->M, g->N, g->ld_out, g->pre, g->M, g->N, g->ld_pre, 1, es),
+             "%s: out overlaps pre", who);
+  e.act = g->act;
+  e.bias = g->bias;
+  e.residual = g->residual;
+  e.pre = g->pre;
+  e.out = g->out;
+  e.ldr = g->ld_residual;
+  e.ldp = g->ld_pre;
+  e.ldo = g->ld_out;
+  e.M = g->M;
+  e.N = g->N;
+  e.vec = rows16(e.bias, 0, es) && rows16(e.residual, e.ldr, es) && rows16(e.pre, e.ldp, es) &&
+          rows16(e.out, e.ldo, es);
+  return run_product(g->dtype, {g->x, g->x_row, g->x_col}, {g->w, g->w_row, g->w_col}, g->K, e,
+                     st);
+}
+
+// Rows of a block of k_layer_dz: about four blocks an SM, at least 64 rows.
+static int dz_rows(int M, int N) {
+  const int strips = (int)((N + 255LL) / 256);
+  const int want = strips >= 592 ? 1 : 592 / strips;
+  int rows = (int)((M + (int64_t)want - 1) / want);
+  rows = (rows + 7) / 8 * 8;
+  if (rows < 64) rows = 64;
+  while ((M + (int64_t)rows - 1) / rows > 65535) rows *= 2;
+  return rows;
+}
+
+struct GradPlan {
+  bool need_dz;     // dz differs from dy, and a product reads it
+  int rows, chunks;
+  int64_t ldz;
+  size_t dz_off, part_off, bytes;
+};
+static GradPlan plan_grad(const fg_linear_grad_args *g) {
+  GradPlan p{};
+  const int es = elem_size(g->dtype);
+  p.need_dz = (g->dx || g->dw) && (g->act != FG_ACT_NONE || g->drop.p > 0.0);
+  p.rows = dz_rows(g->M, g->N);
+  p.chunks = (int)((g->M + (int64_t)p.rows - 1) / p.rows);
+  p.ldz = (g->N + 7LL) / 8 * 8;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at += (n + 255) / 256 * 256;
+    return o;
+  };
+  p.dz_off = take(p.need_dz ? (size_t)g->M * p.ldz * es : 0);
+  p.part_off = take(g->db ? (size_t)p.chunks * g->N * 4 : 0);
+  p.bytes = at;
+  return p;
+}
+
+template <typename T>
+static int linear_grad_t(const fg_linear_grad_args *g, const GradPlan &p, const DropParams &drop,
+                         cudaStream_t st) {
+  const int es = sizeof(T);
+  T *dz = p.need_dz ? reinterpret_cast<T *>(static_cast<char *>(g->workspace) + p.dz_off) : nullptr;
+  float *part =
+      g->db ? reinterpret_cast<float *>(static_cast<char *>(g->workspace) + p.part_off) : nullptr;
+  if (dz || part) {
+    const int vec = g->dy_col == 1 && rows16(g->dy, g->dy_row, es) &&
+                    (g->act == FG_ACT_NONE || rows16(g->pre, g->ld_pre, es));
+    k_layer_dz<T><<<dim3((unsigned)((g->N + 255LL) / 256), p.chunks), 256, 0, st>>>(
+        static_cast<const T *>(g->dy), g->dy_row, g->dy_col, static_cast<const T *>(g->pre),
+        g->ld_pre, g->act, drop, dz, p.ldz, part, g->M, g->N, p.rows, vec);
+    FG_LAUNCH_TRY();
+  }
+  if (g->db) {
+    k_bias_grad<T><<<(unsigned)((g->N + 255LL) / 256), 256, 0, st>>>(part, p.chunks, g->N,
+                                                                     static_cast<T *>(g->db));
+    FG_LAUNCH_TRY();
+  }
+  const Mat z = dz ? Mat{dz, p.ldz, 1} : Mat{g->dy, g->dy_row, g->dy_col};
+  Epilogue e{};
+  if (g->dx && g->K > 0) {  // dx[m, k] = sum_n dz(m, n) w(n, k)
+    e.out = g->dx;
+    e.ldo = g->ld_dx;
+    e.M = g->M;
+    e.N = g->K;
+    e.vec = rows16(e.out, e.ldo, es);
+    int rc = run_product(g->dtype, z, {g->w, g->w_col, g->w_row}, g->N, e, st);
+    if (rc) return rc;
+  }
+  if (g->dw && g->K > 0) {  // dw[n, k] = sum_m dz(m, n) x(m, k)
+    e.out = g->dw;
+    e.ldo = g->ld_dw;
+    e.M = g->N;
+    e.N = g->K;
+    e.vec = rows16(e.out, e.ldo, es);
+    int rc = run_product(g->dtype, {z.ptr, z.col, z.row}, {g->x, g->x_col, g->x_row}, g->M, e, st);
+    if (rc) return rc;
+  }
+  return FG_OK;
+}
+
+static int check_grad(const fg_linear_grad_args *g, DropParams *drop) {
+  const char *who = "fg_linear_grad";
+  FG_REQUIRE(g, "%s: null arguments", who);
+  int rc = check_common(who, g->dtype, g->M, g->N, g->K, g->act);
+  if (rc) return rc;
+  if ((rc = make_drop(who, &g->drop, drop))) return rc;
+  const bool rows = g->M > 0 && g->N > 0;
+  FG_REQUIRE(!rows || g->dy, "%s: null dy", who);
+  FG_REQUIRE(!rows || g->act == FG_ACT_NONE || (g->pre && g->ld_pre >= g->N),
+             "%s: the activation's slope needs the pre-activations", who);
+  FG_REQUIRE(!(g->dx && rows && g->K > 0) || g->w, "%s: dx needs w", who);
+  FG_REQUIRE(!(g->dw && rows && g->K > 0) || g->x, "%s: dw needs x", who);
+  FG_REQUIRE((!g->dx || g->ld_dx >= g->K) && (!g->dw || g->ld_dw >= g->K),
+             "%s: output pitch too small", who);
+  const int es = elem_size(g->dtype);
+  struct Out {
+    const char *name;
+    const void *p;
+    int64_t rows, cols, ld;
+  } outs[3] = {{"dx", g->dx, g->M, g->K, g->ld_dx},
+               {"dw", g->dw, g->N, g->K, g->ld_dw},
+               {"db", g->db, 1, g->N, g->N}};
+  for (int i = 0; i < 3; i++) {
+    const Out &o = outs[i];
+    FG_REQUIRE(
+        !overlap(o.p, o.rows, o.cols, o.ld, g->x, g->M, g->K, g->x_row, g->x_col, es) &&
+            !overlap(o.p, o.rows, o.cols, o.ld, g->w, g->N, g->K, g->w_row, g->w_col, es) &&
+            !overlap(o.p, o.rows, o.cols, o.ld, g->dy, g->M, g->N, g->dy_row, g->dy_col, es) &&
+            !overlap(o.p, o.rows, o.cols, o.ld, g->act ? g->pre : nullptr, g->M, g->N, g->ld_pre,
+                     1, es),
+        "%s: %s overlaps an operand", who, o.name);
+    for (int j = i + 1; j < 3; j++)
+      FG_REQUIRE(!overlap(o.p, o.rows, o.cols, o.ld, outs[j].p, outs[j].rows, outs[j].cols,
+                          outs[j].ld, 1, es),
+                 "%s: %s overlaps %s", who, o.name, outs[j].name);
+  }
+  return FG_OK;
+}
+
+static int zero_rows(void *p, int64_t ld, int64_t rows, int64_t cols, int es, cudaStream_t st) {
+  if (!p || rows == 0 || cols == 0) return FG_OK;
+  FG_CUDA_TRY(cudaMemset2DAsync(p, ld * es, 0, cols * es, rows, st));
+  return FG_OK;
+}
+
+static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
+  DropParams drop;
+  int rc = check_grad(g, &drop);
+  if (rc) return rc;
+  const int es = elem_size(g->dtype);
+  if (g->M == 0 || g->N == 0) {  // sums over nothing
+    if ((rc = zero_rows(g->dx, g->ld_dx, g->M, g->K, es, st))) return rc;
+    if ((rc = zero_rows(g->dw, g->ld_dw, g->N, g->K, es, st))) return rc;
+    return zero_rows(g->db, g->N, 1, g->N, es, st);
+  }
+  const GradPlan p = plan_grad(g);
+  FG_REQUIRE(g->workspace_bytes >= p.bytes && (p.bytes == 0 || g->workspace),
+             "fg_linear_grad: %zu bytes of workspace needed, got %zu", p.bytes,
+             g->workspace_bytes);
+  switch (g->dtype) {
+    case FG_F32:
+      return linear_grad_t<float>(g, p, drop, st);
+    case FG_BF16:
+      return linear_grad_t<__nv_bfloat16>(g, p, drop, st);
+    default:
+      return linear_grad_t<__half>(g, p, drop, st);
+  }
+}
+
+static int dropout(int dtype, int64_t rows, int64_t cols, const void *x, int64_t ldx,
+                   const void *residual, int64_t ldr, void *out, int64_t ldo,
+                   const fg_dropout_spec *spec, cudaStream_t st) {
+  const char *who = "fg_dropout";
+  const int es = elem_size(dtype);
+  FG_REQUIRE(es > 0, "%s: dtype %d is not f32, bf16 or f16", who, dtype);
+  FG_REQUIRE(rows >= 0 && cols >= 0 && rows <= 0x7fffffffLL && cols <= 0x7ffffff0LL,
+             "%s: %lld x %lld is out of range", who, (long long)rows, (long long)cols);
+  DropParams d;
+  int rc = make_drop(who, spec, &d);
+  if (rc) return rc;
+  if (rows == 0 || cols == 0) return FG_OK;
+  FG_REQUIRE(x && out, "%s: null operand", who);
+  FG_REQUIRE(ldo >= cols || rows == 1, "%s: output pitch too small", who);
+  FG_REQUIRE((x == out && ldx == ldo) || !overlap(out, rows, cols, ldo, x, rows, cols, ldx, 1, es),
+             "%s: out overlaps x (it may only be all of it)", who);
+  FG_REQUIRE((residual == out && ldr == ldo) ||
+                 !overlap(out, rows, cols, ldo, residual, rows, cols, ldr, 1, es),
+             "%s: out overlaps the residual (it may only be all of it)", who);
+  const int vec = rows16(x, ldx, es) && rows16(residual, ldr, es) && rows16(out, ldo, es);
+  const int64_t groups = rows * ((cols + 7) / 8);
+  const int64_t want = (groups + 255) / 256, cap = 148 * 8;
+  const unsigned grid = (unsigned)(want < cap ? want : cap);
+  switch (dtype) {
+    case FG_F32:
+      k_dropout<float><<<grid, 256, 0, st>>>(
+          static_cast<const float *>(x), ldx, static_cast<const float *>(residual), ldr,
+          static_cast<float *>(out), ldo, d, rows, (int)cols, vec);
+      break;
+    case FG_BF16:
+      k_dropout<__nv_bfloat16><<<grid, 256, 0, st>>>(
+          static_cast<const __nv_bfloat16 *>(x), ldx, static_cast<const __nv_bfloat16 *>(residual),
+          ldr, static_cast<__nv_bfloat16 *>(out), ldo, d, rows, (int)cols, vec);
+      break;
+    default:
+      k_dropout<__half><<<grid, 256, 0, st>>>(
+          static_cast<const __half *>(x), ldx, static_cast<const __half *>(residual), ldr,
+          static_cast<__half *>(out), ldo, d, rows, (int)cols, vec);
+  }
+  FG_LAUNCH_TRY();
+  return FG_OK;
+}
+
+}  // namespace layer
+}  // namespace fg
+
+extern "C" int fg_linear(const fg_linear_args *args, void *stream) {
+  return fg::layer::linear(args, (cudaStream_t)stream);
+}
+
+extern "C" int fg_linear_workspace(const fg_linear_args *args, size_t *bytes) {
+  FG_REQUIRE(args && bytes, "fg_linear_workspace: null argument");
+  *bytes = 0;
+  return FG_OK;
+}
+
+extern "C" int fg_linear_grad_workspace(const fg_linear_grad_args *args, size_t *bytes) {
+  FG_REQUIRE(args && bytes, "fg_linear_grad_workspace: null argument");
+  *bytes = 0;
+  fg::layer::DropParams d;
+  int rc = fg::layer::check_grad(args, &d);
+  if (rc) return rc;
+  if (args->M > 0 && args->N > 0) *bytes = fg::layer::plan_grad(args).bytes;
+  return FG_OK;
+}
+
+extern "C" int fg_linear_grad(const fg_linear_grad_args *args, void *stream) {
+  return fg::layer::linear_grad(args, (cudaStream_t)stream);
+}
+
+extern "C" int fg_dropout(int dtype, size_t rows, size_t cols, const void *d_x, int64_t ldx,
+                          const void *d_residual, int64_t ldr, void *d_out, int64_t ldo,
+                          const fg_dropout_spec *drop, void *stream) {
+  FG_REQUIRE(rows <= 0x7fffffffu && cols <= 0x7ffffff0u, "fg_dropout: %zu x %zu is out of range",
+             rows, cols);
+  return fg::layer::dropout(dtype, (int64_t)rows, (int64_t)cols, d_x, ldx, d_residual, ldr, d_out,
+                            ldo, drop, (cudaStream_t)stream);
+}

@@ -7,7 +7,7 @@ it implements.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -115,6 +115,197 @@ def gemm(a, b, *, a_lo=None, b_lo=None, a_mn_major=False, b_mn_major=False, one_
          _p(out), _p(out_lo), out.stride(0), flags, epilogue, _p(bias), _p(mask),
          0 if mask is None else mask.stride(0), _stream(stream))
     return out
+
+
+# ---- layer operators: linear + bias + activation + dropout + residual ----------
+class Dropout(NamedTuple):
+    """A dropout draw: probability ``p``, and the ``(seed, offset)`` that fix
+    the mask.  Forward and backward calls with equal values see the same mask
+    (it is recomputed, never stored); a training loop takes a new ``offset``
+    for every layer and step."""
+
+    p: float
+    seed: int
+    offset: int = 0
+
+
+ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
+               "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
+_LAYER_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _layer_check(name: str, t: torch.Tensor, like: torch.Tensor, shape, unit_cols=False) -> None:
+    """``t`` is a CUDA tensor of this shape on ``like``'s device in its dtype
+    (with ``unit_cols``: its last dimension has stride 1)."""
+    if not t.is_cuda or t.device != like.device:
+        raise ValueError(f"{name}: expected a CUDA tensor on {like.device}, got {t.device}")
+    if t.dtype != like.dtype:
+        raise ValueError(f"{name}: expected {like.dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if unit_cols and t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
+        raise ValueError(f"{name}: expected unit stride in the last dimension")
+
+
+def _layer_dtype(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"expected a CUDA tensor, got {t.device}")
+    code = _LAYER_DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {t.dtype}")
+    return code
+
+
+def _drop_spec(spec: _lib.DropoutC, drop: Optional[Dropout]) -> None:
+    if drop is not None:
+        spec.p = drop.p
+        spec.seed = drop.seed & 0xFFFFFFFFFFFFFFFF
+        spec.offset = drop.offset & 0xFFFFFFFFFFFFFFFF
+
+
+def _layer_run(name: str, args, device: torch.device, stream: Optional[int]) -> None:
+    """Calls ``name`` with the workspace it asks for, on ``device``."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _layer_run(name, args, device, stream)
+    need = ctypes.c_size_t()
+    call(name + "_workspace", ctypes.byref(args), ctypes.byref(need))
+    if need.value:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+        if stream is not None:  # the allocator must not hand it out before that stream is done
+            ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
+        args.workspace = ws.data_ptr()
+        args.workspace_bytes = need.value
+    call(name, ctypes.byref(args), _stream(stream))
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row pitch of a 2-D tensor with unit column stride (rows of one row, or
+    of one element, may carry any stride)."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+           act: str = "none", residual: Optional[torch.Tensor] = None,
+           drop: Optional[Dropout] = None, save_pre: bool = False,
+           out: Optional[torch.Tensor] = None, stream: Optional[int] = None):
+    """``residual + dropout(act(x @ w.T + bias))`` in one pass (Linear::forward,
+    src/nn.rs:97-104, with its neighbours in the epilogue).
+
+    ``x`` [M, K] and ``w`` [N, K] in f32, bf16 or f16, any strides (a weight
+    kept as [K, N] is passed as its transpose); ``bias`` [N]; ``residual``
+    [M, N].  ``act`` is one of ``ACTIVATIONS``.  With ``save_pre`` returns
+    ``(out, pre)``, ``pre`` being the pre-activations ``linear_grad`` needs
+    for an activation.  ``out`` may be the residual.
+    """
+    code = _layer_dtype(x)
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError("expected 2-D x and w")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {act!r}")
+    M, K = x.shape
+    N = w.shape[0]
+    _layer_check("w", w, x, (N, K))
+    a = _lib.LinearArgsC(dtype=code, M=M, N=N, K=K, x=x.data_ptr(), x_row=x.stride(0),
+                         x_col=x.stride(1), w=w.data_ptr(), w_row=w.stride(0), w_col=w.stride(1),
+                         act=ACTIVATIONS[act])
+    if bias is not None:
+        _layer_check("bias", bias, x, (N,), True)
+        a.bias = bias.data_ptr()
+    if residual is not None:
+        _layer_check("residual", residual, x, (M, N), True)
+        a.residual, a.ld_residual = residual.data_ptr(), _ld(residual)
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    else:
+        _layer_check("out", out, x, (M, N), True)
+    a.out, a.ld_out = out.data_ptr(), _ld(out)
+    pre = None
+    if save_pre:
+        pre = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        a.pre, a.ld_pre = pre.data_ptr(), N
+    _drop_spec(a.drop, drop)
+    _layer_run("fg_linear", a, x.device, stream)
+    return (out, pre) if save_pre else out
+
+
+def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
+                pre: Optional[torch.Tensor] = None, act: str = "none",
+                drop: Optional[Dropout] = None, need_dx: bool = True, need_dw: bool = True,
+                need_db: bool = True, stream: Optional[int] = None):
+    """``(dx, dw, db)`` of ``linear(x, w, bias, act=act, drop=drop)`` for the
+    gradient ``dy`` of its output; ``pre`` is what ``save_pre`` returned (not
+    needed for ``act="none"``).  Gradients that are not wanted are ``None``.
+    The residual's gradient is ``dy`` itself.  With 16-bit types the gradient
+    at the pre-activations is rounded to that type before the two products."""
+    code = _layer_dtype(x)
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError("expected 2-D x and w")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {act!r}")
+    M, K = x.shape
+    N = w.shape[0]
+    _layer_check("w", w, x, (N, K))
+    _layer_check("dy", dy, x, (M, N))
+    a = _lib.LinearGradArgsC(dtype=code, M=M, N=N, K=K, dy=dy.data_ptr(), dy_row=dy.stride(0),
+                             dy_col=dy.stride(1), x=x.data_ptr(), x_row=x.stride(0),
+                             x_col=x.stride(1), w=w.data_ptr(), w_row=w.stride(0),
+                             w_col=w.stride(1), act=ACTIVATIONS[act])
+    if act != "none":
+        if pre is None:
+            raise ValueError(f"the gradient of {act} needs pre (linear(..., save_pre=True))")
+        _layer_check("pre", pre, x, (M, N), True)
+        a.pre, a.ld_pre = pre.data_ptr(), _ld(pre)
+    dx = dw = db = None
+    if need_dx:
+        dx = torch.empty((M, K), dtype=x.dtype, device=x.device)
+        a.dx, a.ld_dx = dx.data_ptr(), K
+    if need_dw:
+        dw = torch.empty((N, K), dtype=x.dtype, device=x.device)
+        a.dw, a.ld_dw = dw.data_ptr(), K
+    if need_db:
+        db = torch.empty((N,), dtype=x.dtype, device=x.device)
+        a.db = db.data_ptr()
+    _drop_spec(a.drop, drop)
+    _layer_run("fg_linear_grad", a, x.device, stream)
+    return dx, dw, db
+
+
+def dropout(x: torch.Tensor, drop: Optional[Dropout], *, residual: Optional[torch.Tensor] = None,
+            out: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
+    """``residual + dropout(x)`` on the last dimension's columns and the rows
+    before it (a 1-D tensor is one row).  ``out`` may be ``x`` or the residual."""
+    code = _layer_dtype(x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    cols = x.shape[-1] if x.dim() else 1
+    rows = x.numel() // cols if cols else 0
+    ptrs = []
+    for name, t in (("x", x), ("residual", residual), ("out", out)):
+        if t is None:
+            ptrs += [None, 0]
+            continue
+        _layer_check(name, t, x, x.shape, x.dim() > 0)
+        if t.dim() == 2:
+            ptrs += [t.data_ptr(), _ld(t)]
+        elif t.is_contiguous():
+            ptrs += [t.data_ptr(), cols]
+        else:
+            raise ValueError(f"{name}: expected a 2-D or a contiguous tensor")
+    spec = _lib.DropoutC()
+    _drop_spec(spec, drop)
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            call("fg_dropout", code, rows, cols, *ptrs, ctypes.byref(spec), _stream(stream))
+    else:
+        call("fg_dropout", code, rows, cols, *ptrs, ctypes.byref(spec), _stream(stream))
+    return out
+
+
+def dropout_grad(dy: torch.Tensor, drop: Optional[Dropout], *, out: Optional[torch.Tensor] = None,
+                 stream: Optional[int] = None) -> torch.Tensor:
+    """d/dx of ``dropout(x, drop)``: the same mask and scale on ``dy``."""
+    return dropout(dy, drop, out=out, stream=stream)
 
 
 def check_device_error() -> None:

@@ -31,8 +31,10 @@ enum fg_status {
   FG_ERR_UNSUPPORTED = 6 /* shape/layout this build does not handle */
 };
 
-/* dtype codes: src/dtype.rs:19-58 (F32, I32, Bool). */
-enum fg_dtype { FG_F32 = 0, FG_I32 = 1, FG_BOOL = 2 };
+/* dtype codes: src/dtype.rs:19-58 (F32, I32, Bool).  FG_BF16 and FG_F16 have
+ * no counterpart there: the layer operators (fg_linear, fg_linear_grad,
+ * fg_dropout) take them, buffers and the other entry points do not. */
+enum fg_dtype { FG_F32 = 0, FG_I32 = 1, FG_BOOL = 2, FG_BF16 = 3, FG_F16 = 4 };
 
 /* reduce ops: ReduceAxis(Add) / ReduceAxis(Max), src/uop.rs:26-310. */
 enum fg_reduce_op { FG_REDUCE_SUM = 0, FG_REDUCE_MAX = 1 };
@@ -195,6 +197,98 @@ int fg_gemm_3xtf32(int M, int N, int K, const float *d_a, const float *d_a_lo, i
                    const float *d_b, const float *d_b_lo, int ldb, float *d_c, float *d_c_lo,
                    int ldc, int flags, int epilogue, const float *d_bias, const float *d_mask,
                    int ldmask, void *stream);
+
+/* ---- Layer operators (no counterpart in the reference beyond Linear, relu
+ * and their gradients: src/nn.rs:97-104, src/tensor.rs:519-531) -------------
+ * f32, bf16 or f16 (one dtype a call); every sum, activation and mask is
+ * computed in f32 and each output is rounded once, except where stated.
+ * Strides and pitches are in elements, of either sign for inputs; sizes of 0
+ * are allowed (an empty sum is 0).  Work is enqueued on `stream` and nothing
+ * is kept from one call to the next. */
+enum fg_act {
+  FG_ACT_NONE = 0,
+  FG_ACT_RELU = 1,      /* (0 < z) ? z : 0 */
+  FG_ACT_GELU = 2,      /* z Phi(z), Phi the normal distribution function */
+  FG_ACT_GELU_TANH = 3, /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+  FG_ACT_SILU = 4       /* z / (1 + exp(-z)) */
+};
+/* Dropout from a counter-based generator.  t = floor(65536 p + 0.5); element
+ * (m, n) is kept where 16 random bits r16 >= t, and then scaled by
+ * 65536 / (65536 - t); a dropped element is 0 whatever it was.  r16 is 16-bit
+ * piece n % 8 (the low half of each word first) of Philox4x32-10 (Salmon et
+ * al., SC 2011) at the counter words (n / 8, m, offset low, offset high) and
+ * key (seed low, seed high).  The mask is therefore the same wherever it is
+ * computed and is never stored; draws that must differ take different
+ * offsets.  p = 0 turns dropout off, p = 1 drops everything. */
+typedef struct fg_dropout_spec {
+  double p;
+  uint64_t seed, offset;
+} fg_dropout_spec;
+
+/* Linear layer: z = x w^T + bias; out = residual + dropout(act(z)).
+ * x(m, k) = x[m * x_row + k * x_col], w(n, k) likewise (a weight kept as
+ * [K, N] is w_row = 1, w_col = N).  bias [N], residual [M, N] and pre [M, N]
+ * (receives z, for fg_linear_grad) may be NULL; drop.p = 0 for no dropout.
+ * out may be the residual itself (same pointer and pitch); no other output
+ * may overlap an input.  workspace: at least
+ * fg_linear_workspace() bytes of device memory, 256-byte aligned, free for
+ * reuse once the call's work on the stream is done. */
+typedef struct fg_linear_args {
+  int32_t dtype, M, N, K;
+  const void *x;
+  int64_t x_row, x_col;
+  const void *w;
+  int64_t w_row, w_col;
+  const void *bias;
+  const void *residual;
+  int64_t ld_residual;
+  int32_t act, reserved;
+  fg_dropout_spec drop;
+  void *pre;
+  int64_t ld_pre;
+  void *out;
+  int64_t ld_out;
+  void *workspace;
+  size_t workspace_bytes;
+} fg_linear_args;
+int fg_linear_workspace(const fg_linear_args *args, size_t *bytes);
+int fg_linear(const fg_linear_args *args, void *stream);
+
+/* Gradients of a linear layer whose forward call was (x, w, act, drop) and
+ * saved pre, for the gradient dy of its output (the residual's gradient is dy
+ * itself): dz = dropout(dy) act'(pre); dx = dz w [M, K]; dw = dz^T x [N, K];
+ * db = column sums of dz [N].  dx, dw and db may each be NULL (not wanted).
+ * For the 16-bit types dz is rounded to that type before the two products; db is summed from the unrounded dz.  Sums
+ * run in a fixed order: the same inputs give the same bits. */
+typedef struct fg_linear_grad_args {
+  int32_t dtype, M, N, K;
+  const void *dy;
+  int64_t dy_row, dy_col;
+  const void *x;
+  int64_t x_row, x_col;
+  const void *w;
+  int64_t w_row, w_col;
+  const void *pre;
+  int64_t ld_pre;
+  int32_t act, reserved;
+  fg_dropout_spec drop;
+  void *dx;
+  int64_t ld_dx;
+  void *dw;
+  int64_t ld_dw;
+  void *db;
+  void *workspace;
+  size_t workspace_bytes;
+} fg_linear_grad_args;
+int fg_linear_grad_workspace(const fg_linear_grad_args *args, size_t *bytes);
+int fg_linear_grad(const fg_linear_grad_args *args, void *stream);
+
+/* out = residual + dropout(x) over [rows, cols] with row pitches (residual may
+ * be NULL).  Its gradient in x is the same call on dy without a residual.
+ * out may be x or the residual itself. */
+int fg_dropout(int dtype, size_t rows, size_t cols, const void *d_x, int64_t ldx,
+               const void *d_residual, int64_t ldr, void *d_out, int64_t ldo,
+               const fg_dropout_spec *drop, void *stream);
 
 /* ---- MLP training step: forward -> cross_entropy -> backward -> Sgd ----- */
 /* examples/mnist.rs:90-97 on the GPU.  Layers are Linear (src/nn.rs:67-104)
