@@ -68,9 +68,23 @@ __global__ void __launch_bounds__(256)
 // over the rows.  dz may be null (only the sums are wanted).
 // ---------------------------------------------------------------------------
 template <typename T>
+__device__ __forceinline__ void store_dz(void *dz, int64_t at, int64_t, const float (&v)[8]) {
+  store8<T>(static_cast<T *>(dz) + at, v);
+}
+// f32: three bf16 planes, as the products read them
+template <>
+__device__ __forceinline__ void store_dz<float>(void *dz, int64_t at, int64_t plane,
+                                                const float (&v)[8]) {
+  float p[3][8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) split3(v[i], p[0][i], p[1][i], p[2][i]);
+#pragma unroll
+  for (int k = 0; k < 3; k++) store8(static_cast<__nv_bfloat16 *>(dz) + k * plane + at, p[k]);
+}
+template <typename T>
 __global__ void __launch_bounds__(256)
     k_layer_dz(const T *__restrict__ dy, int64_t yr, int64_t yc, const T *__restrict__ pre,
-               int64_t ldp, int act, const DropParams drop, T *__restrict__ dz, int64_t ldz,
+               int64_t ldp, int act, const DropParams drop, void *__restrict__ dz, int64_t ldz,
                float *__restrict__ part, int M, int N, int rows, int vec) {
   __shared__ float red[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -101,15 +115,8 @@ __global__ void __launch_bounds__(256)
       }
 #pragma unroll
       for (int i = 0; i < 8; i++) sum[i] += v[i];
-      if (dz) {
-        if (whole) {
-          store8<T>(dz + r * ldz + col, v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++)
-            if (col + i < N) dz[r * ldz + col + i] = from_f32<T>(v[i]);
-        }
-      }
+      // ldz is a multiple of 8 and the rest of a row's last group is 0
+      if (dz) store_dz<T>(dz, r * ldz + col, (int64_t)M * ldz, v);
     }
   if (!part) return;
 #pragma unroll
@@ -237,16 +244,16 @@ static int run_tile(const Mat &a, const Mat &b, int K, const Epilogue &e, cudaSt
   return FG_OK;
 }
 
-// C = A B^T with an epilogue, by the kernel that fits.
-static int run_product(int dtype, const Mat &a, const Mat &b, int K, const Epilogue &e,
-                       cudaStream_t st) {
+// A K of 0 has nothing to load: the tile kernel's sums are 0.
+static int run_empty_product(int dtype, const Epilogue &e, cudaStream_t st) {
+  const Mat none{};
   switch (dtype) {
     case FG_F32:
-      return run_tile<float>(a, b, K, e, st);
+      return run_tile<float>(none, none, 0, e, st);
     case FG_BF16:
-      return run_tile<__nv_bfloat16>(a, b, K, e, st);
+      return run_tile<__nv_bfloat16>(none, none, 0, e, st);
     default:
-      return run_tile<__half>(a, b, K, e, st);
+      return run_tile<__half>(none, none, 0, e, st);
   }
 }
 
@@ -259,13 +266,26 @@ static int check_common(const char *who, int dtype, int M, int N, int K, int act
   return FG_OK;
 }
 
-static int linear(const fg_linear_args *g, cudaStream_t st) {
+// Where a forward product reads its operands, and the workspace that takes.
+struct LinearPlan {
+  Operand x, w;
+  StageJobs jobs;
+  size_t bytes;
+};
+static LinearPlan plan_linear(const fg_linear_args *g) {
+  LinearPlan p{};
+  if (g->M == 0 || g->N == 0 || g->K == 0) return p;
+  p.x = resolve_operand(g->dtype, {g->x, g->x_row, g->x_col}, g->M, g->K, &p.jobs, &p.bytes);
+  p.w = resolve_operand(g->dtype, {g->w, g->w_row, g->w_col}, g->N, g->K, &p.jobs, &p.bytes);
+  return p;
+}
+
+static int check_linear(const fg_linear_args *g, DropParams *drop) {
   const char *who = "fg_linear";
   FG_REQUIRE(g, "%s: null arguments", who);
   int rc = check_common(who, g->dtype, g->M, g->N, g->K, g->act);
   if (rc) return rc;
-  Epilogue e{};
-  if ((rc = make_drop(who, &g->drop, &e.drop))) return rc;
+  if ((rc = make_drop(who, &g->drop, drop))) return rc;
   if (g->M == 0 || g->N == 0) return FG_OK;
   const int es = elem_size(g->dtype);
   FG_REQUIRE(g->out && (g->K == 0 || (g->x && g->w)), "%s: null operand", who);
@@ -285,6 +305,17 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
   }
   FG_REQUIRE(!overlap(g->out, g->M, g->N, g->ld_out, g->pre, g->M, g->N, g->ld_pre, 1, es),
              "%s: out overlaps pre", who);
+  return FG_OK;
+}
+
+static int linear(const fg_linear_args *g, cudaStream_t st) {
+  Epilogue e{};
+  int rc = check_linear(g, &e.drop);
+  if (rc || g->M == 0 || g->N == 0) return rc;
+  LinearPlan p = plan_linear(g);
+  FG_REQUIRE(g->workspace_bytes >= p.bytes && (p.bytes == 0 || g->workspace),
+             "fg_linear: %zu bytes of workspace needed, got %zu", p.bytes, g->workspace_bytes);
+  const int es = elem_size(g->dtype);
   e.act = g->act;
   e.bias = g->bias;
   e.residual = g->residual;
@@ -297,8 +328,12 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
   e.N = g->N;
   e.vec = rows16(e.bias, 0, es) && rows16(e.residual, e.ldr, es) && rows16(e.pre, e.ldp, es) &&
           rows16(e.out, e.ldo, es);
-  return run_product(g->dtype, {g->x, g->x_row, g->x_col}, {g->w, g->w_row, g->w_col}, g->K, e,
-                     st);
+  if (g->K == 0) return run_empty_product(g->dtype, e, st);
+  place_operand(&p.x, g->workspace);
+  place_operand(&p.w, g->workspace);
+  place_jobs(&p.jobs, g->workspace);
+  if ((rc = run_stage(g->dtype, p.jobs, st))) return rc;
+  return run_tensor_product(g->dtype, p.x, p.w, g->K, e, st);
 }
 
 // Rows of a block of k_layer_dz: about four blocks an SM, at least 64 rows.
@@ -312,70 +347,76 @@ static int dz_rows(int M, int N) {
   return rows;
 }
 
+// dz is written (in a 16-bit type, or as the three planes of f32) where a
+// product reads it and it differs from dy; x and w are read in place or staged.
 struct GradPlan {
-  bool need_dz;     // dz differs from dy, and a product reads it
-  int rows, chunks;
+  bool dx, dw, make_dz;
+  int rows, chunks;   // of k_layer_dz
   int64_t ldz;
   size_t dz_off, part_off, bytes;
+  Operand z_dx, z_dw, w, x;
+  StageJobs jobs;
 };
 static GradPlan plan_grad(const fg_linear_grad_args *g) {
   GradPlan p{};
-  const int es = elem_size(g->dtype);
-  p.need_dz = (g->dx || g->dw) && (g->act != FG_ACT_NONE || g->drop.p > 0.0);
+  p.dx = g->dx && g->K > 0;
+  p.dw = g->dw && g->K > 0;
+  p.make_dz = (p.dx || p.dw) && (g->dtype == FG_F32 || g->act != FG_ACT_NONE || g->drop.p > 0.0);
   p.rows = dz_rows(g->M, g->N);
   p.chunks = (int)((g->M + (int64_t)p.rows - 1) / p.rows);
   p.ldz = (g->N + 7LL) / 8 * 8;
-  size_t at = 0;
   auto take = [&](size_t n) {
-    const size_t o = at;
-    at += (n + 255) / 256 * 256;
+    const size_t o = (p.bytes + 255) / 256 * 256;
+    p.bytes = o + n;
     return o;
   };
-  p.dz_off = take(p.need_dz ? (size_t)g->M * p.ldz * es : 0);
+  const int planes = g->dtype == FG_F32 ? 3 : 1;
+  p.dz_off = take(p.make_dz ? (size_t)planes * g->M * p.ldz * 2 : 0);
   p.part_off = take(g->db ? (size_t)p.chunks * g->N * 4 : 0);
-  p.bytes = at;
+  if (p.make_dz) {
+    p.z_dx.staged_at = p.dz_off;
+    p.z_dx.planes = planes;
+    p.z_dx.inner = g->N, p.z_dx.outer = g->M, p.z_dx.pitch = p.ldz;
+    p.z_dw = p.z_dx;  // read along its rows for dx, across them for dw
+    p.z_dw.mn_major = 1;
+  } else {
+    if (p.dx)
+      p.z_dx = resolve_operand(g->dtype, {g->dy, g->dy_row, g->dy_col}, g->M, g->N, &p.jobs,
+                               &p.bytes);
+    if (p.dx && !p.z_dx.ptr) {  // staged once for both
+      p.z_dw = p.z_dx;
+      p.z_dw.mn_major = !p.z_dx.mn_major;
+    } else if (p.dw) {
+      p.z_dw = resolve_operand(g->dtype, {g->dy, g->dy_col, g->dy_row}, g->N, g->M, &p.jobs,
+                               &p.bytes);
+    }
+  }
+  if (p.dx)
+    p.w = resolve_operand(g->dtype, {g->w, g->w_col, g->w_row}, g->K, g->N, &p.jobs, &p.bytes);
+  if (p.dw)
+    p.x = resolve_operand(g->dtype, {g->x, g->x_col, g->x_row}, g->K, g->M, &p.jobs, &p.bytes);
   return p;
 }
 
 template <typename T>
-static int linear_grad_t(const fg_linear_grad_args *g, const GradPlan &p, const DropParams &drop,
-                         cudaStream_t st) {
+static int run_dz(const fg_linear_grad_args *g, const GradPlan &p, const DropParams &drop,
+                  cudaStream_t st) {
   const int es = sizeof(T);
-  T *dz = p.need_dz ? reinterpret_cast<T *>(static_cast<char *>(g->workspace) + p.dz_off) : nullptr;
-  float *part =
-      g->db ? reinterpret_cast<float *>(static_cast<char *>(g->workspace) + p.part_off) : nullptr;
-  if (dz || part) {
+  char *ws = static_cast<char *>(g->workspace);
+  float *part = g->db ? reinterpret_cast<float *>(ws + p.part_off) : nullptr;
+  if (p.make_dz || part) {
     const int vec = g->dy_col == 1 && rows16(g->dy, g->dy_row, es) &&
                     (g->act == FG_ACT_NONE || rows16(g->pre, g->ld_pre, es));
     k_layer_dz<T><<<dim3((unsigned)((g->N + 255LL) / 256), p.chunks), 256, 0, st>>>(
         static_cast<const T *>(g->dy), g->dy_row, g->dy_col, static_cast<const T *>(g->pre),
-        g->ld_pre, g->act, drop, dz, p.ldz, part, g->M, g->N, p.rows, vec);
+        g->ld_pre, g->act, drop, p.make_dz ? ws + p.dz_off : nullptr, p.ldz, part, g->M, g->N,
+        p.rows, vec);
     FG_LAUNCH_TRY();
   }
   if (g->db) {
     k_bias_grad<T><<<(unsigned)((g->N + 255LL) / 256), 256, 0, st>>>(part, p.chunks, g->N,
                                                                      static_cast<T *>(g->db));
     FG_LAUNCH_TRY();
-  }
-  const Mat z = dz ? Mat{dz, p.ldz, 1} : Mat{g->dy, g->dy_row, g->dy_col};
-  Epilogue e{};
-  if (g->dx && g->K > 0) {  // dx[m, k] = sum_n dz(m, n) w(n, k)
-    e.out = g->dx;
-    e.ldo = g->ld_dx;
-    e.M = g->M;
-    e.N = g->K;
-    e.vec = rows16(e.out, e.ldo, es);
-    int rc = run_product(g->dtype, z, {g->w, g->w_col, g->w_row}, g->N, e, st);
-    if (rc) return rc;
-  }
-  if (g->dw && g->K > 0) {  // dw[n, k] = sum_m dz(m, n) x(m, k)
-    e.out = g->dw;
-    e.ldo = g->ld_dw;
-    e.M = g->N;
-    e.N = g->K;
-    e.vec = rows16(e.out, e.ldo, es);
-    int rc = run_product(g->dtype, {z.ptr, z.col, z.row}, {g->x, g->x_col, g->x_row}, g->M, e, st);
-    if (rc) return rc;
   }
   return FG_OK;
 }
@@ -435,18 +476,44 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
     if ((rc = zero_rows(g->dw, g->ld_dw, g->N, g->K, es, st))) return rc;
     return zero_rows(g->db, g->N, 1, g->N, es, st);
   }
-  const GradPlan p = plan_grad(g);
+  GradPlan p = plan_grad(g);
   FG_REQUIRE(g->workspace_bytes >= p.bytes && (p.bytes == 0 || g->workspace),
              "fg_linear_grad: %zu bytes of workspace needed, got %zu", p.bytes,
              g->workspace_bytes);
+  place_operand(&p.z_dx, g->workspace);
+  place_operand(&p.z_dw, g->workspace);
+  place_operand(&p.w, g->workspace);
+  place_operand(&p.x, g->workspace);
+  place_jobs(&p.jobs, g->workspace);
   switch (g->dtype) {
     case FG_F32:
-      return linear_grad_t<float>(g, p, drop, st);
+      rc = run_dz<float>(g, p, drop, st);
+      break;
     case FG_BF16:
-      return linear_grad_t<__nv_bfloat16>(g, p, drop, st);
+      rc = run_dz<__nv_bfloat16>(g, p, drop, st);
+      break;
     default:
-      return linear_grad_t<__half>(g, p, drop, st);
+      rc = run_dz<__half>(g, p, drop, st);
   }
+  if (rc || (rc = run_stage(g->dtype, p.jobs, st))) return rc;
+  Epilogue e{};
+  if (p.dx) {  // dx[m, k] = sum_n dz(m, n) w(n, k)
+    e.out = g->dx;
+    e.ldo = g->ld_dx;
+    e.M = g->M;
+    e.N = g->K;
+    e.vec = rows16(e.out, e.ldo, es);
+    if ((rc = run_tensor_product(g->dtype, p.z_dx, p.w, g->N, e, st))) return rc;
+  }
+  if (p.dw) {  // dw[n, k] = sum_m dz(m, n) x(m, k)
+    e.out = g->dw;
+    e.ldo = g->ld_dw;
+    e.M = g->N;
+    e.N = g->K;
+    e.vec = rows16(e.out, e.ldo, es);
+    if ((rc = run_tensor_product(g->dtype, p.z_dw, p.x, g->M, e, st))) return rc;
+  }
+  return FG_OK;
 }
 
 static int dropout(int dtype, int64_t rows, int64_t cols, const void *x, int64_t ldx,
@@ -502,6 +569,10 @@ extern "C" int fg_linear(const fg_linear_args *args, void *stream) {
 extern "C" int fg_linear_workspace(const fg_linear_args *args, size_t *bytes) {
   FG_REQUIRE(args && bytes, "fg_linear_workspace: null argument");
   *bytes = 0;
+  fg::layer::DropParams d;
+  int rc = fg::layer::check_linear(args, &d);
+  if (rc) return rc;
+  *bytes = fg::layer::plan_linear(args).bytes;
   return FG_OK;
 }
 

@@ -274,5 +274,54 @@ struct Mat {
   int64_t row, col;
 };
 
+// A product's operand as the tensor-core kernel reads it: 16-bit elements
+// [planes][outer][pitch], `inner` of each row in use.  K-major: outer = rows,
+// inner = k; MN-major: outer = k, inner = rows.
+struct Operand {
+  const void *ptr;   // null until a staged operand is placed in the workspace
+  int64_t inner, outer, pitch;
+  int planes, mn_major;
+  size_t staged_at;
+};
+// One copy into such a layout (k_stage); `at`, dst: its place in the workspace.
+struct StageJob {
+  const void *src;
+  void *dst;
+  int64_t so, si;  // source strides of the outer and inner index
+  int64_t outer, inner, pitch;
+  size_t at;
+  int vec;
+};
+struct StageJobs {
+  StageJob job[3];
+  int n;
+};
+// Describes rows x k elements of m in place, or adds a staging job and grows
+// *ws by its bytes.
+Operand resolve_operand(int dtype, const Mat &m, int64_t rows, int64_t k, StageJobs *jobs,
+                        size_t *ws);
+void place_operand(Operand *o, void *ws);
+void place_jobs(StageJobs *jobs, void *ws);
+int run_stage(int dtype, const StageJobs &jobs, cudaStream_t st);
+
+// How the tensor-core kernel cuts a product up (fg_layer_gemm.cu).
+struct Form {
+  bool pair;
+  int bm, bn, split;
+};
+Form pick_form(int M, int N, int K, int planes, int sms);
+int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, const Epilogue &e,
+                       cudaStream_t st);
+
+// An f32 value as the sum of three bf16 values, each rest exact (an infinity
+// is its own first part; a value that would round up to infinity is cut).
+__device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
+  a = __bfloat162float(__float2bfloat16_rn(v));
+  if (isinf(a) && !isinf(v)) a = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  const float r = isinf(v) ? 0.0f : v - a;
+  b = __bfloat162float(__float2bfloat16_rn(r));
+  c = r - b;
+}
+
 }  // namespace layer
 }  // namespace fg

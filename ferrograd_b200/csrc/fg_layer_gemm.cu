@@ -1,0 +1,659 @@
+// The layer's matrix products on the sm_100a tensor cores (tcgen05 + TMEM,
+// operands by TMA):  C[m, n] = sum_k A(m, k) B(n, k), then the epilogue of
+// fg_layer.cuh in the same kernel.
+//
+// 16-bit operands are read in place where TMA can describe them (one stride
+// 1, the other and the base on 16-byte boundaries); others are first copied to
+// an aligned layout (k_stage).  f32 operands are split into three bf16 planes,
+// x = x0 + x1 + x2 with each rest exact, and a product runs as the six bf16
+// products whose size is at least 2^-16 of the largest; what is dropped is
+// below 2^-24 of a product.
+//
+// The tensor cores truncate each addition to their f32 accumulator, so a long
+// chain drifts towards 0.  A chain is therefore cut after `chain` k-blocks and
+// the epilogue warps add the chains' sums, rounded to nearest, in registers
+// while the next chain runs in the other TMEM buffer.  For f32 a chain is 64
+// deep and adds its five small products first, so that only four additions
+// meet a large accumulator.
+//
+// Two forms, chosen by pick_form:
+//  pair   two CTAs (cta_group::2) on a 256 x 256 tile, persistent.  Each loads
+//         128 rows of A and half of B, so an SM reads 64 bytes of shared
+//         memory a cycle for its MMAs where a lone 128 x 256 CTA reads 96.
+//  split  one CTA a 128 x BN tile, with k split over a cluster of up to 8 CTAs
+//         that add their sums through distributed shared memory in rank order:
+//         for few rows or few tiles.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_runtime.h>
+
+#include <math.h>
+
+#include <mutex>
+
+#include "fg_internal.h"
+#include "fg_layer.cuh"
+#include "fg_ptx.cuh"
+
+namespace fg {
+namespace layer {
+
+using namespace fg::ptx;
+
+constexpr int kMaxStages = 16;
+constexpr unsigned kErrLayer = 5u << 16;  // device error word: role 5
+
+// How an operand's tile lies in shared memory.  K-major: rows of BK elements
+// (128- or 64-byte swizzle, 8-row atoms); MN-major: chunks of 64 rows, each BK
+// k-rows of 128 bytes (128-byte swizzle, 8-k-row atoms).
+struct OperandLayout {
+  int mn_major;
+  int rows;  // rows loaded a CTA (a multiple of 16; of 64 when MN-major)
+};
+
+struct ProductArgs {
+  int M, N, nk;      // nk: k-blocks
+  int chain;         // k-blocks of one accumulation chain
+  int stages, split;
+  int bf16;
+  OperandLayout a, b;
+  unsigned int *err;
+};
+
+template <int PLANES>
+struct Depth {
+  static constexpr int BK = PLANES == 3 ? 32 : 64;
+};
+
+template <int PLANES>
+__device__ __forceinline__ uint64_t desc_base(bool mn_major) {
+  constexpr int BK = Depth<PLANES>::BK;
+  return mn_major ? smem_desc(0, BK * 128, 1024, kLayoutSw128)
+                  : smem_desc(0, 16, 8 * BK * 2, BK == 64 ? kLayoutSw128 : kLayoutSw64);
+}
+
+// Tile index -> (m block, n block), row blocks fastest in groups of `group`
+// rows, so that the tiles in flight share panels of both operands in L2.
+__device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int group, int &mb,
+                                        int &nb) {
+  const int per = group * num_n;
+  const int g = tile / per;
+  const int first = g * group;
+  const int gm = min(group, num_m - first);
+  const int r = tile - g * per;
+  mb = first + r % gm;
+  nb = r / gm;
+}
+
+constexpr int kSlabCols = 16, kSlabPitch = 20;  // floats; a warp's 32 x 16 transpose slab
+
+template <typename T, int PLANES, int CG, int BN>
+__global__ void __launch_bounds__(CG == 2 ? 384 : 192, 1)
+    k_layer_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb,
+                    const ProductArgs g, const Epilogue e) {
+  constexpr int BK = Depth<PLANES>::BK;
+  constexpr int kFirstEpi = CG == 2 ? 4 : 2;   // first epilogue warp
+  constexpr int kEpiWarps = CG == 2 ? 8 : 4;
+  constexpr int COLS = BN * 4 / kEpiWarps;     // accumulator columns of an epilogue thread
+  constexpr int BM = 128 * CG;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t *smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem);
+  uint64_t *empty = full + kMaxStages;
+  uint64_t *tmem_full = empty + kMaxStages;
+  uint64_t *tmem_empty = tmem_full + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tmem_empty + 2);
+  uint8_t *ring = smem + 1024;
+  const uint32_t a_bytes = g.a.rows * (BK * 2), b_bytes = g.b.rows * (BK * 2);
+  const uint32_t stage_bytes = PLANES * (a_bytes + b_bytes);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = CG == 1 || rank == 0;
+  const int num_m = (g.M + BM - 1) / BM, num_n = (g.N + BN - 1) / BN;
+  const int S = g.stages;
+
+  // This CTA's work: whole tiles (pair), or one tile's share of k (split).
+  const int first = CG == 2 ? blockIdx.x / 2 : blockIdx.x / g.split;
+  const int step = CG == 2 ? gridDim.x / 2 : num_m * num_n;
+  const int k0 = CG == 2 ? 0 : (int)((long long)g.nk * rank / g.split);
+  const int k1 = CG == 2 ? g.nk : (int)((long long)g.nk * (rank + 1) / g.split);
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < S; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&tmem_full[i], 1);
+      mbar_init(&tmem_empty[i], CG * kEpiWarps);  // one arrival a warp, from both CTAs
+    }
+    fence_mbar_init();
+    prefetch_tmap(&tma);
+    prefetch_tmap(&tmb);
+  }
+  if (warp == 1) tmem_alloc_cg<CG>(tmem_slot, 2 * BN);
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync_all();  // the peer's barriers and TMEM are ready
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // Pair: 384 threads x 168 registers at launch, of which the epilogue takes
+  // 256 x 224 and the others keep 128 x 56.
+  if (warp < kFirstEpi) {
+    if (CG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 && lane == 0) {
+      // ---------------- TMA producer ----------------
+      int s = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < num_m * num_n; tile += step) {
+        int mb, nb;
+        tile_at(tile, num_m, num_n, 8, mb, nb);
+        const int m0 = mb * BM + (CG == 2 ? 128 * (int)rank : 0);
+        const int n0 = nb * BN + (CG == 2 ? (BN / 2) * (int)rank : 0);
+        for (int kb = k0; kb < k1; kb++, it++) {
+          if (it >= S) {
+            ok = mbar_wait(&empty[s], phase ^ 1, g.err, kErrLayer | 1);
+            if (!ok) break;
+          }
+          const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
+          if (leader) mbar_arrive_expect_tx(&full[s], CG * stage_bytes);
+          uint32_t dst = smem_u32(ring + s * stage_bytes);
+          auto load = [&](const CUtensorMap *map, const OperandLayout &o, int r0, uint32_t bytes) {
+            for (int p = 0; p < PLANES; p++) {
+              const int parts = o.mn_major ? o.rows / 64 : 1;
+              for (int c = 0; c < parts; c++) {
+                const int x = o.mn_major ? r0 + 64 * c : kb * BK;
+                const int y = o.mn_major ? kb * BK : r0;
+                const uint32_t d = dst + c * (BK * 128);
+                if (CG == 2)
+                  tma_load_3d_pair(d, map, bar, x, y, p);
+                else
+                  tma_load_3d(ring + (d - smem_u32(ring)), map, &full[s], x, y, p);
+              }
+              dst += bytes;
+            }
+          };
+          load(&tma, g.a, m0, a_bytes);
+          load(&tmb, g.b, n0, b_bytes);
+          if (++s == S) s = 0, phase ^= 1;
+        }
+      }
+      // After a wait that gave up, loads in flight land before the CTA may
+      // end: the leader sees them on its barriers; the peer, whose loads
+      // complete on the leader's, lets a millisecond pass.
+      if (!ok && leader)
+        for (int i = it - S < 0 ? 0 : it - S; i < it; i++)
+          mbar_wait(&full[i % S], (i / S) & 1, nullptr, 0);
+      else if (!ok)
+        for (const long long t0 = clock64(); clock64() - t0 < 2000000;) __nanosleep(1000);
+    } else if (warp == 1 && lane == 0 && leader) {
+      // ---------------- MMA issuer ----------------
+      const uint32_t idesc = idesc_f16(BM, BN, g.bf16, g.a.mn_major, g.b.mn_major);
+      const uint64_t da0 = desc_base<PLANES>(g.a.mn_major), db0 = desc_base<PLANES>(g.b.mn_major);
+      // 16 elements further in k: 32 bytes inside a swizzled row, or 16 k-rows
+      const uint32_t a_step = (g.a.mn_major ? 2048 : 32) >> 4, b_step = (g.b.mn_major ? 2048 : 32) >> 4;
+      int s = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < num_m * num_n; tile += step)
+        for (int c0 = k0; ok && c0 < k1; c0 += g.chain, local++) {
+          const int c1 = min(c0 + g.chain, k1);
+          const int buf = local & 1;
+          if (local >= 2) {
+            ok = mbar_wait(&tmem_empty[buf], ((local >> 1) - 1) & 1, g.err, kErrLayer | 2);
+            if (!ok) break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem_base + buf * BN;
+          uint32_t acc = 0;
+          const int s_first = s;
+          auto products = [&](int st, int pa, int pb) {
+            // a descriptor holds the 18 low bits of an address (those above
+            // name the CTA within its cluster)
+            const uint32_t base = (smem_u32(ring) & 0x3ffffu) + st * stage_bytes;
+            const uint64_t da = da0 + ((base + pa * a_bytes) >> 4);
+            const uint64_t db = db0 + ((base + PLANES * a_bytes + pb * b_bytes) >> 4);
+#pragma unroll
+            for (int k = 0; k < BK / 16; k++) {
+              mma_f16<CG>(d, da + k * a_step, db + k * b_step, idesc, acc);
+              acc = 1;
+            }
+          };
+          for (int kb = c0; kb < c1; kb++) {
+            ok = mbar_wait(&full[s], phase, g.err, kErrLayer | 3);
+            if (!ok) break;
+            tc_fence_after();
+            if (PLANES == 1) {
+              products(s, 0, 0);
+              CG == 2 ? mma_commit_pair(&empty[s]) : mma_commit(&empty[s]);
+            } else {  // the small products of the whole chain first
+              products(s, 2, 0);
+              products(s, 0, 2);
+              products(s, 1, 1);
+              products(s, 1, 0);
+              products(s, 0, 1);
+            }
+            if (++s == S) s = 0, phase ^= 1;
+          }
+          if (PLANES == 3 && ok) {
+            int t = s_first;
+            for (int kb = c0; kb < c1; kb++) {
+              products(t, 0, 0);
+              CG == 2 ? mma_commit_pair(&empty[t]) : mma_commit(&empty[t]);
+              if (++t == S) t = 0;
+            }
+          }
+          if (ok) CG == 2 ? mma_commit_pair(&tmem_full[buf]) : mma_commit(&tmem_full[buf]);
+        }
+    }
+  } else {
+    if (CG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // ---------------- epilogue ----------------
+    const int q = warp & 3;  // the TMEM lanes this warp may read
+    const int half = (warp - kFirstEpi) / 4;
+    const uint32_t t_addr = tmem_base + ((uint32_t)(32 * q) << 16) + half * COLS;
+    const uint32_t lead_empty0 = CG == 2 ? map_to_rank(smem_u32(&tmem_empty[0]), 0) : 0;
+    int local = 0;
+    bool dead = false;  // a wait gave up: touch nothing more, but keep every barrier
+    for (int tile = first; tile < num_m * num_n; tile += step) {
+      int mb, nb;
+      tile_at(tile, num_m, num_n, 8, mb, nb);
+      float run[COLS];
+#pragma unroll
+      for (int j = 0; j < COLS; j++) run[j] = 0.0f;
+      for (int c0 = k0; c0 < k1; c0 += g.chain, local++) {
+        const int buf = local & 1;
+        if (!dead && !mbar_wait(&tmem_full[buf], (local >> 1) & 1, g.err, kErrLayer | 4))
+          dead = true;
+        dead = __any_sync(0xffffffffu, dead);
+        if (!dead) {
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < COLS; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(t_addr + buf * BN + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j++) run[c + j] += __uint_as_float(r[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2)
+              mbar_arrive_cluster(lead_empty0 + buf * 8);
+            else
+              mbar_arrive_local(&tmem_empty[buf]);
+          }
+        }
+      }
+      if (CG == 2) {
+        if (dead) continue;
+        // 16 columns at a time through the warp's slab, so that lanes hold
+        // eight neighbouring columns and pairs of lanes a row's 16
+        float *slab = reinterpret_cast<float *>(ring + S * stage_bytes) +
+                      (warp - kFirstEpi) * (32 * kSlabPitch);
+        const int row0 = mb * BM + 128 * (int)rank + 32 * q;
+        const int col0 = nb * BN + half * COLS;
+        if (row0 >= g.M) continue;
+#pragma unroll 1
+        for (int c = 0; c < COLS / kSlabCols; c++) {
+          if (col0 + c * kSlabCols >= g.N) break;
+          __syncwarp();
+#pragma unroll
+          for (int cc = 0; cc < COLS / kSlabCols; cc++)
+            if (cc == c) {
+#pragma unroll
+              for (int j = 0; j < kSlabCols; j += 4)
+                *reinterpret_cast<float4 *>(slab + lane * kSlabPitch + j) =
+                    make_float4(run[cc * kSlabCols + j], run[cc * kSlabCols + j + 1],
+                                run[cc * kSlabCols + j + 2], run[cc * kSlabCols + j + 3]);
+            }
+          __syncwarp();
+#pragma unroll 1
+          for (int p = 0; p < 2; p++) {
+            const int r = p * 16 + lane / 2, cg = (lane & 1) * 8;
+            const int row = row0 + r, col = col0 + c * kSlabCols + cg;
+            if (row < g.M && col < g.N) {
+              float v[8];
+              load8<float>(slab + r * kSlabPitch + cg, v);
+              epilogue8<T>(e, row, col, v);
+            }
+          }
+        }
+      } else {
+        // the whole tile's sums to shared memory (the ring is free: every
+        // load was waited for, every MMA has completed)
+        float *sums = reinterpret_cast<float *>(ring) + (32 * q + lane) * (BN + 4);
+        if (!dead) {
+#pragma unroll
+          for (int j = 0; j < COLS; j += 4)
+            *reinterpret_cast<float4 *>(sums + j) =
+                make_float4(run[j], run[j + 1], run[j + 2], run[j + 3]);
+        }
+      }
+    }
+  }
+
+  if (CG == 1) {
+    __syncwarp();
+    cluster_sync_all();
+    // The cluster's CTAs share out the tile's groups of eight columns; each
+    // adds its groups' sums in rank order and applies the epilogue.
+    int mb, nb;
+    tile_at(first, num_m, num_n, 8, mb, nb);
+    const int rows = min(128, g.M - mb * BM);
+    const int groups = rows * (BN / 8);
+    const int lo = (int)((long long)groups * rank / g.split);
+    const int hi = (int)((long long)groups * (rank + 1) / g.split);
+    const uint32_t sums = smem_u32(ring);
+    for (int i = lo + (int)threadIdx.x; i < hi; i += 192) {
+      const int r = i / (BN / 8), cg = (i % (BN / 8)) * 8;
+      const int col = nb * BN + cg;
+      if (col >= g.N) continue;
+      float v[8] = {};
+      const uint32_t at = sums + (r * (BN + 4) + cg) * 4;
+      for (int k = 0; k < g.split; k++) {
+        const uint32_t peer = map_to_rank(at, k);
+        const float4 x = ld_cluster_f4(peer), y = ld_cluster_f4(peer + 16);
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+      }
+      epilogue8<T>(e, mb * BM + r, col, v);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while another may still reach its memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_cg<CG>(tmem_base, 2 * BN);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Operands TMA cannot read in place: copied to [plane][outer][pitch] with
+// the contiguous direction innermost; f32 as three bf16 planes.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void stage8(const T *src, int64_t so, int64_t si, int64_t o, int64_t i,
+                                       int64_t inner, bool vec, uint4 *dst, int64_t plane16) {
+  float v[8];
+  if (vec && i + 8 <= inner) {
+    if (sizeof(T) == 2) {
+      dst[0] = *reinterpret_cast<const uint4 *>(src + o * so + i);
+      return;
+    }
+    load8<T>(src + o * so + i, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = i + j < inner ? to_f32<T>(src[o * so + (i + j) * si]) : 0.0f;
+  }
+  if (sizeof(T) == 2) {
+    store8<T>(reinterpret_cast<T *>(dst), v);
+  } else {
+    float p[3][8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) split3(v[j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+      store8<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16 *>(dst + k * plane16), p[k]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_stage(const StageJobs jobs) {
+  const StageJob &j = jobs.job[blockIdx.y];
+  const int64_t groups = j.pitch / 8, all = groups * j.outer;
+  const T *src = static_cast<const T *>(j.src);
+  uint4 *dst = static_cast<uint4 *>(j.dst);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t o = i / groups, x = (i - o * groups) * 8;
+    stage8<T>(src, j.so, j.si, o, x, j.inner, j.vec, dst + i, groups * j.outer);
+  }
+}
+
+int run_stage(int dtype, const StageJobs &jobs, cudaStream_t st) {
+  if (jobs.n == 0) return FG_OK;
+  int64_t most = 0;
+  for (int i = 0; i < jobs.n; i++) {
+    const int64_t all = jobs.job[i].pitch / 8 * jobs.job[i].outer;
+    if (all > most) most = all;
+  }
+  const int64_t want = (most + 255) / 256;
+  const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8), jobs.n);
+  if (dtype == FG_F32)
+    k_stage<float><<<grid, 256, 0, st>>>(jobs);
+  else if (dtype == FG_BF16)
+    k_stage<__nv_bfloat16><<<grid, 256, 0, st>>>(jobs);
+  else
+    k_stage<__half><<<grid, 256, 0, st>>>(jobs);
+  FG_LAUNCH_TRY();
+  return FG_OK;
+}
+
+Operand resolve_operand(int dtype, const Mat &m, int64_t rows, int64_t k, StageJobs *jobs,
+                        size_t *ws) {
+  Operand o{};
+  o.planes = dtype == FG_F32 ? 3 : 1;
+  const bool base = (uintptr_t)m.ptr % 16 == 0;
+  auto pitch_ok = [](int64_t ld, int64_t outer) { return outer == 1 || (ld > 0 && ld % 8 == 0); };
+  if (dtype != FG_F32 && base && (m.col == 1 || k == 1) && pitch_ok(m.row, rows)) {
+    o.ptr = m.ptr;
+    o.inner = k, o.outer = rows;
+    o.pitch = rows == 1 ? (k + 7) / 8 * 8 : m.row;
+    return o;
+  }
+  if (dtype != FG_F32 && base && (m.row == 1 || rows == 1) && pitch_ok(m.col, k)) {
+    o.ptr = m.ptr;
+    o.mn_major = 1;
+    o.inner = rows, o.outer = k;
+    o.pitch = k == 1 ? (rows + 7) / 8 * 8 : m.col;
+    return o;
+  }
+  // staged with the source's contiguous direction innermost
+  StageJob j{};
+  o.mn_major = m.col != 1 && m.row == 1;
+  o.inner = o.mn_major ? rows : k;
+  o.outer = o.mn_major ? k : rows;
+  o.pitch = (o.inner + 7) / 8 * 8;
+  o.staged_at = (*ws + 255) / 256 * 256;
+  *ws = o.staged_at + (size_t)o.planes * o.outer * o.pitch * 2;
+  j.src = m.ptr;
+  j.so = o.mn_major ? m.col : m.row;
+  j.si = o.mn_major ? m.row : m.col;
+  j.outer = o.outer, j.inner = o.inner, j.pitch = o.pitch;
+  const int es = dtype == FG_F32 ? 4 : 2;
+  j.vec = j.si == 1 && base && (j.so * es) % 16 == 0;
+  j.at = o.staged_at;
+  jobs->job[jobs->n++] = j;
+  return o;
+}
+
+void place_operand(Operand *o, void *ws) {
+  if (!o->ptr) o->ptr = static_cast<char *>(ws) + o->staged_at;
+}
+void place_jobs(StageJobs *jobs, void *ws) {
+  for (int i = 0; i < jobs->n; i++) jobs->job[i].dst = static_cast<char *>(ws) + jobs->job[i].at;
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void *ptr = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = (PFN_cuTensorMapEncodeTiled_v12000)ptr;
+  });
+  return fn;
+}
+
+// [planes][outer][pitch] of 16-bit elements; one box is box_rows K-major rows
+// of BK elements, or BK k-rows of 64 MN-major elements.
+static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bool bf16) {
+  auto fn = encode_fn();
+  if (!fn) return set_error(FG_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t pitch = (cuuint64_t)o.pitch * 2;
+  const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.outer, (cuuint64_t)o.planes};
+  const cuuint64_t strides[2] = {pitch, pitch * (cuuint64_t)o.outer};
+  const cuuint32_t box[3] = {(cuuint32_t)(o.mn_major ? 64 : bk),
+                             (cuuint32_t)(o.mn_major ? bk : box_rows), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      const_cast<void *>(o.ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      o.mn_major || bk == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(FG_ERR_CUDA,
+                     "cuTensorMapEncodeTiled failed (%d): inner=%lld outer=%lld pitch=%lld", (int)r,
+                     (long long)o.inner, (long long)o.outer, (long long)o.pitch);
+  return FG_OK;
+}
+
+// Shared memory a CTA must ask for so that the CTAs that fit on an SM never
+// need more than its 512 TMEM columns between them: an allocation that had to
+// wait while its cluster's other CTAs hold theirs could wait for ever.
+static size_t tmem_share(int cols) { return (size_t)cols / 128 * 47 * 1024; }
+
+template <typename T, int PLANES, int CG, int BN>
+static int launch(const CUtensorMap &ta, const CUtensorMap &tb, ProductArgs g, const Epilogue &e,
+                  int ctas, size_t ring_cap, cudaStream_t st) {
+  constexpr int BK = Depth<PLANES>::BK;
+  auto kern = k_layer_product<T, PLANES, CG, BN>;
+  const size_t stage = (size_t)PLANES * (g.a.rows + g.b.rows) * BK * 2;
+  // past the ring: the pair's slabs, or what an MMA of 128 rows reads beyond
+  // an A tile of fewer (it lands in unused accumulator rows)
+  const size_t tail = CG == 2 ? 8 * 32 * kSlabPitch * 4 : 128 * BK * 2;
+  int64_t stages = (int64_t)(ring_cap / stage);
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (CG == 1) {
+    const int64_t per = (g.nk + g.split - 1) / g.split;
+    if (stages > per) stages = per;
+  }
+  const int64_t least = PLANES == 3 ? 2 : 1;  // an f32 chain holds two k-blocks at once
+  if (stages < least) stages = least;
+  g.stages = (int)stages;
+  size_t bytes = stages * stage + tail;
+  const size_t sums = (size_t)128 * (BN + 4) * 4;
+  if (CG == 1 && bytes < sums) bytes = sums;
+  bytes += 2048;  // barriers, alignment
+  if (bytes < tmem_share(2 * BN)) bytes = tmem_share(2 * BN);
+  static bool attr_done[64] = {};
+  int dev = 0;
+  FG_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+    FG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     227 * 1024));
+    if (dev >= 0 && dev < 64) attr_done[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(CG == 2 ? 384 : 192);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG == 2 ? 2 : g.split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ta, tb, g, e));
+  count_launch();
+  return FG_OK;
+}
+
+template <typename T, int PLANES>
+static int run_form(const Form &f, const CUtensorMap &ta, const CUtensorMap &tb, ProductArgs g,
+                    const Epilogue &e, int sms, cudaStream_t st) {
+  const int64_t tiles = (int64_t)((g.M + f.bm - 1) / f.bm) * ((g.N + f.bn - 1) / f.bn);
+  if (f.pair) {
+    const int pairs = sms / 2;
+    const int ctas = 2 * (int)(tiles < pairs ? tiles : pairs);
+    return launch<T, PLANES, 2, 256>(ta, tb, g, e, ctas, 192 * 1024, st);
+  }
+  const int64_t ctas = tiles * f.split;
+  // more CTAs than SMs: two to an SM, so that one computes while the other joins
+  const size_t cap = ctas > sms ? 92 * 1024 : 190 * 1024;
+  if (f.bn == 128) return launch<T, PLANES, 1, 128>(ta, tb, g, e, (int)ctas, cap, st);
+  return launch<T, PLANES, 1, 64>(ta, tb, g, e, (int)ctas, cap, st);
+}
+
+int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, const Epilogue &e,
+                       cudaStream_t st) {
+  DevCtx *ctx = ctx_current();
+  if (!ctx) return set_error(FG_ERR_CUDA, "no CUDA device context");
+  const int sms = ctx->num_sms ? ctx->num_sms : 148;
+  const int planes = dtype == FG_F32 ? 3 : 1;
+  const bool bf16 = dtype != FG_F16;
+  const int bk = planes == 3 ? 32 : 64;
+  const Form f = pick_form(e.M, e.N, K, planes, sms);
+  ProductArgs g{};
+  g.M = e.M;
+  g.N = e.N;
+  g.nk = (int)((K + (int64_t)bk - 1) / bk);
+  g.chain = planes == 3 ? 2 : 32;
+  g.split = f.split;
+  g.bf16 = bf16;
+  g.err = ctx->d_err;
+  const int unit_a = a.mn_major ? 64 : 16;
+  g.a.mn_major = a.mn_major;
+  g.a.rows = e.M >= 128 ? 128 : (e.M + unit_a - 1) / unit_a * unit_a;
+  g.b.mn_major = b.mn_major;
+  g.b.rows = f.pair ? 128 : f.bn;
+  if (f.pair) g.a.rows = 128;
+  CUtensorMap ta, tb;
+  int rc = make_map(&ta, a, bk, g.a.rows, bf16);
+  if (rc) return rc;
+  if ((rc = make_map(&tb, b, bk, g.b.rows, bf16))) return rc;
+  switch (dtype) {
+    case FG_F32:
+      return run_form<float, 3>(f, ta, tb, g, e, sms, st);
+    case FG_BF16:
+      return run_form<__nv_bfloat16, 1>(f, ta, tb, g, e, sms, st);
+    default:
+      return run_form<__half, 1>(f, ta, tb, g, e, sms, st);
+  }
+}
+
+// The form with the least estimated time, in MMA cycles of an SM: a k-block
+// costs its MMAs, a tile about 2000 cycles around them (start-up, the last
+// chain's drain, the epilogue), and CTAs run in waves.
+Form pick_form(int M, int N, int K, int planes, int sms) {
+  const double per_k = (planes == 3 ? 6.0 : 1.0) / 16.0;  // MMA steps per k
+  auto waves = [](double n, double slots) { return ceil(n / slots); };
+  Form best{true, 256, 256, 1};
+  const double t2 = ceil(M / 256.0) * ceil(N / 256.0);
+  double cost = waves(t2, sms / 2) * (K * per_k * 128.0) + 6000.0;
+  const int bk = planes == 3 ? 32 : 64;
+  const int nk = (int)((K + (int64_t)bk - 1) / bk);
+  for (int bn = 128; bn >= 64; bn /= 2)
+    for (int split = 1; split <= 8; split *= 2) {
+      if (split > nk) break;
+      const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
+      if (ctas > 1e8) continue;
+      // a lone CTA's MMAs read shared memory faster than it delivers
+      const double step = bn == 128 ? 84.0 : 52.0;
+      const double c = waves(ctas, sms) * ((double)K / split * per_k * step + 2500.0) +
+                       (split > 1 ? 1500.0 : 0.0) + 2000.0;
+      if (c < cost) {
+        cost = c;
+        best = Form{false, 128, bn, split};
+      }
+    }
+  return best;
+}
+
+}  // namespace layer
+}  // namespace fg

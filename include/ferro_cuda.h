@@ -230,7 +230,9 @@ typedef struct fg_dropout_spec {
  * [K, N] is w_row = 1, w_col = N).  bias [N], residual [M, N] and pre [M, N]
  * (receives z, for fg_linear_grad) may be NULL; drop.p = 0 for no dropout.
  * out may be the residual itself (same pointer and pitch); no other output
- * may overlap an input.  workspace: at least
+ * may overlap an input.  Products run on the tensor cores, f32 ones as sums of
+ * bf16 products to f32 accuracy (an infinity in an f32 operand may give NaN
+ * where f32 arithmetic gives infinity).  workspace: at least
  * fg_linear_workspace() bytes of device memory, 256-byte aligned, free for
  * reuse once the call's work on the stream is done. */
 typedef struct fg_linear_args {
