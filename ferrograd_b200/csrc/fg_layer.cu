@@ -105,14 +105,8 @@ __global__ void __launch_bounds__(256)
           z[i] = act != FG_ACT_NONE && col + i < N ? to_f32<T>(pre[r * ldp + col + i]) : 0.0f;
         }
       }
-      if (drop.threshold) drop8(drop, r, col, v);
-      if (act == FG_ACT_RELU) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 0.0f < z[i] ? v[i] : 0.0f;
-      } else if (act != FG_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= act_slope(z[i], act);
-      }
+      if (drop.on) drop8(drop, r, col, v);
+      slope8<sizeof(T) == 2>(v, z, act);
 #pragma unroll
       for (int i = 0; i < 8; i++) sum[i] += v[i];
       // ldz is a multiple of 8 and the rest of a row's last group is 0
@@ -165,7 +159,7 @@ __global__ void __launch_bounds__(256)
         t[i] = residual && col + i < cols ? to_f32<T>(residual[r * ldr + col + i]) : 0.0f;
       }
     }
-    if (drop.threshold) drop8(drop, (uint32_t)r, col, v);
+    if (drop.on) drop8(drop, (uint32_t)r, col, v);
     if (residual) {
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] += t[i];
@@ -191,8 +185,11 @@ static int make_drop(const char *who, const fg_dropout_spec *s, DropParams *d) {
   *d = DropParams{};
   if (!s) return FG_OK;
   FG_REQUIRE(s->p >= 0.0 && s->p <= 1.0, "%s: dropout probability %g is not in [0, 1]", who, s->p);
-  d->threshold = (uint32_t)floor(s->p * 65536.0 + 0.5);
-  d->scale = d->threshold < 65536 ? (float)(65536.0 / (65536 - d->threshold)) : 0.0f;
+  const uint32_t t = (uint32_t)floor(s->p * 65536.0 + 0.5);
+  d->on = t > 0;
+  d->some = t < 65536;
+  d->threshold_hi = t << 16;
+  d->scale = d->some ? (float)(65536.0 / (65536 - t)) : 0.0f;
   d->k0 = (uint32_t)s->seed;
   d->k1 = (uint32_t)(s->seed >> 32);
   d->c2 = (uint32_t)s->offset;

@@ -105,52 +105,135 @@ __device__ __forceinline__ float bound_both(float z, float lim) {
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
 
-__device__ __forceinline__ float act_value(float z, int act) {
+// The f32 forms use CUDA's functions; GELU's Phi from erfc keeps the left
+// tail's digits.  The 16-bit forms end in a rounding to 8 or 11 bits, so they
+// use the hardware's approximate exp2 and reciprocal (2 units of f32) and, for
+// Phi, M. Abramowitz and I. Stegun, "Handbook of Mathematical Functions",
+// 7.1.28: erfc(x) = (1 + a1 x + ... + a6 x^6)^-16 for x >= 0, off by 3e-7 at
+// most.  They are what lets an epilogue of GELU and dropout hide behind a
+// 4096-deep bf16 product (27 instructions an element where erfcf and full
+// divisions take about 90).
+template <bool FAST>
+struct Math;
+template <>
+struct Math<false> {
+  static __device__ __forceinline__ float phi(float z) {
+    return 0.5f * erfcf(z * -0.70710678118654752f);
+  }
+  static __device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
+  static __device__ __forceinline__ float gauss(float z) {  // exp(-z^2 / 2)
+    return expf(-0.5f * z * z);
+  }
+};
+template <>
+struct Math<true> {
+  static __device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  }
+  static __device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  }
+  static __device__ __forceinline__ float phi(float z) {
+    // the polynomial in |z|, its coefficients a_i / 2^(i/2)
+    const float x = fabsf(z);
+    float p = 5.38297500e-06f;
+    p = fmaf(p, x, 4.88906356e-05f);
+    p = fmaf(p, x, 3.80035750e-05f);
+    p = fmaf(p, x, 3.27762632e-03f);
+    p = fmaf(p, x, 2.11410062e-02f);
+    p = fmaf(p, x, 4.98673470e-02f);
+    p = fmaf(p, x, 1.0f);
+    p *= p;
+    p *= p;
+    p *= p;
+    p *= p;
+    const float h = 0.5f * rcp(p);  // Phi(-|z|)
+    return z > 0.0f ? 1.0f - h : h;
+  }
+  static __device__ __forceinline__ float logistic(float z) {
+    return rcp(1.0f + ex2(z * -1.4426950408889634f));
+  }
+  static __device__ __forceinline__ float gauss(float z) {
+    return ex2(z * z * -0.72134752044448170f);
+  }
+};
+
+// v = act(v), elementwise.
+template <bool FAST>
+__device__ __forceinline__ void act8(float (&v)[8], int act) {
+  using F = Math<FAST>;
   switch (act) {
     case FG_ACT_RELU:
-      return 0.0f < z ? z : 0.0f;
-    case FG_ACT_GELU: {  // z * Phi(z); Phi from erfc keeps the left tail's digits
-      const float b = bound_below(z, -16.0f);
-      return b * (0.5f * erfcf(b * -0.70710678118654752f));
-    }
-    case FG_ACT_GELU_TANH: {
-      // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u))
-      const float b = bound_below(z, -16.0f);
-      const float u = kGeluC * (b + kGeluB * b * b * b);
-      return b / (1.0f + expf(-2.0f * u));
-    }
-    case FG_ACT_SILU: {
-      const float b = bound_below(z, -128.0f);
-      return b / (1.0f + expf(-b));
-    }
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = 0.0f < v[i] ? v[i] : 0.0f;
+      break;
+    case FG_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float b = bound_below(v[i], -32.0f);
+        v[i] = b * F::phi(b);
+      }
+      break;
+    case FG_ACT_GELU_TANH:  // (1 + tanh u) / 2 = logistic(2u)
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float b = bound_below(v[i], -32.0f);
+        v[i] = b * F::logistic(b * fmaf(2.0f * kGeluC * kGeluB, b * b, 2.0f * kGeluC));
+      }
+      break;
+    case FG_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float b = bound_below(v[i], -128.0f);
+        v[i] = b * F::logistic(b);
+      }
+      break;
     default:
-      return z;
+      break;
   }
 }
 
-// d act / dz.  Beyond |z| = 16 (GELU) or 104 (SiLU) the slopes are 0 or 1 to
-// every bit of f32.
-__device__ __forceinline__ float act_slope(float z, int act) {
+// v *= act'(z), elementwise.  Beyond |z| = 32 (GELU) or 104 (SiLU) the slopes
+// are 0 or 1 to every bit of f32.  ReLU's slope selects: where z <= 0 the
+// result is 0 whatever v is.
+template <bool FAST>
+__device__ __forceinline__ void slope8(float (&v)[8], const float (&z)[8], int act) {
+  using F = Math<FAST>;
   switch (act) {
     case FG_ACT_RELU:
-      return 0.0f < z ? 1.0f : 0.0f;
-    case FG_ACT_GELU: {
-      const float b = bound_both(z, 16.0f);
-      return 0.5f * erfcf(b * -0.70710678118654752f) +
-             b * (0.3989422804014327f * expf(-0.5f * b * b));
-    }
-    case FG_ACT_GELU_TANH: {
-      const float b = bound_both(z, 16.0f);
-      const float g = 1.0f / (1.0f + expf(-2.0f * kGeluC * (b + kGeluB * b * b * b)));
-      return g + b * g * (1.0f - g) * (2.0f * kGeluC * (1.0f + 3.0f * kGeluB * b * b));
-    }
-    case FG_ACT_SILU: {
-      const float b = bound_both(z, 128.0f);
-      const float s = 1.0f / (1.0f + expf(-b));
-      return s * (1.0f + b * (1.0f - s));
-    }
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = 0.0f < z[i] ? v[i] : 0.0f;
+      break;
+    case FG_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float b = bound_both(z[i], 32.0f);
+        v[i] *= fmaf(b * 0.3989422804014327f, F::gauss(b), F::phi(b));
+      }
+      break;
+    case FG_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float b = bound_both(z[i], 32.0f);
+        const float q = b * b;
+        const float g = F::logistic(b * fmaf(2.0f * kGeluC * kGeluB, q, 2.0f * kGeluC));
+        v[i] *= fmaf(b * g * (1.0f - g), fmaf(6.0f * kGeluC * kGeluB, q, 2.0f * kGeluC), g);
+      }
+      break;
+    case FG_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float b = bound_both(z[i], 128.0f);
+        const float g = F::logistic(b);
+        v[i] *= g * fmaf(b, 1.0f - g, 1.0f);
+      }
+      break;
     default:
-      return 1.0f;
+      break;
   }
 }
 
@@ -161,8 +244,10 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 // so the mask depends on (seed, offset, row, column) alone: not on the type,
 // the strides, or which kernel asks for it.
 struct DropParams {
-  uint32_t threshold;  // keep where the 16 bits are >= threshold; 0: dropout is off
-  float scale;         // 65536 / (65536 - threshold), 0 where everything is dropped
+  int on;                 // the threshold t is not 0
+  int some;               // t < 65536: something is kept
+  uint32_t threshold_hi;  // t << 16 (some)
+  float scale;            // 65536 / (65536 - t)
   uint32_t k0, k1;     // seed
   uint32_t c2, c3;     // offset
 };
@@ -171,12 +256,11 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
                                         uint32_t k0, uint32_t k1) {
 #pragma unroll
   for (int r = 0; r < 10; r++) {
-    const uint32_t h0 = __umulhi(0xD2511F53u, c0), l0 = 0xD2511F53u * c0;
-    const uint32_t h1 = __umulhi(0xCD9E8D57u, c2), l1 = 0xCD9E8D57u * c2;
-    c0 = h1 ^ c1 ^ k0;
-    c1 = l1;
-    c2 = h0 ^ c3 ^ k1;
-    c3 = l0;
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)p1;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)p0;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
@@ -187,12 +271,18 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
 // a row.  A dropped element is exactly 0, whatever it was (NaN included).
 __device__ __forceinline__ void drop8(const DropParams &d, uint32_t row, uint32_t col,
                                       float (&v)[8]) {
+  if (!d.some) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = 0.0f;
+    return;
+  }
   const uint4 r = philox(col >> 3, row, d.c2, d.c3, d.k0, d.k1);
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  // r16 >= t, with r16 in the upper half of a word and anything below it
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    v[2 * i] = (w[i] & 0xffffu) >= d.threshold ? v[2 * i] * d.scale : 0.0f;
-    v[2 * i + 1] = (w[i] >> 16) >= d.threshold ? v[2 * i + 1] * d.scale : 0.0f;
+    v[2 * i] = (w[i] << 16) >= d.threshold_hi ? v[2 * i] * d.scale : 0.0f;
+    v[2 * i + 1] = w[i] >= d.threshold_hi ? v[2 * i + 1] * d.scale : 0.0f;
   }
 }
 
@@ -240,11 +330,8 @@ __device__ __forceinline__ void epilogue8(const Epilogue &e, int row, int col, f
         if (i < n) p[i] = from_f32<T>(v[i]);
     }
   }
-  if (e.act != FG_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = act_value(v[i], e.act);
-  }
-  if (e.drop.threshold) drop8(e.drop, row, col, v);
+  act8<sizeof(T) == 2>(v, e.act);
+  if (e.drop.on) drop8(e.drop, row, col, v);
   if (e.residual) {
     const T *r = static_cast<const T *>(e.residual) + (int64_t)row * e.ldr + col;
     if (vec) {

@@ -41,6 +41,10 @@ namespace layer {
 using namespace fg::ptx;
 
 constexpr int kMaxStages = 16;
+// k-blocks of a chain of 16-bit products: 16384 deep, 1024 truncated additions
+// of 2^-24 of the sum each at most.  Outputs of 8 or 11 bits do not show that
+// (f16 rounds by up to 2^-11).
+constexpr int kChain16 = 256;
 constexpr unsigned kErrLayer = 5u << 16;  // device error word: role 5
 
 // How an operand's tile lies in shared memory.  K-major: rows of BK elements
@@ -87,13 +91,23 @@ __device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int grou
 
 constexpr int kSlabCols = 16, kSlabPitch = 20;  // floats; a warp's 32 x 16 transpose slab
 
-template <typename T, int PLANES, int CG, int BN>
-__global__ void __launch_bounds__(CG == 2 ? 384 : 192, 1)
+// The block of each form.  RUN: the epilogue warps keep the running sums of the
+// chains in registers; without it a product is one chain and they read the
+// accumulator where they need it, which leaves registers for twice the warps.
+template <int CG, bool RUN>
+struct Block {
+  static constexpr int first_epi = CG == 2 ? 4 : 2;
+  static constexpr int epi_warps = CG == 1 ? 4 : RUN ? 8 : 16;
+  static constexpr int threads = 32 * (first_epi + epi_warps);
+};
+
+template <typename T, int PLANES, int CG, int BN, bool RUN>
+__global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
     k_layer_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb,
                     const ProductArgs g, const Epilogue e) {
   constexpr int BK = Depth<PLANES>::BK;
-  constexpr int kFirstEpi = CG == 2 ? 4 : 2;   // first epilogue warp
-  constexpr int kEpiWarps = CG == 2 ? 8 : 4;
+  constexpr int kFirstEpi = Block<CG, RUN>::first_epi;  // first epilogue warp
+  constexpr int kEpiWarps = Block<CG, RUN>::epi_warps;
   constexpr int COLS = BN * 4 / kEpiWarps;     // accumulator columns of an epilogue thread
   constexpr int BM = 128 * CG;
   extern __shared__ uint8_t smem_raw[];
@@ -140,10 +154,10 @@ __global__ void __launch_bounds__(CG == 2 ? 384 : 192, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  // Pair: 384 threads x 168 registers at launch, of which the epilogue takes
+  // Pair with running sums: 384 threads x 168 registers at launch, of which the epilogue takes
   // 256 x 224 and the others keep 128 x 56.
   if (warp < kFirstEpi) {
-    if (CG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (CG == 2 && RUN) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && lane == 0) {
       // ---------------- TMA producer ----------------
       int s = 0, it = 0;
@@ -251,54 +265,90 @@ __global__ void __launch_bounds__(CG == 2 ? 384 : 192, 1)
         }
     }
   } else {
-    if (CG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if (CG == 2 && RUN) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ---------------- epilogue ----------------
     const int q = warp & 3;  // the TMEM lanes this warp may read
-    const int half = (warp - kFirstEpi) / 4;
-    const uint32_t t_addr = tmem_base + ((uint32_t)(32 * q) << 16) + half * COLS;
+    const int part = (warp - kFirstEpi) / 4;  // its columns: COLS of the tile's BN
+    const uint32_t t_addr = tmem_base + ((uint32_t)(32 * q) << 16) + part * COLS;
     const uint32_t lead_empty0 = CG == 2 ? map_to_rank(smem_u32(&tmem_empty[0]), 0) : 0;
     int local = 0;
     bool dead = false;  // a wait gave up: touch nothing more, but keep every barrier
+    auto release = [&](int buf) {  // this warp has read its part of a TMEM buffer
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2)
+          mbar_arrive_cluster(lead_empty0 + buf * 8);
+        else
+          mbar_arrive_local(&tmem_empty[buf]);
+      }
+    };
+    auto arrived = [&](int chain_no) {  // a chain's sums are in its buffer
+      if (!dead && !mbar_wait(&tmem_full[chain_no & 1], (chain_no >> 1) & 1, g.err, kErrLayer | 4))
+        dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      tc_fence_after();
+      return !dead;
+    };
+    // 16 columns of a pair's tile through the warp's slab, so that lanes hold
+    // eight neighbouring columns and two lanes a row's 16: 32-byte sectors
+    float *slab = reinterpret_cast<float *>(ring + S * stage_bytes) +
+                  (warp - kFirstEpi) * (32 * kSlabPitch);
+    auto finish16 = [&](int row0, int col0) {
+      __syncwarp();
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const int r = p * 16 + lane / 2, cg = (lane & 1) * 8;
+        if (row0 + r < g.M && col0 + cg < g.N) {
+          float v[8];
+          load8<float>(slab + r * kSlabPitch + cg, v);
+          epilogue8<T>(e, row0 + r, col0 + cg, v);
+        }
+      }
+    };
     for (int tile = first; tile < num_m * num_n; tile += step) {
       int mb, nb;
       tile_at(tile, num_m, num_n, 8, mb, nb);
+      const int row0 = mb * BM + 128 * (int)rank + 32 * q;  // of a pair
+      const int col0 = nb * BN + part * COLS;
+      if (!RUN) {
+        const int buf = local & 1;
+        if (arrived(local++)) {
+#pragma unroll 1
+          for (int c = 0; c < COLS; c += kSlabCols) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(t_addr + buf * BN + c, r);
+            tmem_ld_wait();
+            if (c + kSlabCols >= COLS) release(buf);
+            if (row0 >= g.M || col0 + c >= g.N) continue;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < kSlabCols; j += 4)
+              *reinterpret_cast<uint4 *>(slab + lane * kSlabPitch + j) =
+                  make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            finish16(row0, col0 + c);
+          }
+        }
+        continue;
+      }
       float run[COLS];
 #pragma unroll
       for (int j = 0; j < COLS; j++) run[j] = 0.0f;
       for (int c0 = k0; c0 < k1; c0 += g.chain, local++) {
-        const int buf = local & 1;
-        if (!dead && !mbar_wait(&tmem_full[buf], (local >> 1) & 1, g.err, kErrLayer | 4))
-          dead = true;
-        dead = __any_sync(0xffffffffu, dead);
-        if (!dead) {
-          tc_fence_after();
+        if (arrived(local)) {
 #pragma unroll
           for (int c = 0; c < COLS; c += 32) {
             uint32_t r[32];
-            tmem_ld_32x32b_x32(t_addr + buf * BN + c, r);
+            tmem_ld_32x32b_x32(t_addr + (local & 1) * BN + c, r);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; j++) run[c + j] += __uint_as_float(r[j]);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (CG == 2)
-              mbar_arrive_cluster(lead_empty0 + buf * 8);
-            else
-              mbar_arrive_local(&tmem_empty[buf]);
-          }
+          release(local & 1);
         }
       }
       if (CG == 2) {
-        if (dead) continue;
-        // 16 columns at a time through the warp's slab, so that lanes hold
-        // eight neighbouring columns and pairs of lanes a row's 16
-        float *slab = reinterpret_cast<float *>(ring + S * stage_bytes) +
-                      (warp - kFirstEpi) * (32 * kSlabPitch);
-        const int row0 = mb * BM + 128 * (int)rank + 32 * q;
-        const int col0 = nb * BN + half * COLS;
-        if (row0 >= g.M) continue;
+        if (dead || row0 >= g.M) continue;
 #pragma unroll 1
         for (int c = 0; c < COLS / kSlabCols; c++) {
           if (col0 + c * kSlabCols >= g.N) break;
@@ -312,17 +362,7 @@ __global__ void __launch_bounds__(CG == 2 ? 384 : 192, 1)
                     make_float4(run[cc * kSlabCols + j], run[cc * kSlabCols + j + 1],
                                 run[cc * kSlabCols + j + 2], run[cc * kSlabCols + j + 3]);
             }
-          __syncwarp();
-#pragma unroll 1
-          for (int p = 0; p < 2; p++) {
-            const int r = p * 16 + lane / 2, cg = (lane & 1) * 8;
-            const int row = row0 + r, col = col0 + c * kSlabCols + cg;
-            if (row < g.M && col < g.N) {
-              float v[8];
-              load8<float>(slab + r * kSlabPitch + cg, v);
-              epilogue8<T>(e, row, col, v);
-            }
-          }
+          finish16(row0, col0 + c * kSlabCols);
         }
       } else {
         // the whole tile's sums to shared memory (the ring is free: every
@@ -526,15 +566,16 @@ static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bo
 // wait while its cluster's other CTAs hold theirs could wait for ever.
 static size_t tmem_share(int cols) { return (size_t)cols / 128 * 47 * 1024; }
 
-template <typename T, int PLANES, int CG, int BN>
+template <typename T, int PLANES, int CG, int BN, bool RUN>
 static int launch(const CUtensorMap &ta, const CUtensorMap &tb, ProductArgs g, const Epilogue &e,
                   int ctas, size_t ring_cap, cudaStream_t st) {
   constexpr int BK = Depth<PLANES>::BK;
-  auto kern = k_layer_product<T, PLANES, CG, BN>;
+  auto kern = k_layer_product<T, PLANES, CG, BN, RUN>;
   const size_t stage = (size_t)PLANES * (g.a.rows + g.b.rows) * BK * 2;
   // past the ring: the pair's slabs, or what an MMA of 128 rows reads beyond
   // an A tile of fewer (it lands in unused accumulator rows)
-  const size_t tail = CG == 2 ? 8 * 32 * kSlabPitch * 4 : 128 * BK * 2;
+  const size_t tail =
+      CG == 2 ? Block<CG, RUN>::epi_warps * 32 * kSlabPitch * 4 : 128 * BK * 2;
   int64_t stages = (int64_t)(ring_cap / stage);
   if (stages > kMaxStages) stages = kMaxStages;
   if (CG == 1) {
@@ -559,7 +600,7 @@ static int launch(const CUtensorMap &ta, const CUtensorMap &tb, ProductArgs g, c
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(CG == 2 ? 384 : 192);
+  cfg.blockDim = dim3(Block<CG, RUN>::threads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -581,13 +622,15 @@ static int run_form(const Form &f, const CUtensorMap &ta, const CUtensorMap &tb,
   if (f.pair) {
     const int pairs = sms / 2;
     const int ctas = 2 * (int)(tiles < pairs ? tiles : pairs);
-    return launch<T, PLANES, 2, 256>(ta, tb, g, e, ctas, 192 * 1024, st);
+    if (PLANES == 1 && g.chain >= g.nk)
+      return launch<T, PLANES, 2, 256, PLANES == 3>(ta, tb, g, e, ctas, 160 * 1024, st);
+    return launch<T, PLANES, 2, 256, true>(ta, tb, g, e, ctas, 192 * 1024, st);
   }
   const int64_t ctas = tiles * f.split;
   // more CTAs than SMs: two to an SM, so that one computes while the other joins
   const size_t cap = ctas > sms ? 92 * 1024 : 190 * 1024;
-  if (f.bn == 128) return launch<T, PLANES, 1, 128>(ta, tb, g, e, (int)ctas, cap, st);
-  return launch<T, PLANES, 1, 64>(ta, tb, g, e, (int)ctas, cap, st);
+  if (f.bn == 128) return launch<T, PLANES, 1, 128, true>(ta, tb, g, e, (int)ctas, cap, st);
+  return launch<T, PLANES, 1, 64, true>(ta, tb, g, e, (int)ctas, cap, st);
 }
 
 int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, const Epilogue &e,
@@ -603,7 +646,7 @@ int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, con
   g.M = e.M;
   g.N = e.N;
   g.nk = (int)((K + (int64_t)bk - 1) / bk);
-  g.chain = planes == 3 ? 2 : 32;
+  g.chain = planes == 3 ? 2 : kChain16;
   g.split = f.split;
   g.bf16 = bf16;
   g.err = ctx->d_err;
