@@ -299,6 +299,45 @@ struct Epilogue {
   int vec;  // every array's rows start on 16-byte boundaries: 16-byte accesses
 };
 
+// v += bias for the columns col .. col+7 (those beyond N keep v).
+template <typename T>
+__device__ __forceinline__ void bias8(const Epilogue &e, int col, float (&v)[8]) {
+  if (!e.bias) return;
+  const T *b = static_cast<const T *>(e.bias) + col;
+  if (e.vec && col + 8 <= e.N) {
+    float t[8];
+    load8<T>(b, t);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] += t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (col + i < e.N) v[i] += to_f32<T>(b[i]);
+  }
+}
+
+// Columns c .. c+7 of a lane's row in a swizzled block of 16-byte chunks.
+template <typename T, typename Chunk>
+__device__ __forceinline__ void store8_smem(Chunk chunk, int c, const float (&v)[8]) {
+  if (sizeof(T) == 2) {
+    store8<T>(reinterpret_cast<T *>(chunk(c / 8)), v);
+  } else {
+    *reinterpret_cast<float4 *>(chunk(c / 4)) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(chunk(c / 4 + 1)) = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+template <typename T, typename Chunk>
+__device__ __forceinline__ void load8_smem(Chunk chunk, int c, float (&v)[8]) {
+  if (sizeof(T) == 2) {
+    load8<T>(reinterpret_cast<const T *>(chunk(c / 8)), v);
+  } else {
+    const float4 a = *reinterpret_cast<const float4 *>(chunk(c / 4));
+    const float4 b = *reinterpret_cast<const float4 *>(chunk(c / 4 + 1));
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+}
+
 // z (f32 sums, without the bias) for the columns col .. col+7 of a row ->
 // out (and pre).  Everything is f32 until the one rounding of each store; the
 // activation sees the unrounded z.
@@ -307,19 +346,7 @@ __device__ __forceinline__ void epilogue8(const Epilogue &e, int row, int col, f
   const bool whole = col + 8 <= e.N;
   const int n = whole ? 8 : e.N - col;
   const bool vec = e.vec && whole;
-  if (e.bias) {
-    const T *b = static_cast<const T *>(e.bias) + col;
-    if (vec) {
-      float t[8];
-      load8<T>(b, t);
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] += t[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (i < n) v[i] += to_f32<T>(b[i]);
-    }
-  }
+  bias8<T>(e, col, v);
   if (e.pre) {
     T *p = static_cast<T *>(e.pre) + (int64_t)row * e.ldp + col;
     if (vec) {

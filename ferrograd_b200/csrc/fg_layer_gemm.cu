@@ -58,7 +58,7 @@ struct OperandLayout {
 struct ProductArgs {
   int M, N, nk;      // nk: k-blocks
   int chain;         // k-blocks of one accumulation chain
-  int stages, split;
+  int stages, split, group;
   int bf16;
   OperandLayout a, b;
   unsigned int *err;
@@ -89,6 +89,7 @@ __device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int grou
   nb = r / gm;
 }
 
+constexpr int kBlockCols = 32;                 // IO: a warp's block
 constexpr int kSlabCols = 16, kSlabPitch = 20;  // floats; a warp's 32 x 16 transpose slab
 
 // The block of each form.  RUN: the epilogue warps keep the running sums of the
@@ -101,10 +102,29 @@ struct Block {
   static constexpr int threads = 32 * (first_epi + epi_warps);
 };
 
-template <typename T, int PLANES, int CG, int BN, bool RUN>
+// Case `at` of a switch: v = run[at .. at + 15].  The moves' texts differ, or the
+// compiler joins the cases into one read of an indexed array in memory.
+#define FG_TAKE16(at)                                                                       \
+  case at:                                                                                  \
+    for (int j = 0; j < 16; j++)                                                            \
+      asm volatile("mov.f32 %0, %1; // " #at : "=f"(v[j / 8][j % 8]) : "f"(run[(at) % COLS + j])); \
+    break;
+
+// Tensor maps of a call: the operands, and where IO is set the output, the
+// pre-activations and the residual.
+struct Maps {
+  CUtensorMap a, b, out, pre, residual;
+};
+
+// IO (pair form): out, pre and the residual pass through shared memory by TMA.
+// At 64 bytes of operands in and 64 out a cycle, the MMAs of 16-bit operands
+// leave next to nothing of shared memory's 128, and a warp's 16-byte global
+// accesses to 32 rows cost it 32 passes; a TMA block costs 8 to write and 8 to
+// read.  It needs rows on 16-byte boundaries.
+template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO>
 __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
-    k_layer_product(const __grid_constant__ CUtensorMap tma, const __grid_constant__ CUtensorMap tmb,
-                    const ProductArgs g, const Epilogue e) {
+    k_layer_product(const __grid_constant__ Maps maps, const ProductArgs g, const Epilogue e) {
+  const CUtensorMap &tma = maps.a, &tmb = maps.b;
   constexpr int BK = Depth<PLANES>::BK;
   constexpr int kFirstEpi = Block<CG, RUN>::first_epi;  // first epilogue warp
   constexpr int kEpiWarps = Block<CG, RUN>::epi_warps;
@@ -118,6 +138,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   uint64_t *tmem_full = empty + kMaxStages;
   uint64_t *tmem_empty = tmem_full + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tmem_empty + 2);
+  uint64_t *res_full = tmem_empty + 4;  // IO: a warp's block of the residual has landed
   uint8_t *ring = smem + 1024;
   const uint32_t a_bytes = g.a.rows * (BK * 2), b_bytes = g.b.rows * (BK * 2);
   const uint32_t stage_bytes = PLANES * (a_bytes + b_bytes);
@@ -143,6 +164,8 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       mbar_init(&tmem_full[i], 1);
       mbar_init(&tmem_empty[i], CG * kEpiWarps);  // one arrival a warp, from both CTAs
     }
+    if (IO)
+      for (int i = 0; i < kEpiWarps; i++) mbar_init(&res_full[i], 1);
     fence_mbar_init();
     prefetch_tmap(&tma);
     prefetch_tmap(&tmb);
@@ -155,9 +178,9 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   // Pair with running sums: 384 threads x 168 registers at launch, of which the epilogue takes
-  // 256 x 224 and the others keep 128 x 56.
+  // 256 x 216 and the others keep 128 x 64.
   if (warp < kFirstEpi) {
-    if (CG == 2 && RUN) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (CG == 2 && RUN) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0 && lane == 0) {
       // ---------------- TMA producer ----------------
       int s = 0, it = 0;
@@ -165,12 +188,12 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       bool ok = true;
       for (int tile = first; ok && tile < num_m * num_n; tile += step) {
         int mb, nb;
-        tile_at(tile, num_m, num_n, 8, mb, nb);
+        tile_at(tile, num_m, num_n, g.group, mb, nb);
         const int m0 = mb * BM + (CG == 2 ? 128 * (int)rank : 0);
         const int n0 = nb * BN + (CG == 2 ? (BN / 2) * (int)rank : 0);
         for (int kb = k0; kb < k1; kb++, it++) {
           if (it >= S) {
-            ok = mbar_wait(&empty[s], phase ^ 1, g.err, kErrLayer | 1);
+            ok = mbar_wait_asleep(&empty[s], phase ^ 1, g.err, kErrLayer | 1);
             if (!ok) break;
           }
           const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
@@ -183,7 +206,9 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
                 const int x = o.mn_major ? r0 + 64 * c : kb * BK;
                 const int y = o.mn_major ? kb * BK : r0;
                 const uint32_t d = dst + c * (BK * 128);
-                if (CG == 2)
+                if (CG == 2 && PLANES == 1)
+                  tma_load_2d_pair(d, map, bar, x, y);
+                else if (CG == 2)
                   tma_load_3d_pair(d, map, bar, x, y, p);
                 else
                   tma_load_3d(ring + (d - smem_u32(ring)), map, &full[s], x, y, p);
@@ -218,7 +243,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           const int c1 = min(c0 + g.chain, k1);
           const int buf = local & 1;
           if (local >= 2) {
-            ok = mbar_wait(&tmem_empty[buf], ((local >> 1) - 1) & 1, g.err, kErrLayer | 2);
+            ok = mbar_wait_asleep(&tmem_empty[buf], ((local >> 1) - 1) & 1, g.err, kErrLayer | 2);
             if (!ok) break;
           }
           tc_fence_after();
@@ -238,7 +263,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             }
           };
           for (int kb = c0; kb < c1; kb++) {
-            ok = mbar_wait(&full[s], phase, g.err, kErrLayer | 3);
+            ok = mbar_wait_asleep(&full[s], phase, g.err, kErrLayer | 3);
             if (!ok) break;
             tc_fence_after();
             if (PLANES == 1) {
@@ -265,7 +290,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
         }
     }
   } else {
-    if (CG == 2 && RUN) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if (CG == 2 && RUN) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- epilogue ----------------
     const int q = warp & 3;  // the TMEM lanes this warp may read
     const int part = (warp - kFirstEpi) / 4;  // its columns: COLS of the tile's BN
@@ -284,8 +309,9 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       }
     };
     auto arrived = [&](int chain_no) {  // a chain's sums are in its buffer
-      if (!dead && !mbar_wait(&tmem_full[chain_no & 1], (chain_no >> 1) & 1, g.err, kErrLayer | 4))
-        dead = true;
+      if (lane == 0 && !dead)
+        dead = !mbar_wait_asleep(&tmem_full[chain_no & 1], (chain_no >> 1) & 1, g.err,
+                                 kErrLayer | 4);
       dead = __any_sync(0xffffffffu, dead);
       tc_fence_after();
       return !dead;
@@ -306,11 +332,122 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
         }
       }
     };
+    // IO: this warp's block of 32 rows x 32 columns in shared memory (swizzled
+    // rows of 64 or 128 bytes; a lane holds a row).  Out and pre leave through
+    // it, the residual arrives in it; the previous use is over once its store
+    // has read it.
+    // 16-bit types have a second block for pre, and one pass fills both; f32
+    // writes pre and then out through the one that fits.
+    constexpr int BC = kBlockCols, kRow = BC * sizeof(T);
+    constexpr bool kTwo = sizeof(T) == 2;
+    uint8_t *block = ring + S * stage_bytes + (warp - kFirstEpi) * ((kTwo ? 64 : 32) * kRow);
+    uint64_t *res_bar = &res_full[warp - kFirstEpi];
+    uint32_t res_phase = 0;
+    auto chunk = [&](int j) {
+      const int x = kRow == 128 ? lane & 7 : (lane >> 1) & 3;
+      return block + lane * kRow + ((j ^ x) << 4);
+    };
+    auto pre_chunk = [&](int j) { return chunk(j) + (kTwo ? 32 * kRow : 0); };
+    auto block_free = [&] {
+      if (lane == 0) bulk_wait_read();
+      __syncwarp();
+    };
+    auto block_store = [&](const CUtensorMap *map, const uint8_t *from, int row0, int col) {
+      if (lane == 0) {
+        tma_store_2d(map, from, col, row0);
+        bulk_commit();
+      }
+    };
+    auto residual_load = [&](int row0, int col) {
+      block_free();
+      if (lane == 0) {
+        fence_proxy_async_smem();
+        mbar_arrive_expect_tx(res_bar, 32 * kRow);
+        tma_load_2d(block, &maps.residual, res_bar, col, row0);
+      }
+    };
+    // One block: sums(c, v) gives the sums of columns col + c .. col + c + 15.
+    auto finish_block = [&](int row0, int col, bool loaded,
+                            auto sums) __attribute__((always_inline)) {
+      const int row = row0 + lane;
+      if (!kTwo && e.pre) {
+        block_free();
+#pragma unroll 1
+        for (int c = 0; c < BC; c += 16) {
+          float v[2][8];
+          sums(c, false, v);
+#pragma unroll
+          for (int p = 0; p < 2; p++) {
+            bias8<T>(e, col + c + 8 * p, v[p]);
+            store8_smem<T>(pre_chunk, c + 8 * p, v[p]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        block_store(&maps.pre, block, row0, col);
+      }
+      if (e.residual) {
+        if (!loaded) residual_load(row0, col);
+        if (lane == 0 && !dead)
+          dead = !mbar_wait_asleep(res_bar, res_phase, g.err, kErrLayer | 5);
+        dead = __any_sync(0xffffffffu, dead);
+        res_phase ^= 1;
+      } else {
+        block_free();
+      }
+#pragma unroll 1
+      for (int c = 0; c < BC; c += 16) {
+        float v[2][8];
+        sums(c, true, v);
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+          bias8<T>(e, col + c + 8 * p, v[p]);
+          if (kTwo && e.pre) store8_smem<T>(pre_chunk, c + 8 * p, v[p]);
+          act8<sizeof(T) == 2>(v[p], e.act);
+          if (e.drop.on) drop8(e.drop, row, col + c + 8 * p, v[p]);
+          if (e.residual) {
+            float t[8];
+            load8_smem<T>(chunk, c + 8 * p, t);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[p][i] += t[i];
+          }
+          store8_smem<T>(chunk, c + 8 * p, v[p]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (kTwo && e.pre) block_store(&maps.pre, block + 32 * kRow, row0, col);
+      block_store(&maps.out, block, row0, col);
+    };
     for (int tile = first; tile < num_m * num_n; tile += step) {
       int mb, nb;
-      tile_at(tile, num_m, num_n, 8, mb, nb);
+      tile_at(tile, num_m, num_n, g.group, mb, nb);
       const int row0 = mb * BM + 128 * (int)rank + 32 * q;  // of a pair
       const int col0 = nb * BN + part * COLS;
+      const bool inside = row0 < g.M && col0 < g.N;
+      if (!RUN && IO) {
+        const int buf = local & 1;
+        const bool early = inside && e.residual;
+        if (early) residual_load(row0, col0);
+        if (arrived(local++)) {
+#pragma unroll 1
+          for (int b = 0; b < COLS; b += BC) {
+            const bool some = inside && col0 + b < g.N;
+            if (some)
+              finish_block(row0, col0 + b, early && b == 0, [&](int c, bool last, float(&v)[2][8]) {
+                uint32_t r[16];
+                tmem_ld_32x32b_x16(t_addr + buf * BN + b + c, r);
+                tmem_ld_wait();
+                if (last && b + c + 16 >= COLS) release(buf);
+#pragma unroll
+                for (int j = 0; j < 16; j++) v[j / 8][j % 8] = __uint_as_float(r[j]);
+              });
+            else if (b + BC >= COLS)
+              release(buf);
+          }
+        }
+        continue;
+      }
       if (!RUN) {
         const int buf = local & 1;
         if (arrived(local++)) {
@@ -347,7 +484,25 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           release(local & 1);
         }
       }
-      if (CG == 2) {
+      if (IO) {
+        if (dead || !inside) continue;
+#pragma unroll 1
+        for (int b = 0; b < COLS; b += BC) {
+          if (col0 + b >= g.N) break;
+          finish_block(row0, col0 + b, false, [&](int c, bool, float(&v)[2][8]) __attribute__((always_inline)) {
+            switch (b + c) {
+              FG_TAKE16(0)
+              FG_TAKE16(16)
+              FG_TAKE16(32)
+              FG_TAKE16(48)
+              FG_TAKE16(64)
+              FG_TAKE16(80)
+              FG_TAKE16(96)
+              FG_TAKE16(112)
+            }
+          });
+        }
+      } else if (CG == 2) {
         if (dead || row0 >= g.M) continue;
 #pragma unroll 1
         for (int c = 0; c < COLS / kSlabCols; c++) {
@@ -384,7 +539,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
     // The cluster's CTAs share out the tile's groups of eight columns; each
     // adds its groups' sums in rank order and applies the epilogue.
     int mb, nb;
-    tile_at(first, num_m, num_n, 8, mb, nb);
+    tile_at(first, num_m, num_n, g.group, mb, nb);
     const int rows = min(128, g.M - mb * BM);
     const int groups = rows * (BN / 8);
     const int lo = (int)((long long)groups * rank / g.split);
@@ -405,6 +560,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       epilogue8<T>(e, mb * BM + r, col, v);
     }
   }
+  if (IO && warp >= kFirstEpi && lane == 0) bulk_wait_read();
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while another may still reach its memory
@@ -538,9 +694,11 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [planes][outer][pitch] of 16-bit elements; one box is box_rows K-major rows
+// [planes][outer][pitch] of 16-bit elements (without the planes for a pair's
+// 16-bit operands: 2-D loads keep the TMA unit 2% busier); one box is box_rows K-major rows
 // of BK elements, or BK k-rows of 64 MN-major elements.
-static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bool bf16) {
+static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bool bf16,
+                    bool pair) {
   auto fn = encode_fn();
   if (!fn) return set_error(FG_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t pitch = (cuuint64_t)o.pitch * 2;
@@ -550,7 +708,7 @@ static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bo
                              (cuuint32_t)(o.mn_major ? bk : box_rows), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(
-      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.planes == 1 && pair ? 2 : 3,
       const_cast<void *>(o.ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
       o.mn_major || bk == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -561,21 +719,42 @@ static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bo
   return FG_OK;
 }
 
+// [M, N] with pitch ld, in blocks of 32 x 32 (rows of 64 or 128 bytes, swizzled).
+template <typename T>
+static int make_io_map(CUtensorMap *map, const void *ptr, int M, int N, int64_t ld) {
+  auto fn = encode_fn();
+  if (!fn) return set_error(FG_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * sizeof(T)};
+  const cuuint32_t box[2] = {kBlockCols, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  // 16-bit types are only moved, so either 16-bit map type serves
+  const CUresult r =
+      fn(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+         2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(FG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): %d x %d, pitch %lld", (int)r,
+                     M, N, (long long)ld);
+  return FG_OK;
+}
+
 // Shared memory a CTA must ask for so that the CTAs that fit on an SM never
 // need more than its 512 TMEM columns between them: an allocation that had to
 // wait while its cluster's other CTAs hold theirs could wait for ever.
 static size_t tmem_share(int cols) { return (size_t)cols / 128 * 47 * 1024; }
 
-template <typename T, int PLANES, int CG, int BN, bool RUN>
-static int launch(const CUtensorMap &ta, const CUtensorMap &tb, ProductArgs g, const Epilogue &e,
-                  int ctas, size_t ring_cap, cudaStream_t st) {
+template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO>
+static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, size_t ring_cap,
+                  cudaStream_t st) {
   constexpr int BK = Depth<PLANES>::BK;
-  auto kern = k_layer_product<T, PLANES, CG, BN, RUN>;
+  auto kern = k_layer_product<T, PLANES, CG, BN, RUN, IO>;
   const size_t stage = (size_t)PLANES * (g.a.rows + g.b.rows) * BK * 2;
-  // past the ring: the pair's slabs, or what an MMA of 128 rows reads beyond
-  // an A tile of fewer (it lands in unused accumulator rows)
-  const size_t tail =
-      CG == 2 ? Block<CG, RUN>::epi_warps * 32 * kSlabPitch * 4 : 128 * BK * 2;
+  // past the ring: the pair's blocks or slabs, or what an MMA of 128 rows reads
+  // beyond an A tile of fewer (it lands in unused accumulator rows)
+  const size_t tail = CG == 2 ? Block<CG, RUN>::epi_warps * (IO ? 4096 : 32 * kSlabPitch * 4)
+                              : 128 * BK * 2;
   int64_t stages = (int64_t)(ring_cap / stage);
   if (stages > kMaxStages) stages = kMaxStages;
   if (CG == 1) {
@@ -610,27 +789,40 @@ static int launch(const CUtensorMap &ta, const CUtensorMap &tb, ProductArgs g, c
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ta, tb, g, e));
+  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, g, e));
   count_launch();
   return FG_OK;
 }
 
 template <typename T, int PLANES>
-static int run_form(const Form &f, const CUtensorMap &ta, const CUtensorMap &tb, ProductArgs g,
-                    const Epilogue &e, int sms, cudaStream_t st) {
+static int run_form(const Form &f, Maps &maps, ProductArgs g, const Epilogue &e, int sms,
+                    cudaStream_t st) {
   const int64_t tiles = (int64_t)((g.M + f.bm - 1) / f.bm) * ((g.N + f.bn - 1) / f.bn);
   if (f.pair) {
     const int pairs = sms / 2;
     const int ctas = 2 * (int)(tiles < pairs ? tiles : pairs);
-    if (PLANES == 1 && g.chain >= g.nk)
-      return launch<T, PLANES, 2, 256, PLANES == 3>(ta, tb, g, e, ctas, 160 * 1024, st);
-    return launch<T, PLANES, 2, 256, true>(ta, tb, g, e, ctas, 192 * 1024, st);
+    // 16-bit: five stages of 32 KB (a sixth gains nothing) beside sixteen
+    // warps' two blocks of 2 KB; f32: four of 48 KB beside eight of 4 KB
+    constexpr bool kLong = PLANES == 3;
+    const size_t ring = (kLong ? 192 : 160) * 1024;
+    if (e.vec) {
+      int rc = make_io_map<T>(&maps.out, e.out, e.M, e.N, e.ldo);
+      if (!rc && e.pre) rc = make_io_map<T>(&maps.pre, e.pre, e.M, e.N, e.ldp);
+      if (!rc && e.residual) rc = make_io_map<T>(&maps.residual, e.residual, e.M, e.N, e.ldr);
+      if (rc) return rc;
+      if (g.chain >= g.nk)
+        return launch<T, PLANES, 2, 256, kLong, true>(maps, g, e, ctas, ring, st);
+      return launch<T, PLANES, 2, 256, true, true>(maps, g, e, ctas, 192 * 1024, st);
+    }
+    if (g.chain >= g.nk)
+      return launch<T, PLANES, 2, 256, kLong, false>(maps, g, e, ctas, ring, st);
+    return launch<T, PLANES, 2, 256, true, false>(maps, g, e, ctas, 192 * 1024, st);
   }
   const int64_t ctas = tiles * f.split;
   // more CTAs than SMs: two to an SM, so that one computes while the other joins
   const size_t cap = ctas > sms ? 92 * 1024 : 190 * 1024;
-  if (f.bn == 128) return launch<T, PLANES, 1, 128, true>(ta, tb, g, e, (int)ctas, cap, st);
-  return launch<T, PLANES, 1, 64, true>(ta, tb, g, e, (int)ctas, cap, st);
+  if (f.bn == 128) return launch<T, PLANES, 1, 128, true, false>(maps, g, e, (int)ctas, cap, st);
+  return launch<T, PLANES, 1, 64, true, false>(maps, g, e, (int)ctas, cap, st);
 }
 
 int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, const Epilogue &e,
@@ -648,6 +840,7 @@ int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, con
   g.nk = (int)((K + (int64_t)bk - 1) / bk);
   g.chain = planes == 3 ? 2 : kChain16;
   g.split = f.split;
+  g.group = f.pair ? 16 : 8;
   g.bf16 = bf16;
   g.err = ctx->d_err;
   const int unit_a = a.mn_major ? 64 : 16;
@@ -656,17 +849,17 @@ int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, con
   g.b.mn_major = b.mn_major;
   g.b.rows = f.pair ? 128 : f.bn;
   if (f.pair) g.a.rows = 128;
-  CUtensorMap ta, tb;
-  int rc = make_map(&ta, a, bk, g.a.rows, bf16);
+  Maps maps = {};
+  int rc = make_map(&maps.a, a, bk, g.a.rows, bf16, f.pair);
   if (rc) return rc;
-  if ((rc = make_map(&tb, b, bk, g.b.rows, bf16))) return rc;
+  if ((rc = make_map(&maps.b, b, bk, g.b.rows, bf16, f.pair))) return rc;
   switch (dtype) {
     case FG_F32:
-      return run_form<float, 3>(f, ta, tb, g, e, sms, st);
+      return run_form<float, 3>(f, maps, g, e, sms, st);
     case FG_BF16:
-      return run_form<__nv_bfloat16, 1>(f, ta, tb, g, e, sms, st);
+      return run_form<__nv_bfloat16, 1>(f, maps, g, e, sms, st);
     default:
-      return run_form<__half, 1>(f, ta, tb, g, e, sms, st);
+      return run_form<__half, 1>(f, maps, g, e, sms, st);
   }
 }
 

@@ -58,6 +58,28 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, unsign
   return true;
 }
 
+// mbar_wait for waits that are long as a rule: the thread may be suspended for
+// up to a millisecond at a time instead of polling.
+__device__ __forceinline__ bool mbar_wait_asleep(uint64_t *bar, uint32_t parity, unsigned int *err,
+                                                 unsigned int code) {
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      if (err) atomicOr(err, code);
+      return false;
+    }
+  }
+}
+
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)m) : "memory");
 }
@@ -86,6 +108,23 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *m
       " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem_dst)),
       "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
+}
+
+// 2-D tiled TMA store from this CTA's shared memory (elements outside the
+// tensor are not written), tracked by the thread's bulk groups.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *smem_src, int x,
+                                             int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::
+                   "l"((uint64_t)map),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Every store of this thread's committed groups has read its shared memory.
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 // ---- tcgen05 -------------------------------------------------------------
@@ -284,8 +323,16 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
   return v;
 }
 
-// 3-D tiled TMA load into this CTA's own shared memory whose bytes complete on
-// a barrier given by its shared::cluster address (the pair's leader's).
+// Tiled TMA loads into this CTA's own shared memory whose bytes complete on a
+// barrier given by its shared::cluster address (the pair's leader's).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap *map,
+                                                 uint32_t bar_cluster, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx"
+      "::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar_cluster)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtensorMap *map,
                                                  uint32_t bar_cluster, int x, int y, int z) {
   asm volatile(
