@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
         const int n0 = nb * BN + (CG == 2 ? (BN / 2) * (int)rank : 0);
         for (int kb = k0; kb < k1; kb++, it++) {
           if (it >= S) {
-            ok = mbar_wait_asleep(&empty[s], phase ^ 1, g.err, kErrLayer | 1);
+            ok = mbar_wait_suspended(&empty[s], phase ^ 1, g.err, kErrLayer | 1);
             if (!ok) break;
           }
           const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           const int c1 = min(c0 + g.chain, k1);
           const int buf = local & 1;
           if (local >= 2) {
-            ok = mbar_wait_asleep(&tmem_empty[buf], ((local >> 1) - 1) & 1, g.err, kErrLayer | 2);
+            ok = mbar_wait_suspended(&tmem_empty[buf], ((local >> 1) - 1) & 1, g.err, kErrLayer | 2);
             if (!ok) break;
           }
           tc_fence_after();
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             }
           };
           for (int kb = c0; kb < c1; kb++) {
-            ok = mbar_wait_asleep(&full[s], phase, g.err, kErrLayer | 3);
+            ok = mbar_wait_suspended(&full[s], phase, g.err, kErrLayer | 3);
             if (!ok) break;
             tc_fence_after();
             if (PLANES == 1) {
@@ -309,10 +309,13 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       }
     };
     auto arrived = [&](int chain_no) {  // a chain's sums are in its buffer
-      if (lane == 0 && !dead)
-        dead = !mbar_wait_asleep(&tmem_full[chain_no & 1], (chain_no >> 1) & 1, g.err,
-                                 kErrLayer | 4);
-      dead = __any_sync(0xffffffffu, dead);
+      // One lane of four warps polls, and they sleep at a barrier: sixteen
+      // polling warps cost the MMAs 4% through the shared memory they share.
+      if (q == (kFirstEpi & 3) && lane == 0 && !dead)
+        dead = !mbar_wait_suspended(&tmem_full[chain_no & 1], (chain_no >> 1) & 1, g.err,
+                                    kErrLayer | 4);
+      __syncwarp();
+      dead = named_bar_or(1 + part, 128, dead);
       tc_fence_after();
       return !dead;
     };
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       if (e.residual) {
         if (!loaded) residual_load(row0, col);
         if (lane == 0 && !dead)
-          dead = !mbar_wait_asleep(res_bar, res_phase, g.err, kErrLayer | 5);
+          dead = !mbar_wait_suspended(res_bar, res_phase, g.err, kErrLayer | 5);
         dead = __any_sync(0xffffffffu, dead);
         res_phase ^= 1;
       } else {

@@ -58,10 +58,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, unsign
   return true;
 }
 
-// mbar_wait for waits that are long as a rule: the thread may be suspended for
-// up to a millisecond at a time instead of polling.
-__device__ __forceinline__ bool mbar_wait_asleep(uint64_t *bar, uint32_t parity, unsigned int *err,
-                                                 unsigned int code) {
+// mbar_wait whose polls may each suspend the thread for up to a millisecond.
+__device__ __forceinline__ bool mbar_wait_suspended(uint64_t *bar, uint32_t parity,
+                                                    unsigned int *err, unsigned int code) {
   const long long t0 = clock64();
   for (;;) {
     uint32_t ok;
@@ -125,6 +124,18 @@ __device__ __forceinline__ void bulk_commit() {
 // Every store of this thread's committed groups has read its shared memory.
 __device__ __forceinline__ void bulk_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
+// Named barrier over `threads` threads; true if any of them passed true.
+__device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t threads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred.aligned q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((uint32_t)pred)
+      : "memory");
+  return r != 0;
 }
 
 // ---- tcgen05 -------------------------------------------------------------
