@@ -57,6 +57,16 @@ __device__ __forceinline__ float2 unpack2(uint32_t u, __half) {
   return __half22float2(*reinterpret_cast<__half2 *>(&u));
 }
 
+// T itself where it is a 16-bit type (what the pair functions above take).
+template <typename T>
+struct Half16 {
+  using type = T;
+};
+template <>
+struct Half16<float> {
+  using type = __half;
+};
+
 // Eight consecutive elements in 16-byte accesses (the address is aligned).
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
@@ -380,6 +390,29 @@ __device__ __forceinline__ void epilogue8(const Epilogue &e, int row, int col, f
     for (int i = 0; i < 8; i++)
       if (i < n) o[i] = from_f32<T>(v[i]);
   }
+}
+
+// The same for one element.
+template <typename T>
+__device__ __forceinline__ void epilogue1(const Epilogue &e, int row, int col, float z) {
+  if (e.bias) z += to_f32<T>(static_cast<const T *>(e.bias)[col]);
+  if (e.pre) static_cast<T *>(e.pre)[(int64_t)row * e.ldp + col] = from_f32<T>(z);
+  float v[8] = {z, z, z, z, z, z, z, z};
+  if (e.act) {
+    act8<sizeof(T) == 2>(v, e.act);
+    z = v[0];
+  }
+  if (e.drop.on) {
+    drop8(e.drop, row, col & ~7, v);
+    const int i = col & 7;
+    z = v[0];
+#pragma unroll
+    for (int k = 1; k < 8; k++)
+      if (i == k) z = v[k];
+  }
+  if (e.residual)
+    z += to_f32<T>(static_cast<const T *>(e.residual)[(int64_t)row * e.ldr + col]);
+  static_cast<T *>(e.out)[(int64_t)row * e.ldo + col] = from_f32<T>(z);
 }
 
 // A matrix operand: element (r, c) at ptr[r * row + c * col].

@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       const int row0 = mb * BM + 128 * (int)rank + 32 * q;  // of a pair
       const int col0 = nb * BN + part * COLS;
       const bool inside = row0 < g.M && col0 < g.N;
-      if (!RUN && IO) {
+      if constexpr (!RUN && IO) {
         const int buf = local & 1;
         const bool early = inside && e.residual;
         if (early) residual_load(row0, col0);
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
         }
         continue;
       }
-      if (!RUN) {
+      if constexpr (!RUN) {
         const int buf = local & 1;
         if (arrived(local++)) {
 #pragma unroll 1
@@ -471,66 +471,68 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
         }
         continue;
       }
-      float run[COLS];
+      if constexpr (RUN) {
+        float run[COLS];
 #pragma unroll
-      for (int j = 0; j < COLS; j++) run[j] = 0.0f;
-      for (int c0 = k0; c0 < k1; c0 += g.chain, local++) {
-        if (arrived(local)) {
+        for (int j = 0; j < COLS; j++) run[j] = 0.0f;
+        for (int c0 = k0; c0 < k1; c0 += g.chain, local++) {
+          if (arrived(local)) {
 #pragma unroll
-          for (int c = 0; c < COLS; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(t_addr + (local & 1) * BN + c, r);
-            tmem_ld_wait();
+            for (int c = 0; c < COLS; c += 32) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(t_addr + (local & 1) * BN + c, r);
+              tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j++) run[c + j] += __uint_as_float(r[j]);
+              for (int j = 0; j < 32; j++) run[c + j] += __uint_as_float(r[j]);
+            }
+            release(local & 1);
           }
-          release(local & 1);
         }
-      }
-      if (IO) {
-        if (dead || !inside) continue;
+        if (IO) {
+          if (dead || !inside) continue;
 #pragma unroll 1
-        for (int b = 0; b < COLS; b += BC) {
-          if (col0 + b >= g.N) break;
-          finish_block(row0, col0 + b, false, [&](int c, bool, float(&v)[2][8]) __attribute__((always_inline)) {
-            switch (b + c) {
-              FG_TAKE16(0)
-              FG_TAKE16(16)
-              FG_TAKE16(32)
-              FG_TAKE16(48)
-              FG_TAKE16(64)
-              FG_TAKE16(80)
-              FG_TAKE16(96)
-              FG_TAKE16(112)
-            }
-          });
-        }
-      } else if (CG == 2) {
-        if (dead || row0 >= g.M) continue;
+          for (int b = 0; b < COLS; b += BC) {
+            if (col0 + b >= g.N) break;
+            finish_block(row0, col0 + b, false, [&](int c, bool, float(&v)[2][8]) __attribute__((always_inline)) {
+              switch (b + c) {
+                FG_TAKE16(0)
+                FG_TAKE16(16)
+                FG_TAKE16(32)
+                FG_TAKE16(48)
+                FG_TAKE16(64)
+                FG_TAKE16(80)
+                FG_TAKE16(96)
+                FG_TAKE16(112)
+              }
+            });
+          }
+        } else if (CG == 2) {
+          if (dead || row0 >= g.M) continue;
 #pragma unroll 1
-        for (int c = 0; c < COLS / kSlabCols; c++) {
-          if (col0 + c * kSlabCols >= g.N) break;
-          __syncwarp();
+          for (int c = 0; c < COLS / kSlabCols; c++) {
+            if (col0 + c * kSlabCols >= g.N) break;
+            __syncwarp();
 #pragma unroll
-          for (int cc = 0; cc < COLS / kSlabCols; cc++)
-            if (cc == c) {
+            for (int cc = 0; cc < COLS / kSlabCols; cc++)
+              if (cc == c) {
 #pragma unroll
-              for (int j = 0; j < kSlabCols; j += 4)
-                *reinterpret_cast<float4 *>(slab + lane * kSlabPitch + j) =
-                    make_float4(run[cc * kSlabCols + j], run[cc * kSlabCols + j + 1],
-                                run[cc * kSlabCols + j + 2], run[cc * kSlabCols + j + 3]);
-            }
-          finish16(row0, col0 + c * kSlabCols);
-        }
-      } else {
-        // the whole tile's sums to shared memory (the ring is free: every
-        // load was waited for, every MMA has completed)
-        float *sums = reinterpret_cast<float *>(ring) + (32 * q + lane) * (BN + 4);
-        if (!dead) {
+                for (int j = 0; j < kSlabCols; j += 4)
+                  *reinterpret_cast<float4 *>(slab + lane * kSlabPitch + j) =
+                      make_float4(run[cc * kSlabCols + j], run[cc * kSlabCols + j + 1],
+                                  run[cc * kSlabCols + j + 2], run[cc * kSlabCols + j + 3]);
+              }
+            finish16(row0, col0 + c * kSlabCols);
+          }
+        } else {
+          // the whole tile's sums to shared memory (the ring is free: every
+          // load was waited for, every MMA has completed)
+          float *sums = reinterpret_cast<float *>(ring) + (32 * q + lane) * (BN + 4);
+          if (!dead) {
 #pragma unroll
-          for (int j = 0; j < COLS; j += 4)
-            *reinterpret_cast<float4 *>(sums + j) =
-                make_float4(run[j], run[j + 1], run[j + 2], run[j + 3]);
+            for (int j = 0; j < COLS; j += 4)
+              *reinterpret_cast<float4 *>(sums + j) =
+                  make_float4(run[j], run[j + 1], run[j + 2], run[j + 3]);
+          }
         }
       }
     }

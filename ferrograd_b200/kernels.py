@@ -135,15 +135,15 @@ _LAYER_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float
 
 
 def _layer_check(name: str, t: torch.Tensor, like: torch.Tensor, shape, unit_cols=False) -> None:
-    """``t`` is a CUDA tensor of this shape on ``like``'s device in its dtype
-    (with ``unit_cols``: its last dimension has stride 1)."""
-    if not t.is_cuda or t.device != like.device:
+    """``t`` is a tensor of this shape on ``like``'s device in its dtype (with
+    ``unit_cols``: its last dimension has stride 1)."""
+    if t.device != like.device:
         raise ValueError(f"{name}: expected a CUDA tensor on {like.device}, got {t.device}")
-    if t.dtype != like.dtype:
+    if t.dtype is not like.dtype:
         raise ValueError(f"{name}: expected {like.dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if unit_cols and t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
+    if unit_cols and t.stride()[-1] != 1 and t.shape[-1] > 1 and t.numel():
         raise ValueError(f"{name}: expected unit stride in the last dimension")
 
 
@@ -156,33 +156,45 @@ def _layer_dtype(t: torch.Tensor) -> int:
     return code
 
 
-def _drop_spec(spec: _lib.DropoutC, drop: Optional[Dropout]) -> None:
-    if drop is not None:
-        spec.p = drop.p
-        spec.seed = drop.seed & 0xFFFFFFFFFFFFFFFF
-        spec.offset = drop.offset & 0xFFFFFFFFFFFFFFFF
+def _drop_spec(spec: _lib.DropoutC, drop: Dropout) -> None:
+    spec.p = drop.p
+    spec.seed = drop.seed & 0xFFFFFFFFFFFFFFFF
+    spec.offset = drop.offset & 0xFFFFFFFFFFFFFFFF
 
 
-def _layer_run(name: str, args, device: torch.device, stream: Optional[int]) -> None:
-    """Calls ``name`` with the workspace it asks for, on ``device``."""
-    if device.index != torch.cuda.current_device():
+# Handle of the current stream without building a torch.cuda.Stream for it (3 us).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _layer_run(name: str, args, x: torch.Tensor, stream: Optional[int]) -> None:
+    """Calls ``name`` with the workspace it asks for, on ``x``'s device."""
+    device = x.device.index
+    if device != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _layer_run(name, args, device, stream)
+            return _layer_run(name, args, x, stream)
+    lib = _lib.lib()
+    ref = ctypes.byref(args)
     need = ctypes.c_size_t()
-    call(name + "_workspace", ctypes.byref(args), ctypes.byref(need))
+    code = getattr(lib, name + "_workspace")(ref, ctypes.byref(need))
+    if code:
+        _lib.check(code)
     if need.value:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
         if stream is not None:  # the allocator must not hand it out before that stream is done
-            ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
+            ws.record_stream(torch.cuda.ExternalStream(stream, device=x.device))
         args.workspace = ws.data_ptr()
         args.workspace_bytes = need.value
-    call(name, ctypes.byref(args), _stream(stream))
+    code = getattr(lib, name)(ref, _raw_stream(device) if stream is None else stream)
+    if code:
+        _lib.check(code)
 
 
 def _ld(t: torch.Tensor) -> int:
     """Row pitch of a 2-D tensor with unit column stride (rows of one row, or
     of one element, may carry any stride)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+    rows, cols = t.shape
+    pitch = t.stride()[0]
+    return max(pitch, cols) if rows <= 1 else pitch
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -206,9 +218,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     M, K = x.shape
     N = w.shape[0]
     _layer_check("w", w, x, (N, K))
-    a = _lib.LinearArgsC(dtype=code, M=M, N=N, K=K, x=x.data_ptr(), x_row=x.stride(0),
-                         x_col=x.stride(1), w=w.data_ptr(), w_row=w.stride(0), w_col=w.stride(1),
-                         act=ACTIVATIONS[act])
+    a = _lib.LinearArgsC(code, M, N, K, x.data_ptr(), *x.stride(), w.data_ptr(), *w.stride())
+    a.act = ACTIVATIONS[act]
     if bias is not None:
         _layer_check("bias", bias, x, (N,), True)
         a.bias = bias.data_ptr()
@@ -216,16 +227,19 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
         _layer_check("residual", residual, x, (M, N), True)
         a.residual, a.ld_residual = residual.data_ptr(), _ld(residual)
     if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        out = x.new_empty(M, N)
+        a.ld_out = N
     else:
         _layer_check("out", out, x, (M, N), True)
-    a.out, a.ld_out = out.data_ptr(), _ld(out)
+        a.ld_out = _ld(out)
+    a.out = out.data_ptr()
     pre = None
     if save_pre:
-        pre = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        pre = x.new_empty(M, N)
         a.pre, a.ld_pre = pre.data_ptr(), N
-    _drop_spec(a.drop, drop)
-    _layer_run("fg_linear", a, x.device, stream)
+    if drop is not None:
+        _drop_spec(a.drop, drop)
+    _layer_run("fg_linear", a, x, stream)
     return (out, pre) if save_pre else out
 
 
@@ -247,10 +261,9 @@ def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
     N = w.shape[0]
     _layer_check("w", w, x, (N, K))
     _layer_check("dy", dy, x, (M, N))
-    a = _lib.LinearGradArgsC(dtype=code, M=M, N=N, K=K, dy=dy.data_ptr(), dy_row=dy.stride(0),
-                             dy_col=dy.stride(1), x=x.data_ptr(), x_row=x.stride(0),
-                             x_col=x.stride(1), w=w.data_ptr(), w_row=w.stride(0),
-                             w_col=w.stride(1), act=ACTIVATIONS[act])
+    a = _lib.LinearGradArgsC(code, M, N, K, dy.data_ptr(), *dy.stride(), x.data_ptr(),
+                             *x.stride(), w.data_ptr(), *w.stride())
+    a.act = ACTIVATIONS[act]
     if act != "none":
         if pre is None:
             raise ValueError(f"the gradient of {act} needs pre (linear(..., save_pre=True))")
@@ -258,16 +271,17 @@ def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
         a.pre, a.ld_pre = pre.data_ptr(), _ld(pre)
     dx = dw = db = None
     if need_dx:
-        dx = torch.empty((M, K), dtype=x.dtype, device=x.device)
+        dx = x.new_empty(M, K)
         a.dx, a.ld_dx = dx.data_ptr(), K
     if need_dw:
-        dw = torch.empty((N, K), dtype=x.dtype, device=x.device)
+        dw = x.new_empty(N, K)
         a.dw, a.ld_dw = dw.data_ptr(), K
     if need_db:
-        db = torch.empty((N,), dtype=x.dtype, device=x.device)
+        db = x.new_empty(N)
         a.db = db.data_ptr()
-    _drop_spec(a.drop, drop)
-    _layer_run("fg_linear_grad", a, x.device, stream)
+    if drop is not None:
+        _drop_spec(a.drop, drop)
+    _layer_run("fg_linear_grad", a, x, stream)
     return dx, dw, db
 
 
@@ -276,29 +290,34 @@ def dropout(x: torch.Tensor, drop: Optional[Dropout], *, residual: Optional[torc
     """``residual + dropout(x)`` on the last dimension's columns and the rows
     before it (a 1-D tensor is one row).  ``out`` may be ``x`` or the residual."""
     code = _layer_dtype(x)
+    shape = x.shape
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    cols = x.shape[-1] if x.dim() else 1
+        out = x.new_empty(shape)
+    cols = shape[-1] if shape else 1
     rows = x.numel() // cols if cols else 0
     ptrs = []
     for name, t in (("x", x), ("residual", residual), ("out", out)):
         if t is None:
-            ptrs += [None, 0]
+            ptrs += (None, 0)
             continue
-        _layer_check(name, t, x, x.shape, x.dim() > 0)
-        if t.dim() == 2:
-            ptrs += [t.data_ptr(), _ld(t)]
+        _layer_check(name, t, x, shape, len(shape) > 0)
+        if len(shape) == 2:
+            ptrs += (t.data_ptr(), _ld(t))
         elif t.is_contiguous():
-            ptrs += [t.data_ptr(), cols]
+            ptrs += (t.data_ptr(), cols)
         else:
             raise ValueError(f"{name}: expected a 2-D or a contiguous tensor")
     spec = _lib.DropoutC()
-    _drop_spec(spec, drop)
-    if x.device.index != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
-            call("fg_dropout", code, rows, cols, *ptrs, ctypes.byref(spec), _stream(stream))
-    else:
-        call("fg_dropout", code, rows, cols, *ptrs, ctypes.byref(spec), _stream(stream))
+    if drop is not None:
+        _drop_spec(spec, drop)
+    device = x.device.index
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return dropout(x, drop, residual=residual, out=out, stream=stream)
+    code = _lib.lib().fg_dropout(code, rows, cols, *ptrs, ctypes.byref(spec),
+                                 _raw_stream(device) if stream is None else stream)
+    if code:
+        _lib.check(code)
     return out
 
 
