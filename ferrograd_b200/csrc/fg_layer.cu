@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256)
     k_linear_rows(const T *__restrict__ x, int64_t xr, const T *__restrict__ w, int64_t wr, int K,
                   const Epilogue e) {
   constexpr int V = VEC ? 16 / sizeof(T) : 1;  // elements a lane reads at once
-  constexpr int U = MR == 1 ? 8 : MR <= 4 ? 4 : 2;  // steps in flight
+  constexpr int U = MR == 1 ? 8 : MR <= 4 ? 4 : 2;  // steps in flight (rows past M repeat the last)
   const int lane = threadIdx.x & 31;
   const int n0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 2;
   if (n0 >= e.N) return;
@@ -127,11 +127,13 @@ __global__ void __launch_bounds__(256)
     float a[V], b[V];
     unraw<T>(ra, a);
     unraw<T>(rb, b);
+    Raw rx[MR];
+#pragma unroll
+    for (int m = 0; m < MR; m++) rx[m] = read(x + min(m, e.M - 1) * xr + k);
 #pragma unroll
     for (int m = 0; m < MR; m++) {
-      if (m >= e.M) break;
       float t[V];
-      unraw<T>(read(x + m * xr + k), t);
+      unraw<T>(rx[m], t);
 #pragma unroll
       for (int i = 0; i < V; i++) {
         acc[m][0] = fmaf(t[i], a[i], acc[m][0]);
@@ -156,8 +158,7 @@ __global__ void __launch_bounds__(256)
     for (; k < K; k++)
 #pragma unroll
       for (int m = 0; m < MR; m++) {
-        if (m >= e.M) break;
-        const float t = to_f32<T>(x[m * xr + k]);
+        const float t = to_f32<T>(x[min(m, e.M - 1) * xr + k]);
         acc[m][0] = fmaf(t, to_f32<T>(w0[k]), acc[m][0]);
         acc[m][1] = fmaf(t, to_f32<T>(w1[k]), acc[m][1]);
       }
@@ -179,6 +180,8 @@ static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaSt
   auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(x, g->x_row, w, g->w_row, g->K, e); };
   if (g->M == 1)
     vec ? go(k_linear_rows<T, 1, true>) : go(k_linear_rows<T, 1, false>);
+  else if (g->M == 2)
+    vec ? go(k_linear_rows<T, 2, true>) : go(k_linear_rows<T, 2, false>);
   else if (g->M <= 4)
     vec ? go(k_linear_rows<T, 4, true>) : go(k_linear_rows<T, 4, false>);
   else

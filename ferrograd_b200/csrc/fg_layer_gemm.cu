@@ -30,6 +30,7 @@
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "fg_internal.h"
 #include "fg_layer.cuh"
@@ -39,6 +40,9 @@ namespace fg {
 namespace layer {
 
 using namespace fg::ptx;
+
+using True = std::true_type;
+using False = std::false_type;
 
 constexpr int kMaxStages = 16;
 // k-blocks of a chain of 16-bit products: 16384 deep, 1024 truncated additions
@@ -140,6 +144,9 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tmem_empty + 2);
   uint64_t *res_full = tmem_empty + 4;  // IO: a warp's block of the residual has landed
   uint8_t *ring = smem + 1024;
+  // split: where this rank's columns are summed, [split][128][BN / split], once
+  // the ring is done with
+  float *sums = reinterpret_cast<float *>(ring);
   const uint32_t a_bytes = g.a.rows * (BK * 2), b_bytes = g.b.rows * (BK * 2);
   const uint32_t stage_bytes = PLANES * (a_bytes + b_bytes);
 
@@ -175,14 +182,21 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   __syncthreads();
   if (CG == 2) cluster_sync_all();  // the peer's barriers and TMEM are ready
   tc_fence_after();
+  grid_wait();  // everything above overlaps the previous kernel's end
+  if (CG == 1) grid_launch_next();
   const uint32_t tmem_base = *tmem_slot;
 
   // Pair with running sums: 384 threads x 168 registers at launch, of which the epilogue takes
   // 256 x 216 and the others keep 128 x 64.
   if (warp < kFirstEpi) {
     if (CG == 2 && RUN) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 0 && lane == 0) {
+    // Both loops below run in whole warps with one lane's instructions switched
+    // on, and are instantiated for each pair of layouts.
+    const uint32_t on = lane == 0;
+    const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), ring0 = smem_u32(ring);
+    auto produce = [&](auto a_layout, auto b_layout) {
       // ---------------- TMA producer ----------------
+      const uint32_t bars = CG == 2 ? map_to_rank(full0, 0) : full0;
       int s = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -193,31 +207,30 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
         const int n0 = nb * BN + (CG == 2 ? (BN / 2) * (int)rank : 0);
         for (int kb = k0; kb < k1; kb++, it++) {
           if (it >= S) {
-            ok = mbar_wait_suspended(&empty[s], phase ^ 1, g.err, kErrLayer | 1);
+            ok = mbar_wait_suspended(empty0 + 8 * s, phase ^ 1, g.err, kErrLayer | 1);
             if (!ok) break;
           }
-          const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
-          if (leader) mbar_arrive_expect_tx(&full[s], CG * stage_bytes);
-          uint32_t dst = smem_u32(ring + s * stage_bytes);
-          auto load = [&](const CUtensorMap *map, const OperandLayout &o, int r0, uint32_t bytes) {
+          if (leader) mbar_expect_tx(on, full0 + 8 * s, CG * stage_bytes);
+          uint32_t dst = ring0 + s * stage_bytes;
+          const uint32_t bar = bars + 8 * s;
+          auto load = [&](const CUtensorMap *map, auto layout, int rows, int r0, uint32_t bytes) {
+            constexpr bool mn = decltype(layout)::value;
+#pragma unroll
             for (int p = 0; p < PLANES; p++) {
-              const int parts = o.mn_major ? o.rows / 64 : 1;
-              for (int c = 0; c < parts; c++) {
-                const int x = o.mn_major ? r0 + 64 * c : kb * BK;
-                const int y = o.mn_major ? kb * BK : r0;
-                const uint32_t d = dst + c * (BK * 128);
-                if (CG == 2 && PLANES == 1)
-                  tma_load_2d_pair(d, map, bar, x, y);
-                else if (CG == 2)
-                  tma_load_3d_pair(d, map, bar, x, y, p);
+#pragma unroll
+              for (int c = 0; c < (mn ? 2 : 1); c++) {  // 128 rows at most
+                if (mn && 64 * c >= rows) break;
+                const int x = mn ? r0 + 64 * c : kb * BK, y = mn ? kb * BK : r0;
+                if (PLANES == 1)
+                  tma_load_2d_cg<CG>(on, dst + c * (BK * 128), map, bar, x, y);
                 else
-                  tma_load_3d(ring + (d - smem_u32(ring)), map, &full[s], x, y, p);
+                  tma_load_3d_cg<CG>(on, dst + c * (BK * 128), map, bar, x, y, p);
               }
               dst += bytes;
             }
           };
-          load(&tma, g.a, m0, a_bytes);
-          load(&tmb, g.b, n0, b_bytes);
+          load(&tma, a_layout, g.a.rows, m0, a_bytes);
+          load(&tmb, b_layout, g.b.rows, n0, b_bytes);
           if (++s == S) s = 0, phase ^= 1;
         }
       }
@@ -229,12 +242,19 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           mbar_wait(&full[i % S], (i / S) & 1, nullptr, 0);
       else if (!ok)
         for (const long long t0 = clock64(); clock64() - t0 < 2000000;) __nanosleep(1000);
-    } else if (warp == 1 && lane == 0 && leader) {
+    };
+    auto multiply = [&](auto a_layout, auto b_layout) {
+      constexpr bool a_mn = decltype(a_layout)::value, b_mn = decltype(b_layout)::value;
       // ---------------- MMA issuer ----------------
-      const uint32_t idesc = idesc_f16(BM, BN, g.bf16, g.a.mn_major, g.b.mn_major);
-      const uint64_t da0 = desc_base<PLANES>(g.a.mn_major), db0 = desc_base<PLANES>(g.b.mn_major);
+      const uint32_t idesc = idesc_f16(BM, BN, g.bf16, a_mn, b_mn);
+      // a descriptor holds the 18 low bits of an address (those above name the
+      // CTA within its cluster)
+      const uint64_t da0 = desc_base<PLANES>(a_mn) + ((ring0 & 0x3ffffu) >> 4);
+      const uint64_t db0 =
+          desc_base<PLANES>(b_mn) + (((ring0 & 0x3ffffu) + PLANES * a_bytes) >> 4);
       // 16 elements further in k: 32 bytes inside a swizzled row, or 16 k-rows
-      const uint32_t a_step = (g.a.mn_major ? 2048 : 32) >> 4, b_step = (g.b.mn_major ? 2048 : 32) >> 4;
+      constexpr uint32_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
+      const uint32_t tmem_full0 = smem_u32(tmem_full), tmem_empty0 = smem_u32(tmem_empty);
       int s = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -243,7 +263,8 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           const int c1 = min(c0 + g.chain, k1);
           const int buf = local & 1;
           if (local >= 2) {
-            ok = mbar_wait_suspended(&tmem_empty[buf], ((local >> 1) - 1) & 1, g.err, kErrLayer | 2);
+            ok = mbar_wait_suspended(tmem_empty0 + 8 * buf, ((local >> 1) - 1) & 1, g.err,
+                                     kErrLayer | 2);
             if (!ok) break;
           }
           tc_fence_after();
@@ -251,24 +272,21 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           uint32_t acc = 0;
           const int s_first = s;
           auto products = [&](int st, int pa, int pb) {
-            // a descriptor holds the 18 low bits of an address (those above
-            // name the CTA within its cluster)
-            const uint32_t base = (smem_u32(ring) & 0x3ffffu) + st * stage_bytes;
-            const uint64_t da = da0 + ((base + pa * a_bytes) >> 4);
-            const uint64_t db = db0 + ((base + PLANES * a_bytes + pb * b_bytes) >> 4);
+            const uint64_t da = da0 + ((st * stage_bytes + pa * a_bytes) >> 4);
+            const uint64_t db = db0 + ((st * stage_bytes + pb * b_bytes) >> 4);
 #pragma unroll
             for (int k = 0; k < BK / 16; k++) {
-              mma_f16<CG>(d, da + k * a_step, db + k * b_step, idesc, acc);
+              mma_f16<CG>(on, d, da + k * a_step, db + k * b_step, idesc, acc);
               acc = 1;
             }
           };
           for (int kb = c0; kb < c1; kb++) {
-            ok = mbar_wait_suspended(&full[s], phase, g.err, kErrLayer | 3);
+            ok = mbar_wait_suspended(full0 + 8 * s, phase, g.err, kErrLayer | 3);
             if (!ok) break;
             tc_fence_after();
             if (PLANES == 1) {
               products(s, 0, 0);
-              CG == 2 ? mma_commit_pair(&empty[s]) : mma_commit(&empty[s]);
+              mma_commit_cg<CG>(on, empty0 + 8 * s);
             } else {  // the small products of the whole chain first
               products(s, 2, 0);
               products(s, 0, 2);
@@ -282,13 +300,23 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             int t = s_first;
             for (int kb = c0; kb < c1; kb++) {
               products(t, 0, 0);
-              CG == 2 ? mma_commit_pair(&empty[t]) : mma_commit(&empty[t]);
+              mma_commit_cg<CG>(on, empty0 + 8 * t);
               if (++t == S) t = 0;
             }
           }
-          if (ok) CG == 2 ? mma_commit_pair(&tmem_full[buf]) : mma_commit(&tmem_full[buf]);
+          if (ok) mma_commit_cg<CG>(on, tmem_full0 + 8 * buf);
         }
-    }
+    };
+    auto by_layout = [&](auto role) {
+      if (g.a.mn_major)
+        g.b.mn_major ? role(True{}, True{}) : role(True{}, False{});
+      else
+        g.b.mn_major ? role(False{}, True{}) : role(False{}, False{});
+    };
+    if (warp == 0)
+      by_layout(produce);
+    else if (warp == 1 && leader)
+      by_layout(multiply);
   } else {
     if (CG == 2 && RUN) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- epilogue ----------------
@@ -312,7 +340,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       // One lane of four warps polls, and they sleep at a barrier: sixteen
       // polling warps cost the MMAs 4% through the shared memory they share.
       if (q == (kFirstEpi & 3) && lane == 0 && !dead)
-        dead = !mbar_wait_suspended(&tmem_full[chain_no & 1], (chain_no >> 1) & 1, g.err,
+        dead = !mbar_wait_suspended(smem_u32(&tmem_full[chain_no & 1]), (chain_no >> 1) & 1, g.err,
                                     kErrLayer | 4);
       __syncwarp();
       dead = named_bar_or(1 + part, 128, dead);
@@ -392,7 +420,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       if (e.residual) {
         if (!loaded) residual_load(row0, col);
         if (lane == 0 && !dead)
-          dead = !mbar_wait_suspended(res_bar, res_phase, g.err, kErrLayer | 5);
+          dead = !mbar_wait_suspended(smem_u32(res_bar), res_phase, g.err, kErrLayer | 5);
         dead = __any_sync(0xffffffffu, dead);
         res_phase ^= 1;
       } else {
@@ -524,14 +552,20 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             finish16(row0, col0 + c * kSlabCols);
           }
         } else {
-          // the whole tile's sums to shared memory (the ring is free: every
-          // load was waited for, every MMA has completed)
-          float *sums = reinterpret_cast<float *>(ring) + (32 * q + lane) * (BN + 4);
-          if (!dead) {
+          // Every rank owns BN / split columns of the tile; the sums of their
+          // k-ranges go straight to its shared memory.
+          __syncwarp();
+          if (g.split > 1) cluster_sync_all();  // every CTA's ring is free
+          const int own = BN / g.split;  // a multiple of 8
+          const uint32_t mine = smem_u32(sums) + (((int)rank * 128 + 32 * q + lane) * own) * 4;
+          if (!dead && 32 * q + lane < g.M - mb * BM) {
 #pragma unroll
-            for (int j = 0; j < COLS; j += 4)
-              *reinterpret_cast<float4 *>(sums + j) =
-                  make_float4(run[j], run[j + 1], run[j + 2], run[j + 3]);
+            for (int j = 0; j < COLS; j += 4) {
+              const int r = j / own;
+              const uint32_t at = mine + (j - r * own) * 4;
+              st_cluster_f4(g.split > 1 ? map_to_rank(at, r) : at, run[j], run[j + 1], run[j + 2],
+                            run[j + 3]);
+            }
           }
         }
       }
@@ -540,27 +574,28 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
 
   if (CG == 1) {
     __syncwarp();
-    cluster_sync_all();
-    // The cluster's CTAs share out the tile's groups of eight columns; each
-    // adds its groups' sums in rank order and applies the epilogue.
+    if (g.split > 1) {
+      if (warp < kFirstEpi) cluster_sync_all();  // the epilogue warps' first
+      cluster_sync_all();
+    } else {
+      __syncthreads();
+    }
+    // add this rank's columns in rank order and apply the epilogue
     int mb, nb;
     tile_at(first, num_m, num_n, g.group, mb, nb);
     const int rows = min(128, g.M - mb * BM);
-    const int groups = rows * (BN / 8);
-    const int lo = (int)((long long)groups * rank / g.split);
-    const int hi = (int)((long long)groups * (rank + 1) / g.split);
-    const uint32_t sums = smem_u32(ring);
-    for (int i = lo + (int)threadIdx.x; i < hi; i += 192) {
-      const int r = i / (BN / 8), cg = (i % (BN / 8)) * 8;
-      const int col = nb * BN + cg;
+    const int own = BN / g.split, groups = own / 8;
+    for (int i = threadIdx.x; i < rows * groups; i += Block<CG, RUN>::threads) {
+      const int r = i / groups, cg = (i - r * groups) * 8;
+      const int col = nb * BN + (int)rank * own + cg;
       if (col >= g.N) continue;
       float v[8] = {};
-      const uint32_t at = sums + (r * (BN + 4) + cg) * 4;
+#pragma unroll 4
       for (int k = 0; k < g.split; k++) {
-        const uint32_t peer = map_to_rank(at, k);
-        const float4 x = ld_cluster_f4(peer), y = ld_cluster_f4(peer + 16);
-        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-        v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+        float t[8];
+        load8<float>(sums + (k * 128 + r) * own + cg, t);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] += t[j];
       }
       epilogue8<T>(e, mb * BM + r, col, v);
     }
@@ -568,7 +603,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   if (IO && warp >= kFirstEpi && lane == 0) bulk_wait_read();
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();  // no CTA leaves while another may still reach its memory
+  if (CG == 2) cluster_sync_all();  // no CTA leaves while its peer may still reach its memory
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_cg<CG>(tmem_base, 2 * BN);
@@ -699,11 +734,9 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [planes][outer][pitch] of 16-bit elements (without the planes for a pair's
-// 16-bit operands: 2-D loads keep the TMA unit 2% busier); one box is box_rows K-major rows
+// [planes][outer][pitch] of 16-bit elements, or [outer][pitch]; one box is box_rows K-major rows
 // of BK elements, or BK k-rows of 64 MN-major elements.
-static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bool bf16,
-                    bool pair) {
+static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bool bf16) {
   auto fn = encode_fn();
   if (!fn) return set_error(FG_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t pitch = (cuuint64_t)o.pitch * 2;
@@ -713,7 +746,7 @@ static int make_map(CUtensorMap *map, const Operand &o, int bk, int box_rows, bo
                              (cuuint32_t)(o.mn_major ? bk : box_rows), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(
-      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.planes == 1 && pair ? 2 : 3,
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, o.planes == 1 ? 2 : 3,
       const_cast<void *>(o.ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
       o.mn_major || bk == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -770,7 +803,7 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
   if (stages < least) stages = least;
   g.stages = (int)stages;
   size_t bytes = stages * stage + tail;
-  const size_t sums = (size_t)128 * (BN + 4) * 4;
+  const size_t sums = (size_t)128 * BN * 4;
   if (CG == 1 && bytes < sums) bytes = sums;
   bytes += 2048;  // barriers, alignment
   if (bytes < tmem_share(2 * BN)) bytes = tmem_share(2 * BN);
@@ -787,13 +820,15 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
   cfg.blockDim = dim3(Block<CG, RUN>::threads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CG == 2 ? 2 : g.split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, g, e));
   count_launch();
   return FG_OK;
@@ -825,7 +860,7 @@ static int run_form(const Form &f, Maps &maps, ProductArgs g, const Epilogue &e,
   }
   const int64_t ctas = tiles * f.split;
   // more CTAs than SMs: two to an SM, so that one computes while the other joins
-  const size_t cap = ctas > sms ? 92 * 1024 : 190 * 1024;
+  const size_t cap = (ctas > sms ? 92 : 190) * 1024;
   if (f.bn == 128) return launch<T, PLANES, 1, 128, true, false>(maps, g, e, (int)ctas, cap, st);
   return launch<T, PLANES, 1, 64, true, false>(maps, g, e, (int)ctas, cap, st);
 }
@@ -855,9 +890,9 @@ int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, con
   g.b.rows = f.pair ? 128 : f.bn;
   if (f.pair) g.a.rows = 128;
   Maps maps = {};
-  int rc = make_map(&maps.a, a, bk, g.a.rows, bf16, f.pair);
+  int rc = make_map(&maps.a, a, bk, g.a.rows, bf16);
   if (rc) return rc;
-  if ((rc = make_map(&maps.b, b, bk, g.b.rows, bf16, f.pair))) return rc;
+  if ((rc = make_map(&maps.b, b, bk, g.b.rows, bf16))) return rc;
   switch (dtype) {
     case FG_F32:
       return run_form<float, 3>(f, maps, g, e, sms, st);

@@ -58,25 +58,30 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, unsign
   return true;
 }
 
-// mbar_wait whose polls may each suspend the thread for up to a millisecond.
-__device__ __forceinline__ bool mbar_wait_suspended(uint64_t *bar, uint32_t parity,
+// mbar_wait whose polls may each suspend the thread for up to a millisecond,
+// on a barrier given by its shared-memory address.
+__device__ __forceinline__ bool mbar_try_suspended(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_suspended(uint32_t bar, uint32_t parity,
                                                     unsigned int *err, unsigned int code) {
+  if (mbar_try_suspended(bar, parity)) return true;
   const long long t0 = clock64();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
-        : "memory");
-    if (ok) return true;
+  while (!mbar_try_suspended(bar, parity)) {
     if (clock64() - t0 > kWaitLimitCycles) {
       if (err) atomicOr(err, code);
       return false;
     }
   }
+  return true;
 }
 
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *m) {
@@ -251,31 +256,54 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool a
          ((uint32_t)(M >> 4) << 24);
 }
 
+// The instructions below run in the lanes whose `on` is not 0 (one lane of a
+// warp that passes through them whole): predicated, not branched around, so
+// that the compiler keeps their operands in the warp's uniform registers.  A
+// loop in a branch of one lane took 600 cycles a step, mostly to move them.
+
 // D[tmem] (+)= A * B, kind::f16, one CTA or a CTA pair (issued by its leader).
 template <int CG>
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                        uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16(uint32_t on, uint32_t d_tmem, uint64_t adesc,
+                                        uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   if (CG == 1)
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
         : "memory");
 }
 
-// Arrive on the barrier at this shared-memory offset in both CTAs of the pair
-// once every tcgen05 op this thread issued so far completes.
-__device__ __forceinline__ void mma_commit_pair(uint64_t *bar) {
+// Arrive, once every tcgen05 op this thread issued so far completes, on the
+// barrier at this shared-memory address, for a pair in both its CTAs.
+template <int CG>
+__device__ __forceinline__ void mma_commit_cg(uint32_t on, uint32_t bar) {
+  if (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            bar),
+        "r"(on)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster"
+        ".b64 [%0], %1;\n\t}" ::"r"(bar),
+        "h"((uint16_t)3), "r"(on)
+        : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect_tx(uint32_t on, uint32_t bar, uint32_t bytes) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"((uint16_t)3)
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(on)
       : "memory");
 }
 
@@ -317,6 +345,20 @@ __device__ __forceinline__ void cluster_sync_all() {
       "barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
           : "memory");
 }
+__device__ __forceinline__ void st_cluster_f4(uint32_t cluster_addr, float a, float b, float c,
+                                              float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(a),
+               "f"(b), "f"(c), "f"(d)
+               : "memory");
+}
+// Programmatic dependent launch: wait for the stream's previous kernel (and
+// its memory) / let the next kernel start its prologue.
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void grid_launch_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 // Arrive on a barrier given by its shared::cluster address.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
@@ -325,32 +367,45 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 __device__ __forceinline__ void mbar_arrive_local(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(cluster_addr)
-               : "memory");
-  return v;
-}
 
-// Tiled TMA loads into this CTA's own shared memory whose bytes complete on a
-// barrier given by its shared::cluster address (the pair's leader's).
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap *map,
-                                                 uint32_t bar_cluster, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx"
-      "::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_dst),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar_cluster)
-      : "memory");
+// Tiled TMA loads into this CTA's own shared memory.  Of a pair's, the bytes
+// complete on a barrier given by its shared::cluster address (the leader's).
+template <int CG>
+__device__ __forceinline__ void tma_load_2d_cg(uint32_t on, uint32_t smem_dst,
+                                               const CUtensorMap *map, uint32_t bar, int x, int y) {
+  if (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(smem_dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar), "r"(on)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier"
+        "::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(smem_dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar), "r"(on)
+        : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtensorMap *map,
-                                                 uint32_t bar_cluster, int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx"
-      "::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar_cluster)
-      : "memory");
+template <int CG>
+__device__ __forceinline__ void tma_load_3d_cg(uint32_t on, uint32_t smem_dst,
+                                               const CUtensorMap *map, uint32_t bar, int x, int y,
+                                               int z) {
+  if (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(smem_dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier"
+        "::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(smem_dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
+        : "memory");
 }
 
 }  // namespace ptx
