@@ -144,14 +144,16 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tmem_empty + 2);
   uint64_t *res_full = tmem_empty + 4;  // IO: a warp's block of the residual has landed
   uint8_t *ring = smem + 1024;
-  // split: where this rank's columns are summed, [split][128][BN / split], once
-  // the ring is done with
+  // split: where this rank's columns are summed once the ring is done with,
+  // [split][128][BN / split + 4] (rows of different banks)
   float *sums = reinterpret_cast<float *>(ring);
   const uint32_t a_bytes = g.a.rows * (BK * 2), b_bytes = g.b.rows * (BK * 2);
   const uint32_t stage_bytes = PLANES * (a_bytes + b_bytes);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  // (the shuffle tells the compiler that a warp's index is the same in all its
+  // lanes, and so the branches and operands that follow from it)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? blockIdx.x & 1 : blockIdx.x % g.split;  // in the cluster
   const bool leader = CG == 1 || rank == 0;
   const int num_m = (g.M + BM - 1) / BM, num_n = (g.N + BN - 1) / BN;
   const int S = g.stages;
@@ -184,33 +186,33 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   tc_fence_after();
   grid_wait();  // everything above overlaps the previous kernel's end
   if (CG == 1) grid_launch_next();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   // Pair with running sums: 384 threads x 168 registers at launch, of which the epilogue takes
   // 256 x 216 and the others keep 128 x 64.
   if (warp < kFirstEpi) {
     if (CG == 2 && RUN) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // Both loops below run in whole warps with one lane's instructions switched
-    // on, and are instantiated for each pair of layouts.
+    // on, and are instantiated for each pair of layouts.  After a wait that
+    // gave up they run on with everything switched off, so that no branch of
+    // theirs hangs on a barrier's answer.
     const uint32_t on = lane == 0;
+    bool alive = true;
     const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), ring0 = smem_u32(ring);
     auto produce = [&](auto a_layout, auto b_layout) {
       // ---------------- TMA producer ----------------
       const uint32_t bars = CG == 2 ? map_to_rank(full0, 0) : full0;
-      int s = 0, it = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int tile = first; ok && tile < num_m * num_n; tile += step) {
+      int s = 0, it = 0, last = 0;
+      uint32_t phase = 0, go = on;
+      for (int tile = first; tile < num_m * num_n; tile += step) {
         int mb, nb;
         tile_at(tile, num_m, num_n, g.group, mb, nb);
         const int m0 = mb * BM + (CG == 2 ? 128 * (int)rank : 0);
         const int n0 = nb * BN + (CG == 2 ? (BN / 2) * (int)rank : 0);
         for (int kb = k0; kb < k1; kb++, it++) {
-          if (it >= S) {
-            ok = mbar_wait_suspended(empty0 + 8 * s, phase ^ 1, g.err, kErrLayer | 1);
-            if (!ok) break;
-          }
-          if (leader) mbar_expect_tx(on, full0 + 8 * s, CG * stage_bytes);
+          if (it >= S && alive && !mbar_wait_suspended(empty0 + 8 * s, phase ^ 1, g.err, kErrLayer | 1))
+            alive = false, go = 0, last = it;
+          if (leader) mbar_expect_tx(go, full0 + 8 * s, CG * stage_bytes);
           uint32_t dst = ring0 + s * stage_bytes;
           const uint32_t bar = bars + 8 * s;
           auto load = [&](const CUtensorMap *map, auto layout, int rows, int r0, uint32_t bytes) {
@@ -222,9 +224,9 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
                 if (mn && 64 * c >= rows) break;
                 const int x = mn ? r0 + 64 * c : kb * BK, y = mn ? kb * BK : r0;
                 if (PLANES == 1)
-                  tma_load_2d_cg<CG>(on, dst + c * (BK * 128), map, bar, x, y);
+                  tma_load_2d_cg<CG>(go, dst + c * (BK * 128), map, bar, x, y);
                 else
-                  tma_load_3d_cg<CG>(on, dst + c * (BK * 128), map, bar, x, y, p);
+                  tma_load_3d_cg<CG>(go, dst + c * (BK * 128), map, bar, x, y, p);
               }
               dst += bytes;
             }
@@ -237,10 +239,10 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       // After a wait that gave up, loads in flight land before the CTA may
       // end: the leader sees them on its barriers; the peer, whose loads
       // complete on the leader's, lets a millisecond pass.
-      if (!ok && leader)
-        for (int i = it - S < 0 ? 0 : it - S; i < it; i++)
+      if (!alive && leader)
+        for (int i = last - S < 0 ? 0 : last - S; i < last; i++)
           mbar_wait(&full[i % S], (i / S) & 1, nullptr, 0);
-      else if (!ok)
+      else if (!alive)
         for (const long long t0 = clock64(); clock64() - t0 < 2000000;) __nanosleep(1000);
     };
     auto multiply = [&](auto a_layout, auto b_layout) {
@@ -256,17 +258,15 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       constexpr uint32_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
       const uint32_t tmem_full0 = smem_u32(tmem_full), tmem_empty0 = smem_u32(tmem_empty);
       int s = 0, local = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int tile = first; ok && tile < num_m * num_n; tile += step)
-        for (int c0 = k0; ok && c0 < k1; c0 += g.chain, local++) {
+      uint32_t phase = 0, go = on;
+      for (int tile = first; tile < num_m * num_n; tile += step)
+        for (int c0 = k0; c0 < k1; c0 += g.chain, local++) {
           const int c1 = min(c0 + g.chain, k1);
           const int buf = local & 1;
-          if (local >= 2) {
-            ok = mbar_wait_suspended(tmem_empty0 + 8 * buf, ((local >> 1) - 1) & 1, g.err,
-                                     kErrLayer | 2);
-            if (!ok) break;
-          }
+          if (local >= 2 && alive &&
+              !mbar_wait_suspended(tmem_empty0 + 8 * buf, ((local >> 1) - 1) & 1, g.err,
+                                   kErrLayer | 2))
+            alive = false, go = 0;
           tc_fence_after();
           const uint32_t d = tmem_base + buf * BN;
           uint32_t acc = 0;
@@ -276,17 +276,17 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             const uint64_t db = db0 + ((st * stage_bytes + pb * b_bytes) >> 4);
 #pragma unroll
             for (int k = 0; k < BK / 16; k++) {
-              mma_f16<CG>(on, d, da + k * a_step, db + k * b_step, idesc, acc);
+              mma_f16<CG>(go, d, da + k * a_step, db + k * b_step, idesc, acc);
               acc = 1;
             }
           };
           for (int kb = c0; kb < c1; kb++) {
-            ok = mbar_wait_suspended(full0 + 8 * s, phase, g.err, kErrLayer | 3);
-            if (!ok) break;
+            if (alive && !mbar_wait_suspended(full0 + 8 * s, phase, g.err, kErrLayer | 3))
+              alive = false, go = 0;
             tc_fence_after();
             if (PLANES == 1) {
               products(s, 0, 0);
-              mma_commit_cg<CG>(on, empty0 + 8 * s);
+              mma_commit_cg<CG>(go, empty0 + 8 * s);
             } else {  // the small products of the whole chain first
               products(s, 2, 0);
               products(s, 0, 2);
@@ -296,15 +296,15 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             }
             if (++s == S) s = 0, phase ^= 1;
           }
-          if (PLANES == 3 && ok) {
+          if (PLANES == 3) {
             int t = s_first;
             for (int kb = c0; kb < c1; kb++) {
               products(t, 0, 0);
-              mma_commit_cg<CG>(on, empty0 + 8 * t);
+              mma_commit_cg<CG>(go, empty0 + 8 * t);
               if (++t == S) t = 0;
             }
           }
-          if (ok) mma_commit_cg<CG>(on, tmem_full0 + 8 * buf);
+          mma_commit_cg<CG>(go, tmem_full0 + 8 * buf);
         }
     };
     auto by_layout = [&](auto role) {
@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           __syncwarp();
           if (g.split > 1) cluster_sync_all();  // every CTA's ring is free
           const int own = BN / g.split;  // a multiple of 8
-          const uint32_t mine = smem_u32(sums) + (((int)rank * 128 + 32 * q + lane) * own) * 4;
+          const uint32_t mine = smem_u32(sums) + (((int)rank * 128 + 32 * q + lane) * (own + 4)) * 4;
           if (!dead && 32 * q + lane < g.M - mb * BM) {
 #pragma unroll
             for (int j = 0; j < COLS; j += 4) {
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
 #pragma unroll 4
       for (int k = 0; k < g.split; k++) {
         float t[8];
-        load8<float>(sums + (k * 128 + r) * own + cg, t);
+        load8<float>(sums + (k * 128 + r) * (own + 4) + cg, t);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] += t[j];
       }
@@ -803,7 +803,7 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
   if (stages < least) stages = least;
   g.stages = (int)stages;
   size_t bytes = stages * stage + tail;
-  const size_t sums = (size_t)128 * BN * 4;
+  const size_t sums = (size_t)128 * (BN + 4 * g.split) * 4;
   if (CG == 1 && bytes < sums) bytes = sums;
   bytes += 2048;  // barriers, alignment
   if (bytes < tmem_share(2 * BN)) bytes = tmem_share(2 * BN);
