@@ -72,6 +72,12 @@ __global__ void __launch_bounds__(256)
 // without it elements are read one by one, still in neighbouring lanes.
 // ---------------------------------------------------------------------------
 constexpr int kRowsMax = 8;
+// Rows up to which it beats the tensor cores' few-row tiles (4096 x 4096): in
+// f32 8 (22 us against 56, which has to split the weight into planes first),
+// in 16 bits 2, or 4 where the weight would have to be copied to be aligned.
+static int rows_limit(int dtype, bool aligned) {
+  return dtype == FG_F32 ? kRowsMax : aligned ? 2 : 4;
+}
 
 // What a lane reads at once: 16 bytes, or one element.
 template <typename T, bool VEC>
@@ -394,7 +400,7 @@ static int check_common(const char *who, int dtype, int M, int N, int K, int act
 
 // Where a forward product reads its operands, and the workspace that takes.
 struct LinearPlan {
-  bool rows;  // k_linear_rows
+  bool rows, vec;  // k_linear_rows, with 16-byte reads
   Operand x, w;
   StageJobs jobs;
   size_t bytes;
@@ -402,7 +408,10 @@ struct LinearPlan {
 static LinearPlan plan_linear(const fg_linear_args *g) {
   LinearPlan p{};
   if (g->M == 0 || g->N == 0 || g->K == 0) return p;
-  p.rows = g->M <= kRowsMax && (g->x_col == 1 || g->K == 1) && (g->w_col == 1 || g->K == 1);
+  const int es = elem_size(g->dtype);
+  p.vec = rows16(g->x, g->M == 1 ? 0 : g->x_row, es) && rows16(g->w, g->w_row, es);
+  p.rows = g->M <= rows_limit(g->dtype, p.vec) && (g->x_col == 1 || g->K == 1) &&
+           (g->w_col == 1 || g->K == 1);
   if (p.rows) return p;
   p.x = resolve_operand(g->dtype, {g->x, g->x_row, g->x_col}, g->M, g->K, &p.jobs, &p.bytes);
   p.w = resolve_operand(g->dtype, {g->w, g->w_row, g->w_col}, g->N, g->K, &p.jobs, &p.bytes);
@@ -459,15 +468,13 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
           rows16(e.out, e.ldo, es);
   if (g->K == 0) return run_empty_product(g->dtype, e, st);
   if (p.rows) {
-    const bool vec = (g->M == 1 || g->x_row * es % 16 == 0) && g->w_row * es % 16 == 0 &&
-                     (uintptr_t)g->x % 16 == 0 && (uintptr_t)g->w % 16 == 0;
     switch (g->dtype) {
       case FG_F32:
-        return run_rows<float>(g, e, vec, st);
+        return run_rows<float>(g, e, p.vec, st);
       case FG_BF16:
-        return run_rows<__nv_bfloat16>(g, e, vec, st);
+        return run_rows<__nv_bfloat16>(g, e, p.vec, st);
       default:
-        return run_rows<__half>(g, e, vec, st);
+        return run_rows<__half>(g, e, p.vec, st);
     }
   }
   place_operand(&p.x, g->workspace);

@@ -63,6 +63,7 @@ struct ProductArgs {
   int M, N, nk;      // nk: k-blocks
   int chain;         // k-blocks of one accumulation chain
   int stages, split, group;
+  int join_at;       // split: offset from the ring of the joined sums
   int bf16;
   OperandLayout a, b;
   unsigned int *err;
@@ -144,9 +145,12 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tmem_empty + 2);
   uint64_t *res_full = tmem_empty + 4;  // IO: a warp's block of the residual has landed
   uint8_t *ring = smem + 1024;
-  // split: where this rank's columns are summed once the ring is done with,
-  // [split][128][BN / split + 4] (rows of different banks)
-  float *sums = reinterpret_cast<float *>(ring);
+  // split: a CTA's sums go where its ring was, [BN / 4][row] of float4; each
+  // rank's share of the columns, BN / split, is then copied to that rank's
+  // `joined`, [source rank][BN / split / 4][row], completing on `join_bar`
+  uint64_t *join_bar = tmem_empty + 4;
+  float4 *sums = reinterpret_cast<float4 *>(ring);
+  float4 *joined = reinterpret_cast<float4 *>(ring + (g.split > 1 ? g.join_at : 0));
   const uint32_t a_bytes = g.a.rows * (BK * 2), b_bytes = g.b.rows * (BK * 2);
   const uint32_t stage_bytes = PLANES * (a_bytes + b_bytes);
 
@@ -175,6 +179,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
     }
     if (IO)
       for (int i = 0; i < kEpiWarps; i++) mbar_init(&res_full[i], 1);
+    if (CG == 1) mbar_init(join_bar, 1);
     fence_mbar_init();
     prefetch_tmap(&tma);
     prefetch_tmap(&tmb);
@@ -183,6 +188,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync_all();  // the peer's barriers and TMEM are ready
+  if (CG == 1 && g.split > 1) cluster_arrive();  // waited for before the first copy to a peer
   tc_fence_after();
   grid_wait();  // everything above overlaps the previous kernel's end
   if (CG == 1) grid_launch_next();
@@ -552,19 +558,23 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             finish16(row0, col0 + c * kSlabCols);
           }
         } else {
-          // Every rank owns BN / split columns of the tile; the sums of their
-          // k-ranges go straight to its shared memory.
-          __syncwarp();
-          if (g.split > 1) cluster_sync_all();  // every CTA's ring is free
-          const int own = BN / g.split;  // a multiple of 8
-          const uint32_t mine = smem_u32(sums) + (((int)rank * 128 + 32 * q + lane) * (own + 4)) * 4;
-          if (!dead && 32 * q + lane < g.M - mb * BM) {
+          const int pitch = (min(128, g.M - mb * BM) + 7) & ~7;  // rows, a multiple of 8
+          const int row = 32 * q + lane;
+          if (!dead && row < pitch) {
 #pragma unroll
-            for (int j = 0; j < COLS; j += 4) {
-              const int r = j / own;
-              const uint32_t at = mine + (j - r * own) * 4;
-              st_cluster_f4(g.split > 1 ? map_to_rank(at, r) : at, run[j], run[j + 1], run[j + 2],
-                            run[j + 3]);
+            for (int j = 0; j < COLS; j += 4)
+              sums[j / 4 * pitch + row] = make_float4(run[j], run[j + 1], run[j + 2], run[j + 3]);
+          }
+          if (g.split > 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            cluster_wait();  // the peers have started: their barriers are set up
+            if (!named_bar_or(1, 128, dead) && warp == kFirstEpi && lane < g.split) {
+              const uint32_t bytes = BN / g.split / 4 * pitch * 16;
+              const uint32_t bar = smem_u32(join_bar);
+              if (lane == 0) mbar_arrive_expect_tx(join_bar, g.split * bytes);
+              bulk_copy_to_cta(map_to_rank(smem_u32(joined) + rank * bytes, lane),
+                               smem_u32(sums) + lane * bytes, bytes, map_to_rank(bar, lane));
             }
           }
         }
@@ -575,27 +585,33 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   if (CG == 1) {
     __syncwarp();
     if (g.split > 1) {
-      if (warp < kFirstEpi) cluster_sync_all();  // the epilogue warps' first
-      cluster_sync_all();
+      if (warp < kFirstEpi) cluster_wait();
+      mbar_wait(join_bar, 0, g.err, kErrLayer | 6);
+      __syncwarp();
+      cluster_arrive();  // (every copy into this CTA is done; waited for at the end)
     } else {
       __syncthreads();
     }
     // add this rank's columns in rank order and apply the epilogue
     int mb, nb;
     tile_at(first, num_m, num_n, g.group, mb, nb);
-    const int rows = min(128, g.M - mb * BM);
+    const int rows = min(128, g.M - mb * BM), pitch = (rows + 7) & ~7;
     const int own = BN / g.split, groups = own / 8;
-    for (int i = threadIdx.x; i < rows * groups; i += Block<CG, RUN>::threads) {
-      const int r = i / groups, cg = (i - r * groups) * 8;
+    // a warp takes gw groups of eight columns of 32 / gw rows at a time: eight
+    // lanes read 128 neighbouring bytes, gw lanes write a row's
+    const int gw = groups < 4 ? groups : 4, rw = 32 / gw, across = groups / gw;
+    for (int t = warp; t < (rows + rw - 1) / rw * across; t += Block<CG, RUN>::threads / 32) {
+      const int r = t / across * rw + lane % rw;
+      const int cg = (t % across * gw + lane / rw) * 8;
       const int col = nb * BN + (int)rank * own + cg;
-      if (col >= g.N) continue;
+      if (r >= rows || col >= g.N) continue;
       float v[8] = {};
 #pragma unroll 4
       for (int k = 0; k < g.split; k++) {
-        float t[8];
-        load8<float>(sums + (k * 128 + r) * (own + 4) + cg, t);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] += t[j];
+        const float4 *x = joined + (k * (own / 4) + cg / 4) * pitch + r;
+        const float4 lo = x[0], hi = x[pitch];
+        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+        v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
       }
       epilogue8<T>(e, mb * BM + r, col, v);
     }
@@ -603,7 +619,9 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   if (IO && warp >= kFirstEpi && lane == 0) bulk_wait_read();
   tc_fence_before();
   __syncthreads();
-  if (CG == 2) cluster_sync_all();  // no CTA leaves while its peer may still reach its memory
+  // no CTA leaves while another may still reach its memory
+  if (CG == 2) cluster_sync_all();
+  if (CG == 1 && g.split > 1) cluster_wait();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_cg<CG>(tmem_base, 2 * BN);
@@ -803,8 +821,12 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
   if (stages < least) stages = least;
   g.stages = (int)stages;
   size_t bytes = stages * stage + tail;
-  const size_t sums = (size_t)128 * (BN + 4 * g.split) * 4;
-  if (CG == 1 && bytes < sums) bytes = sums;
+  if (CG == 1) {
+    const size_t sums = (size_t)((g.M < 128 ? g.M + 7 : 128) & ~7) * BN * 4;
+    if (bytes < sums) bytes = sums;
+    g.join_at = (int)((bytes + 127) & ~(size_t)127);
+    if (g.split > 1) bytes = g.join_at + sums;
+  }
   bytes += 2048;  // barriers, alignment
   if (bytes < tmem_share(2 * BN)) bytes = tmem_share(2 * BN);
   static bool attr_done[64] = {};
@@ -860,7 +882,8 @@ static int run_form(const Form &f, Maps &maps, ProductArgs g, const Epilogue &e,
   }
   const int64_t ctas = tiles * f.split;
   // more CTAs than SMs: two to an SM, so that one computes while the other joins
-  const size_t cap = (ctas > sms ? 92 : 190) * 1024;
+  size_t cap = (ctas > sms ? 92 : 190) * 1024;
+  if (f.split > 1) cap -= (size_t)(g.M < 128 ? g.M : 128) * f.bn * 4;  // the joined sums
   if (f.bn == 128) return launch<T, PLANES, 1, 128, true, false>(maps, g, e, (int)ctas, cap, st);
   return launch<T, PLANES, 1, 64, true, false>(maps, g, e, (int)ctas, cap, st);
 }
@@ -903,26 +926,33 @@ int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, con
   }
 }
 
-// The form with the least estimated time, in MMA cycles of an SM: a k-block
-// costs its MMAs, a tile about 2000 cycles around them (start-up, the last
-// chain's drain, the epilogue), and CTAs run in waves.
+// The form with the least estimated time, in microseconds.  Measured on one
+// B200 over 17 shapes from 24 x 64 x 2048 to 2048 x 2048 x 2048 in bf16 and f32,
+// every form of each: an MMA step (16 deep) costs a pair 0.07 and a lone CTA
+// 0.052 at either width; around them a pair spends 6.8, a lone CTA 1.8 and its
+// epilogue 2.8 or 4.8 for 128 rows; joining a cluster's sums costs 1.  The
+// 64-wide CTAs run two to an SM and hide each other's fixed part.  It picks the
+// fastest form or one within 10% of it on 15 of the 17 (24 x 8192 x 2048 f16:
+// 64 wide, k over 8 CTAs, 10.6 against 32.3 unsplit; 1024 x 4096 x 4096: pairs,
+// 26.2 against 52.1).
 Form pick_form(int M, int N, int K, int planes, int sms) {
-  const double per_k = (planes == 3 ? 6.0 : 1.0) / 16.0;  // MMA steps per k
-  auto waves = [](double n, double slots) { return ceil(n / slots); };
+  const double steps = K / 16.0 * (planes == 3 ? 6.0 : 1.0);
   Form best{true, 256, 256, 1};
-  const double t2 = ceil(M / 256.0) * ceil(N / 256.0);
-  double cost = waves(t2, sms / 2) * (K * per_k * 128.0) + 6000.0;
+  const double pairs = ceil(M / 256.0) * ceil(N / 256.0);
+  double cost = ceil(pairs / (sms / 2)) * steps * 0.07 + 6.8;
   const int bk = planes == 3 ? 32 : 64;
   const int nk = (int)((K + (int64_t)bk - 1) / bk);
-  for (int bn = 128; bn >= 64; bn /= 2)
-    for (int split = 1; split <= 8; split *= 2) {
-      if (split > nk) break;
+  const double rows = M < 128 ? M / 128.0 : 1.0;
+  for (int bn = 64; bn <= 128; bn *= 2)
+    // (128-wide CTAs run one to an SM, and not enough clusters of 8 then fit)
+    for (int split = 1; split <= (bn == 64 ? 8 : 4) && split <= nk; split *= 2) {
       const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
       if (ctas > 1e8) continue;
-      // a lone CTA's MMAs read shared memory faster than it delivers
-      const double step = bn == 128 ? 84.0 : 52.0;
-      const double c = waves(ctas, sms) * ((double)K / split * per_k * step + 2500.0) +
-                       (split > 1 ? 1500.0 : 0.0) + 2000.0;
+      const double fixed = 1.8 + rows * (bn == 64 ? 2.8 : 4.8);
+      const int resident = bn == 64 ? 2 : 1;
+      const double load = bn == 64 ? (ctas > sms ? ctas / sms : 1.0) : ceil(ctas / sms);
+      const double c = 1.5 + (split > 1 ? 1.0 : 0.0) + ceil(ctas / (resident * sms)) * fixed +
+                       load * steps / split * 0.052;
       if (c < cost) {
         cost = c;
         best = Form{false, 128, bn, split};
