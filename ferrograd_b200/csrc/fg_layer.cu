@@ -12,6 +12,7 @@
 
 #include "fg_internal.h"
 #include "fg_layer.cuh"
+#include "fg_ptx.cuh"
 
 namespace fg {
 namespace layer {
@@ -71,6 +72,9 @@ __global__ void __launch_bounds__(256)
 // us against 7.6 us here.)  VEC: every row starts on a 16-byte boundary;
 // without it elements are read one by one, still in neighbouring lanes.
 // ---------------------------------------------------------------------------
+using ptx::grid_launch_next;
+using ptx::grid_wait;
+
 constexpr int kRowsMax = 8;
 // Rows up to which it beats the tensor cores' few-row tiles (4096 x 4096): in
 // f32 8 (22 us against 56, which has to split the weight into planes first),
@@ -217,36 +221,62 @@ __device__ __forceinline__ void store_dz<float>(void *dz, int64_t at, int64_t pl
   for (int k = 0; k < 3; k++) store8(static_cast<__nv_bfloat16 *>(dz) + k * plane + at, p[k]);
 }
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
     k_layer_dz(const T *__restrict__ dy, int64_t yr, int64_t yc, const T *__restrict__ pre,
                int64_t ldp, int act, const DropParams drop, void *__restrict__ dz, int64_t ldz,
                float *__restrict__ part, int M, int N, int rows, int vec) {
   __shared__ float red[8][256];
+  constexpr int U = 2;  // rows in flight, and as many again asked for
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * 256 + lane * 8;
   const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
-  const bool whole = vec && col + 8 <= N;
   float sum[8] = {};
-  if (col < N)
+  grid_wait();
+  grid_launch_next();
+  auto one = [&](int r, float(&v)[8], const float(&z)[8]) {
+    if (drop.on) drop8(drop, r, col, v);
+    slope8<sizeof(T) == 2>(v, z, act);
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum[i] += v[i];
+    // ldz is a multiple of 8 and the rest of a row's last group is 0
+    if (dz) store_dz<T>(dz, r * ldz + col, (int64_t)M * ldz, v);
+  };
+  if (vec && col + 8 <= N) {
+    Raw8<T> y[U], p[U], yn[U], pn[U];
+    auto ask = [&](int r, Raw8<T>(&a)[U], Raw8<T>(&b)[U]) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (r + 8 * u < r1) {
+          a[u].load(dy + (r + 8 * u) * yr + col);
+          if (act != FG_ACT_NONE) b[u].load(pre + (r + 8 * u) * ldp + col);
+        }
+    };
+    ask(r0 + warp, y, p);
+    for (int r = r0 + warp; r < r1; r += 8 * U) {
+      ask(r + 8 * U, yn, pn);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (r + 8 * u < r1) {
+          float v[8], z[8];
+          y[u].get(v);
+          p[u].get(z);
+          one(r + 8 * u, v, z);
+        }
+        y[u] = yn[u];
+        p[u] = pn[u];
+      }
+    }
+  } else if (col < N) {
     for (int r = r0 + warp; r < r1; r += 8) {
       float v[8], z[8];
-      if (whole) {
-        load8<T>(dy + r * yr + col, v);
-        if (act != FG_ACT_NONE) load8<T>(pre + r * ldp + col, z);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          v[i] = col + i < N ? to_f32<T>(dy[r * yr + (col + i) * yc]) : 0.0f;
-          z[i] = act != FG_ACT_NONE && col + i < N ? to_f32<T>(pre[r * ldp + col + i]) : 0.0f;
-        }
+      for (int i = 0; i < 8; i++) {
+        v[i] = col + i < N ? to_f32<T>(dy[r * yr + (col + i) * yc]) : 0.0f;
+        z[i] = act != FG_ACT_NONE && col + i < N ? to_f32<T>(pre[r * ldp + col + i]) : 0.0f;
       }
-      if (drop.on) drop8(drop, r, col, v);
-      slope8<sizeof(T) == 2>(v, z, act);
-#pragma unroll
-      for (int i = 0; i < 8; i++) sum[i] += v[i];
-      // ldz is a multiple of 8 and the rest of a row's last group is 0
-      if (dz) store_dz<T>(dz, r * ldz + col, (int64_t)M * ldz, v);
+      one(r, v, z);
     }
+  }
   if (!part) return;
 #pragma unroll
   for (int i = 0; i < 8; i++) red[warp][lane * 8 + i] = sum[i];
@@ -264,8 +294,11 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     k_bias_grad(const float *__restrict__ part, int chunks, int N, T *__restrict__ db) {
   const int c = blockIdx.x * 256 + threadIdx.x;
+  grid_wait();
+  grid_launch_next();
   if (c >= N) return;
   float s = 0.0f;
+#pragma unroll 8
   for (int i = 0; i < chunks; i++) s += part[(size_t)i * N + c];
   db[c] = from_f32<T>(s);
 }
@@ -273,38 +306,65 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // out = residual + D(x): eight columns of a row a step.
 // ---------------------------------------------------------------------------
+// Groups of eight columns a thread takes, 256 groups apart.
 template <typename T>
-__global__ void __launch_bounds__(256)
-    k_dropout(const T *x, int64_t ldx, const T *residual, int64_t ldr, T *out,
-              int64_t ldo, const DropParams drop, int64_t rows, int cols, int vec) {
-  const int64_t groups = (cols + 7) / 8, all = rows * groups;
-  for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < all;
-       g += (int64_t)gridDim.x * 256) {
-    const int64_t r = g / groups;
-    const int col = (int)(g - r * groups) * 8;
-    const bool whole = vec && col + 8 <= cols;
-    float v[8], t[8];
-    if (whole) {
-      load8<T>(x + r * ldx + col, v);
-      if (residual) load8<T>(residual + r * ldr + col, t);
-    } else {
+struct DropGroups {
+  static constexpr int value = sizeof(T) == 2 ? 4 : 2;
+};
+
+// A group of n <= 8 columns, element by element.
+template <typename T>
+__device__ __forceinline__ void drop_tail(const T *x, const T *residual, T *out,
+                                          const DropParams &drop, int64_t row, int col, int n) {
+  float v[8], t[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        v[i] = col + i < cols ? to_f32<T>(x[r * ldx + col + i]) : 0.0f;
-        t[i] = residual && col + i < cols ? to_f32<T>(residual[r * ldr + col + i]) : 0.0f;
+  for (int i = 0; i < 8; i++) {
+    v[i] = i < n ? to_f32<T>(x[i]) : 0.0f;
+    t[i] = residual && i < n ? to_f32<T>(residual[i]) : 0.0f;
+  }
+  if (drop.on) drop8(drop, (uint32_t)row, col, v);
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < n) out[i] = from_f32<T>(residual ? v[i] + t[i] : v[i]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 4)
+    k_dropout(const T *x, int64_t ldx, const T *residual, int64_t ldr, T *out, int64_t ldo,
+              const DropParams drop, int64_t rows, int cols, int vec) {
+  constexpr int U = DropGroups<T>::value;
+  Walk at(rows, (cols + 7) / 8, (int64_t)blockIdx.x * (256 * U) + threadIdx.x, 256);
+  grid_wait();
+  grid_launch_next();
+  Raw8<T> a[U], b[U];
+  int64_t row[U];
+  int col[U];
+#pragma unroll
+  for (int u = 0; u < U; u++, at.next()) {  // every load first
+    row[u] = at.row;
+    col[u] = at.group * 8;
+    if (vec && at.inside() && col[u] + 8 <= cols) {
+      a[u].load(x + row[u] * ldx + col[u]);
+      if (residual) b[u].load(residual + row[u] * ldr + col[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    if (row[u] >= rows) return;
+    T *o = out + row[u] * ldo + col[u];
+    if (vec && col[u] + 8 <= cols) {
+      float v[8], t[8];
+      a[u].get(v);
+      if (drop.on) drop8(drop, (uint32_t)row[u], col[u], v);
+      if (residual) {
+        b[u].get(t);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] += t[i];
       }
-    }
-    if (drop.on) drop8(drop, (uint32_t)r, col, v);
-    if (residual) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] += t[i];
-    }
-    if (whole) {
-      store8<T>(out + r * ldo + col, v);
+      store8<T>(o, v);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (col + i < cols) out[r * ldo + col + i] = from_f32<T>(v[i]);
+      drop_tail(x + row[u] * ldx + col[u], residual ? residual + row[u] * ldr + col[u] : nullptr, o,
+                drop, row[u], col[u], min(8, cols - col[u]));
     }
   }
 }
@@ -325,8 +385,10 @@ static int make_drop(const char *who, const fg_dropout_spec *s, DropParams *d) {
   d->some = t < 65536;
   d->threshold_hi = t << 16;
   d->scale = d->some ? (float)(65536.0 / (65536 - t)) : 0.0f;
-  d->k0 = (uint32_t)s->seed;
-  d->k1 = (uint32_t)(s->seed >> 32);
+  for (uint32_t r = 0; r < 10; r++) {
+    d->k0[r] = (uint32_t)s->seed + r * 0x9E3779B9u;
+    d->k1[r] = (uint32_t)(s->seed >> 32) + r * 0xBB67AE85u;
+  }
   d->c2 = (uint32_t)s->offset;
   d->c3 = (uint32_t)(s->offset >> 32);
   return FG_OK;
@@ -484,15 +546,14 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
   return run_tensor_product(g->dtype, p.x, p.w, g->K, e, st);
 }
 
-// Rows of a block of k_layer_dz: about four blocks an SM, at least 64 rows.
+// Rows of a block of k_layer_dz: enough blocks for several waves, at most 128
+// partial sums a column, at least 64 rows.
 static int dz_rows(int M, int N) {
-  const int strips = (int)((N + 255LL) / 256);
-  const int want = strips >= 592 ? 1 : 592 / strips;
-  int rows = (int)((M + (int64_t)want - 1) / want);
-  rows = (rows + 7) / 8 * 8;
-  if (rows < 64) rows = 64;
-  while ((M + (int64_t)rows - 1) / rows > 65535) rows *= 2;
-  return rows;
+  const int64_t strips = (N + 255LL) / 256;
+  int64_t chunks = strips >= 4096 ? 1 : 4096 / strips;
+  if (chunks > 128) chunks = 128;
+  int64_t rows = ((M + chunks - 1) / chunks + 7) / 8 * 8;
+  return (int)(rows < 64 ? 64 : rows);
 }
 
 // dz is written (in a 16-bit type, or as the three planes of f32) where a
@@ -555,17 +616,16 @@ static int run_dz(const fg_linear_grad_args *g, const GradPlan &p, const DropPar
   if (p.make_dz || part) {
     const int vec = g->dy_col == 1 && rows16(g->dy, g->dy_row, es) &&
                     (g->act == FG_ACT_NONE || rows16(g->pre, g->ld_pre, es));
-    k_layer_dz<T><<<dim3((unsigned)((g->N + 255LL) / 256), p.chunks), 256, 0, st>>>(
-        static_cast<const T *>(g->dy), g->dy_row, g->dy_col, static_cast<const T *>(g->pre),
-        g->ld_pre, g->act, drop, p.make_dz ? ws + p.dz_off : nullptr, p.ldz, part, g->M, g->N,
-        p.rows, vec);
-    FG_LAUNCH_TRY();
+    int rc = launch_early(k_layer_dz<T>, dim3((unsigned)((g->N + 255LL) / 256), p.chunks), 256, st,
+                          static_cast<const T *>(g->dy), g->dy_row, g->dy_col,
+                          static_cast<const T *>(g->pre), g->ld_pre, g->act, drop,
+                          p.make_dz ? ws + p.dz_off : nullptr, p.ldz, part, g->M, g->N, p.rows,
+                          vec);
+    if (rc) return rc;
   }
-  if (g->db) {
-    k_bias_grad<T><<<(unsigned)((g->N + 255LL) / 256), 256, 0, st>>>(part, p.chunks, g->N,
-                                                                     static_cast<T *>(g->db));
-    FG_LAUNCH_TRY();
-  }
+  if (g->db)
+    return launch_early(k_bias_grad<T>, dim3((unsigned)((g->N + 255LL) / 256)), 256, st, part,
+                        p.chunks, g->N, static_cast<T *>(g->db));
   return FG_OK;
 }
 
@@ -685,26 +745,20 @@ static int dropout(int dtype, int64_t rows, int64_t cols, const void *x, int64_t
              "%s: out overlaps the residual (it may only be all of it)", who);
   const int vec = rows16(x, ldx, es) && rows16(residual, ldr, es) && rows16(out, ldo, es);
   const int64_t groups = rows * ((cols + 7) / 8);
-  const int64_t want = (groups + 255) / 256, cap = 148 * 8;
-  const unsigned grid = (unsigned)(want < cap ? want : cap);
-  switch (dtype) {
-    case FG_F32:
-      k_dropout<float><<<grid, 256, 0, st>>>(
-          static_cast<const float *>(x), ldx, static_cast<const float *>(residual), ldr,
-          static_cast<float *>(out), ldo, d, rows, (int)cols, vec);
-      break;
-    case FG_BF16:
-      k_dropout<__nv_bfloat16><<<grid, 256, 0, st>>>(
-          static_cast<const __nv_bfloat16 *>(x), ldx, static_cast<const __nv_bfloat16 *>(residual),
-          ldr, static_cast<__nv_bfloat16 *>(out), ldo, d, rows, (int)cols, vec);
-      break;
-    default:
-      k_dropout<__half><<<grid, 256, 0, st>>>(
-          static_cast<const __half *>(x), ldx, static_cast<const __half *>(residual), ldr,
-          static_cast<__half *>(out), ldo, d, rows, (int)cols, vec);
-  }
-  FG_LAUNCH_TRY();
-  return FG_OK;
+  const int64_t per = 256 * (es == 2 ? DropGroups<__half>::value : DropGroups<float>::value);
+  const int64_t blocks = (groups + per - 1) / per;
+  FG_REQUIRE(blocks <= 0x7fffffffLL, "%s: %lld x %lld is out of range", who, (long long)rows,
+             (long long)cols);
+  const dim3 grid((unsigned)blocks);
+  auto go = [&](auto kern, auto type) {
+    using T = decltype(type);
+    return launch_early(kern, grid, 256, st, static_cast<const T *>(x), ldx,
+                        static_cast<const T *>(residual), ldr, static_cast<T *>(out), ldo, d, rows,
+                        (int)cols, vec);
+  };
+  if (dtype == FG_F32) return go(k_dropout<float>, float{});
+  if (dtype == FG_BF16) return go(k_dropout<__nv_bfloat16>, __nv_bfloat16{});
+  return go(k_dropout<__half>, __half{});
 }
 
 }  // namespace layer

@@ -86,6 +86,32 @@ __device__ __forceinline__ void load8<float>(const float *p, float (&v)[8]) {
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
   v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
+// The same in two steps, so that a loop can ask for its next elements before
+// it computes with the present ones.
+template <typename T>
+struct Raw8 {
+  uint4 q[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) q[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+      const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (sizeof(T) == 4) {
+          v[4 * i + j] = __uint_as_float(w[j]);
+        } else {
+          const float2 f = unpack2(w[j], typename Half16<T>::type{});
+          v[2 * j] = f.x;
+          v[2 * j + 1] = f.y;
+        }
+      }
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
   uint4 u;
@@ -107,9 +133,16 @@ __device__ __forceinline__ void store8<float>(float *p, const float (&v)[8]) {
 // of 0 and infinity are kept out by bounding z from below where exp(-z) would
 // overflow, and from both sides where a slope multiplies z by a vanishing
 // factor.
-__device__ __forceinline__ float bound_below(float z, float lo) { return z < lo ? lo : z; }
+__device__ __forceinline__ float bound_below(float z, float lo) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(lo));
+  return r;
+}
 __device__ __forceinline__ float bound_both(float z, float lim) {
-  return z < -lim ? -lim : (z > lim ? lim : z);
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(-lim));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(lim));
+  return r;
 }
 
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
@@ -131,8 +164,8 @@ struct Math<false> {
     return 0.5f * erfcf(z * -0.70710678118654752f);
   }
   static __device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
-  static __device__ __forceinline__ float gauss(float z) {  // exp(-z^2 / 2)
-    return expf(-0.5f * z * z);
+  static __device__ __forceinline__ float gelu_slope(float z) {
+    return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), phi(z));
   }
 };
 template <>
@@ -167,8 +200,21 @@ struct Math<true> {
   static __device__ __forceinline__ float logistic(float z) {
     return rcp(1.0f + ex2(z * -1.4426950408889634f));
   }
-  static __device__ __forceinline__ float gauss(float z) {
-    return ex2(z * z * -0.72134752044448170f);
+  // Phi(z) + z phi(z) from one exponential: with x = |z| and s = Phi(-x) - x
+  // phi(x), it is s to the left of 0 and 1 - s to the right.  Phi by 7.1.26,
+  // erfc(y) = (a1 t + ... + a5 t^5) exp(-y^2), t = 1 / (1 + 0.3275911 y), off by
+  // 1.5e-7 at most; y = x / sqrt(2).
+  static __device__ __forceinline__ float gelu_slope(float z) {
+    const float x = fabsf(z);
+    const float t = rcp(fmaf(0.23164189f, x, 1.0f));
+    const float g = ex2(x * x * -0.72134752044448170f);
+    float p = 0.5307027145f;
+    p = fmaf(p, t, -0.7265760135f);
+    p = fmaf(p, t, 0.7107068705f);
+    p = fmaf(p, t, -0.142248368f);
+    p = fmaf(p, t, 0.127414796f);
+    const float s = g * fmaf(p, t, x * -0.3989422804014327f);
+    return z > 0.0f ? 1.0f - s : s;
   }
 };
 
@@ -222,7 +268,7 @@ __device__ __forceinline__ void slope8(float (&v)[8], const float (&z)[8], int a
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const float b = bound_both(z[i], 32.0f);
-        v[i] *= fmaf(b * 0.3989422804014327f, F::gauss(b), F::phi(b));
+        v[i] *= F::gelu_slope(b);
       }
       break;
     case FG_ACT_GELU_TANH:
@@ -258,21 +304,19 @@ struct DropParams {
   int some;               // t < 65536: something is kept
   uint32_t threshold_hi;  // t << 16 (some)
   float scale;            // 65536 / (65536 - t)
-  uint32_t k0, k1;     // seed
-  uint32_t c2, c3;     // offset
+  uint32_t c2, c3;        // offset
+  uint32_t k0[10], k1[10];  // the rounds' keys: seed + round * (0x9E3779B9, 0xBB67AE85)
 };
 
-__device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3,
-                                        uint32_t k0, uint32_t k1) {
+__device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, const DropParams &d) {
+  uint32_t c2 = d.c2, c3 = d.c3;
 #pragma unroll
   for (int r = 0; r < 10; r++) {
     const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ d.k0[r];
     c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ d.k1[r];
     c3 = (uint32_t)p0;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
@@ -286,7 +330,7 @@ __device__ __forceinline__ void drop8(const DropParams &d, uint32_t row, uint32_
     for (int i = 0; i < 8; i++) v[i] = 0.0f;
     return;
   }
-  const uint4 r = philox(col >> 3, row, d.c2, d.c3, d.k0, d.k1);
+  const uint4 r = philox(col >> 3, row, d);
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
   // r16 >= t, with r16 in the upper half of a word and anything below it
 #pragma unroll
@@ -413,6 +457,52 @@ __device__ __forceinline__ void epilogue1(const Epilogue &e, int row, int col, f
   if (e.residual)
     z += to_f32<T>(static_cast<const T *>(e.residual)[(int64_t)row * e.ldr + col]);
   static_cast<T *>(e.out)[(int64_t)row * e.ldo + col] = from_f32<T>(z);
+}
+
+// Walks a rows x groups array from a thread's first piece in equal steps, with
+// a division at the start only: (row, group) of the next piece.
+struct Walk {
+  int64_t row, rows, step_row;
+  int group, groups, step_group;
+  __device__ Walk(int64_t rows_, int groups_, int64_t at, int64_t step)
+      : rows(rows_), groups(groups_) {
+    if (at < 0x7fffffff && step < 0x7fffffff) {
+      row = (uint32_t)at / (uint32_t)groups;
+      step_row = (uint32_t)step / (uint32_t)groups;
+    } else {
+      row = at / groups;
+      step_row = step / groups;
+    }
+    group = (int)(at - row * groups);
+    step_group = (int)(step - step_row * groups);
+  }
+  __device__ bool inside() const { return row < rows; }
+  __device__ void next() {
+    row += step_row;
+    group += step_group;
+    if (group >= groups) {
+      group -= groups;
+      row++;
+    }
+  }
+};
+
+// Launches a kernel whose blocks begin with grid_wait() (fg_ptx.cuh), so that
+// it may start while the stream's previous kernel ends.
+template <typename... P, typename... A>
+int launch_early(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
+  count_launch();
+  return FG_OK;
 }
 
 // A matrix operand: element (r, c) at ptr[r * row + c * col].

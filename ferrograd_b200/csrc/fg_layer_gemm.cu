@@ -661,14 +661,16 @@ __device__ __forceinline__ void stage8(const T *src, int64_t so, int64_t si, int
 template <typename T>
 __global__ void __launch_bounds__(256) k_stage(const StageJobs jobs) {
   const StageJob &j = jobs.job[blockIdx.y];
-  const int64_t groups = j.pitch / 8, all = groups * j.outer;
+  const int groups = (int)(j.pitch / 8);
+  const int64_t plane = groups * j.outer;
   const T *src = static_cast<const T *>(j.src);
   uint4 *dst = static_cast<uint4 *>(j.dst);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t o = i / groups, x = (i - o * groups) * 8;
-    stage8<T>(src, j.so, j.si, o, x, j.inner, j.vec, dst + i, groups * j.outer);
-  }
+  grid_wait();
+  grid_launch_next();
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  for (Walk at(j.outer, groups, first, step); at.inside(); at.next())
+    stage8<T>(src, j.so, j.si, at.row, (int64_t)at.group * 8, j.inner, j.vec,
+              dst + at.row * groups + at.group, plane);
 }
 
 int run_stage(int dtype, const StageJobs &jobs, cudaStream_t st) {
@@ -680,14 +682,9 @@ int run_stage(int dtype, const StageJobs &jobs, cudaStream_t st) {
   }
   const int64_t want = (most + 255) / 256;
   const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8), jobs.n);
-  if (dtype == FG_F32)
-    k_stage<float><<<grid, 256, 0, st>>>(jobs);
-  else if (dtype == FG_BF16)
-    k_stage<__nv_bfloat16><<<grid, 256, 0, st>>>(jobs);
-  else
-    k_stage<__half><<<grid, 256, 0, st>>>(jobs);
-  FG_LAUNCH_TRY();
-  return FG_OK;
+  if (dtype == FG_F32) return launch_early(k_stage<float>, grid, 256, st, jobs);
+  if (dtype == FG_BF16) return launch_early(k_stage<__nv_bfloat16>, grid, 256, st, jobs);
+  return launch_early(k_stage<__half>, grid, 256, st, jobs);
 }
 
 Operand resolve_operand(int dtype, const Mat &m, int64_t rows, int64_t k, StageJobs *jobs,
