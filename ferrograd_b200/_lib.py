@@ -73,6 +73,7 @@ class LinearGradArgsC(ctypes.Structure):
                 ("pre", ctypes.c_void_p), ("ld_pre", ctypes.c_int64),
                 ("act", ctypes.c_int32), ("reserved", ctypes.c_int32), ("drop", DropoutC),
                 ("dx", ctypes.c_void_p), ("ld_dx", ctypes.c_int64),
+                ("dx_residual", ctypes.c_void_p), ("ld_dx_residual", ctypes.c_int64),
                 ("dw", ctypes.c_void_p), ("ld_dw", ctypes.c_int64),
                 ("db", ctypes.c_void_p),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]

@@ -660,6 +660,10 @@ static int check_grad(const fg_linear_grad_args *g, DropParams *drop) {
             !overlap(o.p, o.rows, o.cols, o.ld, g->act ? g->pre : nullptr, g->M, g->N, g->ld_pre,
                      1, es),
         "%s: %s overlaps an operand", who, o.name);
+    const bool same = i == 0 && g->dx_residual == g->dx && g->ld_dx_residual == g->ld_dx;
+    FG_REQUIRE(same || !overlap(o.p, o.rows, o.cols, o.ld, g->dx ? g->dx_residual : nullptr, g->M,
+                                g->K, g->ld_dx_residual, 1, es),
+               "%s: %s overlaps dx_residual (only dx may, and only be all of it)", who, o.name);
     for (int j = i + 1; j < 3; j++)
       FG_REQUIRE(!overlap(o.p, o.rows, o.cols, o.ld, outs[j].p, outs[j].rows, outs[j].cols,
                           outs[j].ld, 1, es),
@@ -680,7 +684,14 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
   if (rc) return rc;
   const int es = elem_size(g->dtype);
   if (g->M == 0 || g->N == 0) {  // sums over nothing
-    if ((rc = zero_rows(g->dx, g->ld_dx, g->M, g->K, es, st))) return rc;
+    if (g->dx_residual && g->dx && g->M > 0 && g->K > 0) {
+      if (g->dx_residual != g->dx)
+        FG_CUDA_TRY(cudaMemcpy2DAsync(g->dx, g->ld_dx * es, g->dx_residual,
+                                      g->ld_dx_residual * es, (size_t)g->K * es, g->M,
+                                      cudaMemcpyDeviceToDevice, st));
+    } else if ((rc = zero_rows(g->dx, g->ld_dx, g->M, g->K, es, st))) {
+      return rc;
+    }
     if ((rc = zero_rows(g->dw, g->ld_dw, g->N, g->K, es, st))) return rc;
     return zero_rows(g->db, g->N, 1, g->N, es, st);
   }
@@ -708,12 +719,15 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
   if (p.dx) {  // dx[m, k] = sum_n dz(m, n) w(n, k)
     e.out = g->dx;
     e.ldo = g->ld_dx;
+    e.residual = g->dx_residual;
+    e.ldr = g->ld_dx_residual;
     e.M = g->M;
     e.N = g->K;
-    e.vec = rows16(e.out, e.ldo, es);
+    e.vec = rows16(e.out, e.ldo, es) && rows16(e.residual, e.ldr, es);
     if ((rc = run_tensor_product(g->dtype, p.z_dx, p.w, g->N, e, st))) return rc;
   }
   if (p.dw) {  // dw[n, k] = sum_m dz(m, n) x(m, k)
+    e.residual = nullptr;
     e.out = g->dw;
     e.ldo = g->ld_dw;
     e.M = g->N;

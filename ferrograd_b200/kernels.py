@@ -246,11 +246,13 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
 def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
                 pre: Optional[torch.Tensor] = None, act: str = "none",
                 drop: Optional[Dropout] = None, need_dx: bool = True, need_dw: bool = True,
-                need_db: bool = True, stream: Optional[int] = None):
+                need_db: bool = True, dx_residual: Optional[torch.Tensor] = None,
+                stream: Optional[int] = None):
     """``(dx, dw, db)`` of ``linear(x, w, bias, act=act, drop=drop)`` for the
     gradient ``dy`` of its output; ``pre`` is what ``save_pre`` returned (not
     needed for ``act="none"``).  Gradients that are not wanted are ``None``.
-    The residual's gradient is ``dy`` itself.  With 16-bit types the gradient
+    The residual's gradient is ``dy`` itself; ``dx_residual`` [M, K] is added to
+    ``dx`` in the product's epilogue.  With 16-bit types the gradient
     at the pre-activations is rounded to that type before the two products."""
     code = _layer_dtype(x)
     if x.dim() != 2 or w.dim() != 2:
@@ -273,6 +275,11 @@ def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
     if need_dx:
         dx = x.new_empty(M, K)
         a.dx, a.ld_dx = dx.data_ptr(), K
+        if dx_residual is not None:
+            _layer_check("dx_residual", dx_residual, x, (M, K), True)
+            a.dx_residual, a.ld_dx_residual = dx_residual.data_ptr(), _ld(dx_residual)
+    elif dx_residual is not None:
+        raise ValueError("dx_residual without dx")
     if need_dw:
         dw = x.new_empty(N, K)
         a.dw, a.ld_dw = dw.data_ptr(), K

@@ -258,8 +258,10 @@ int fg_linear(const fg_linear_args *args, void *stream);
 
 /* Gradients of a linear layer whose forward call was (x, w, act, drop) and
  * saved pre, for the gradient dy of its output (the residual's gradient is dy
- * itself): dz = dropout(dy) act'(pre); dx = dz w [M, K]; dw = dz^T x [N, K];
- * db = column sums of dz [N].  dx, dw and db may each be NULL (not wanted).
+ * itself): dz = dropout(dy) act'(pre); dx = dx_residual + dz w [M, K]; dw =
+ * dz^T x [N, K]; db = column sums of dz [N].  dx, dw and db may each be NULL
+ * (not wanted); dx_residual [M, K] may be NULL, or dx itself (same pointer and
+ * pitch): where x also went round the layer, the gradient that came that way.
  * For the 16-bit types dz is rounded to that type before the two products; db is summed from the unrounded dz.  Sums
  * run in a fixed order: the same inputs give the same bits. */
 typedef struct fg_linear_grad_args {
@@ -276,6 +278,8 @@ typedef struct fg_linear_grad_args {
   fg_dropout_spec drop;
   void *dx;
   int64_t ld_dx;
+  const void *dx_residual;
+  int64_t ld_dx_residual;
   void *dw;
   int64_t ld_dw;
   void *db;

@@ -196,6 +196,27 @@ def test_linear_grad_of_what_is_wanted(need):
     grad_case("bf16", 70, 40, 24, "silu", (0.2, 1, 9), 2, need=need)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(3, 40, 24), (200, 136, 264), (130, 77, 51), (6, 0, 9)])
+def test_gradient_that_went_round(dtype, m, n, k):
+    """dx_residual is added before dx is rounded."""
+    rng = np.random.default_rng(m)
+    dt = TYPES[dtype]
+    x, w, dy = randn(rng, m, k, dt), randn(rng, n, k, dt, 0.2), randn(rng, m, n, dt)
+    r = layouts(randn(rng, m, k, dt), "pitched", rng)
+    got = kernels.linear_grad(dy, x, w, dx_residual=r)
+    product = f64(dy) @ f64(w)
+    ref = f64(r) + product
+    tol = (n + 16) * STEP * (np.abs(f64(dy)) @ np.abs(f64(w))) + 2 * STEP * np.abs(f64(r))
+    check(got[0], ref, tol + ROUND[dtype] * np.abs(ref) + TINY[dtype], "dx")
+    plain = kernels.linear_grad(dy, x, w)
+    assert torch.equal(got[1], plain[1]) and torch.equal(got[2], plain[2])
+    with pytest.raises(ValueError):
+        kernels.linear_grad(dy, x, w, need_dx=False, dx_residual=r)
+    with pytest.raises(ValueError):
+        kernels.linear_grad(dy, x, w, dx_residual=r[:, 1:])
+
+
 def test_broadcast_gradient():
     """The gradient of a sum arrives as one value expanded (strides 0)."""
     rng = np.random.default_rng(0)
