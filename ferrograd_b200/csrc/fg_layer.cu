@@ -203,8 +203,7 @@ static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaSt
 // ---------------------------------------------------------------------------
 // dz = D(dy) * act'(pre), and the column sums of dz over this block's rows
 // (f32, one row of `part` a block; k_bias_grad adds them up in order).
-// A block takes 256 columns and `rows` rows: 32 lanes x 8 columns, 8 warps
-// over the rows.  dz may be null (only the sums are wanted).
+// dz may be null (only the sums are wanted).
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void store_dz(void *dz, int64_t at, int64_t, const float (&v)[8]) {
@@ -220,15 +219,19 @@ __device__ __forceinline__ void store_dz<float>(void *dz, int64_t at, int64_t pl
 #pragma unroll
   for (int k = 0; k < 3; k++) store8(static_cast<__nv_bfloat16 *>(dz) + k * plane + at, p[k]);
 }
-template <typename T>
+// TX: groups of eight columns across a block, 32 or 4 (small matrices); 256 /
+// TX rows down it.  Where one block has all rows of its columns it writes db
+// itself.
+template <typename T, int TX>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
     k_layer_dz(const T *__restrict__ dy, int64_t yr, int64_t yc, const T *__restrict__ pre,
                int64_t ldp, int act, const DropParams drop, void *__restrict__ dz, int64_t ldz,
-               float *__restrict__ part, int M, int N, int rows, int vec) {
-  __shared__ float red[8][256];
+               float *__restrict__ part, T *__restrict__ db, int M, int N, int rows, int vec) {
+  constexpr int TY = 256 / TX;
+  __shared__ float red[TY][TX * 8];
   constexpr int U = 2;  // rows in flight, and as many again asked for
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = blockIdx.x * 256 + lane * 8;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+  const int col = blockIdx.x * (TX * 8) + tx * 8;
   const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
   float sum[8] = {};
   grid_wait();
@@ -246,28 +249,28 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
     auto ask = [&](int r, Raw8<T>(&a)[U], Raw8<T>(&b)[U]) {
 #pragma unroll
       for (int u = 0; u < U; u++)
-        if (r + 8 * u < r1) {
-          a[u].load(dy + (r + 8 * u) * yr + col);
-          if (act != FG_ACT_NONE) b[u].load(pre + (r + 8 * u) * ldp + col);
+        if (r + TY * u < r1) {
+          a[u].load(dy + (r + TY * u) * yr + col);
+          if (act != FG_ACT_NONE) b[u].load(pre + (r + TY * u) * ldp + col);
         }
     };
-    ask(r0 + warp, y, p);
-    for (int r = r0 + warp; r < r1; r += 8 * U) {
-      ask(r + 8 * U, yn, pn);
+    ask(r0 + ty, y, p);
+    for (int r = r0 + ty; r < r1; r += TY * U) {
+      ask(r + TY * U, yn, pn);
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        if (r + 8 * u < r1) {
+        if (r + TY * u < r1) {
           float v[8], z[8];
           y[u].get(v);
           p[u].get(z);
-          one(r + 8 * u, v, z);
+          one(r + TY * u, v, z);
         }
         y[u] = yn[u];
         p[u] = pn[u];
       }
     }
   } else if (col < N) {
-    for (int r = r0 + warp; r < r1; r += 8) {
+    for (int r = r0 + ty; r < r1; r += TY) {
       float v[8], z[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -277,16 +280,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
       one(r, v, z);
     }
   }
-  if (!part) return;
 #pragma unroll
-  for (int i = 0; i < 8; i++) red[warp][lane * 8 + i] = sum[i];
+  for (int i = 0; i < 8; i++) red[ty][tx * 8 + i] = sum[i];
   __syncthreads();
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c < N) {
+  const int c = blockIdx.x * (TX * 8) + threadIdx.x;
+  if (db && threadIdx.x < TX * 8 && c < N) {
     float s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; w++) s += red[w][threadIdx.x];
-    part[(size_t)blockIdx.y * N + c] = s;
+#pragma unroll 8
+    for (int w = 0; w < TY; w++) s += red[w][threadIdx.x];
+    if (gridDim.y == 1)
+      db[c] = from_f32<T>(s);
+    else
+      part[(size_t)blockIdx.y * N + c] = s;
   }
 }
 
@@ -546,21 +551,35 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
   return run_tensor_product(g->dtype, p.x, p.w, g->K, e, st);
 }
 
-// Rows of a block of k_layer_dz: enough blocks for several waves, at most 128
-// partial sums a column, at least 64 rows.
-static int dz_rows(int M, int N) {
-  const int64_t strips = (N + 255LL) / 256;
-  int64_t chunks = strips >= 4096 ? 1 : 4096 / strips;
+// How k_layer_dz is cut: blocks of 256 columns for large arrays (16384 x 16384
+// bf16: 391 us), of 32 columns x 64 rows for small ones; rows a
+// block such that there are several waves of blocks but at most 128 partial sums
+// a column, and one block for all rows where eight passes do (then it writes db
+// itself and a launch is saved).
+struct DzShape {
+  int vec, tx, rows, chunks;
+};
+static DzShape dz_shape(const fg_linear_grad_args *g) {
+  DzShape d{};
+  const int es = elem_size(g->dtype);
+  d.vec = g->dy_col == 1 && rows16(g->dy, g->dy_row, es) &&
+          (g->act == FG_ACT_NONE || rows16(g->pre, g->ld_pre, es));
+  d.tx = (int64_t)g->M * g->N >= (4 << 20) ? 32 : 4;
+  const int64_t strips = (g->N + 8LL * d.tx - 1) / (8 * d.tx), down = 256 / d.tx;
+  const int64_t blocks = d.tx == 32 ? 4096 : 592;
+  int64_t chunks = g->M <= 8 * down ? 1 : strips >= blocks ? 1 : blocks / strips;
   if (chunks > 128) chunks = 128;
-  int64_t rows = ((M + chunks - 1) / chunks + 7) / 8 * 8;
-  return (int)(rows < 64 ? 64 : rows);
+  const int64_t rows = ((g->M + chunks - 1) / chunks + down - 1) / down * down;
+  d.rows = (int)(rows < 0x7fffff00 ? rows : 0x7fffff00);
+  d.chunks = (int)((g->M + (int64_t)d.rows - 1) / d.rows);
+  return d;
 }
 
 // dz is written (in a 16-bit type, or as the three planes of f32) where a
 // product reads it and it differs from dy; x and w are read in place or staged.
 struct GradPlan {
   bool dx, dw, make_dz;
-  int rows, chunks;   // of k_layer_dz
+  DzShape shape;
   int64_t ldz;
   size_t dz_off, part_off, bytes;
   Operand z_dx, z_dw, w, x;
@@ -571,8 +590,7 @@ static GradPlan plan_grad(const fg_linear_grad_args *g) {
   p.dx = g->dx && g->K > 0;
   p.dw = g->dw && g->K > 0;
   p.make_dz = (p.dx || p.dw) && (g->dtype == FG_F32 || g->act != FG_ACT_NONE || g->drop.p > 0.0);
-  p.rows = dz_rows(g->M, g->N);
-  p.chunks = (int)((g->M + (int64_t)p.rows - 1) / p.rows);
+  p.shape = dz_shape(g);
   p.ldz = (g->N + 7LL) / 8 * 8;
   auto take = [&](size_t n) {
     const size_t o = (p.bytes + 255) / 256 * 256;
@@ -581,7 +599,7 @@ static GradPlan plan_grad(const fg_linear_grad_args *g) {
   };
   const int planes = g->dtype == FG_F32 ? 3 : 1;
   p.dz_off = take(p.make_dz ? (size_t)planes * g->M * p.ldz * 2 : 0);
-  p.part_off = take(g->db ? (size_t)p.chunks * g->N * 4 : 0);
+  p.part_off = take(g->db && p.shape.chunks > 1 ? (size_t)p.shape.chunks * g->N * 4 : 0);
   if (p.make_dz) {
     p.z_dx.staged_at = p.dz_off;
     p.z_dx.planes = planes;
@@ -610,23 +628,18 @@ static GradPlan plan_grad(const fg_linear_grad_args *g) {
 template <typename T>
 static int run_dz(const fg_linear_grad_args *g, const GradPlan &p, const DropParams &drop,
                   cudaStream_t st) {
-  const int es = sizeof(T);
   char *ws = static_cast<char *>(g->workspace);
-  float *part = g->db ? reinterpret_cast<float *>(ws + p.part_off) : nullptr;
-  if (p.make_dz || part) {
-    const int vec = g->dy_col == 1 && rows16(g->dy, g->dy_row, es) &&
-                    (g->act == FG_ACT_NONE || rows16(g->pre, g->ld_pre, es));
-    int rc = launch_early(k_layer_dz<T>, dim3((unsigned)((g->N + 255LL) / 256), p.chunks), 256, st,
-                          static_cast<const T *>(g->dy), g->dy_row, g->dy_col,
-                          static_cast<const T *>(g->pre), g->ld_pre, g->act, drop,
-                          p.make_dz ? ws + p.dz_off : nullptr, p.ldz, part, g->M, g->N, p.rows,
-                          vec);
-    if (rc) return rc;
-  }
-  if (g->db)
-    return launch_early(k_bias_grad<T>, dim3((unsigned)((g->N + 255LL) / 256)), 256, st, part,
-                        p.chunks, g->N, static_cast<T *>(g->db));
-  return FG_OK;
+  const DzShape &d = p.shape;
+  float *part = g->db && d.chunks > 1 ? reinterpret_cast<float *>(ws + p.part_off) : nullptr;
+  const dim3 grid((unsigned)((g->N + 8LL * d.tx - 1) / (8 * d.tx)), d.chunks);
+  int rc = launch_early(d.tx == 32 ? k_layer_dz<T, 32> : k_layer_dz<T, 4>, grid, 256, st,
+                        static_cast<const T *>(g->dy), g->dy_row, g->dy_col,
+                        static_cast<const T *>(g->pre), g->ld_pre, g->act, drop,
+                        p.make_dz ? ws + p.dz_off : nullptr, p.ldz, part, static_cast<T *>(g->db),
+                        g->M, g->N, d.rows, d.vec);
+  if (rc || !part) return rc;
+  return launch_early(k_bias_grad<T>, dim3((unsigned)((g->N + 255LL) / 256)), 256, st, part,
+                      d.chunks, g->N, static_cast<T *>(g->db));
 }
 
 static int check_grad(const fg_linear_grad_args *g, DropParams *drop) {
@@ -704,17 +717,20 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
   place_operand(&p.w, g->workspace);
   place_operand(&p.x, g->workspace);
   place_jobs(&p.jobs, g->workspace);
-  switch (g->dtype) {
-    case FG_F32:
-      rc = run_dz<float>(g, p, drop, st);
-      break;
-    case FG_BF16:
-      rc = run_dz<__nv_bfloat16>(g, p, drop, st);
-      break;
-    default:
-      rc = run_dz<__half>(g, p, drop, st);
+  if ((rc = run_stage(g->dtype, p.jobs, st))) return rc;
+  if (p.make_dz || g->db) {
+    switch (g->dtype) {
+      case FG_F32:
+        rc = run_dz<float>(g, p, drop, st);
+        break;
+      case FG_BF16:
+        rc = run_dz<__nv_bfloat16>(g, p, drop, st);
+        break;
+      default:
+        rc = run_dz<__half>(g, p, drop, st);
+    }
+    if (rc) return rc;
   }
-  if (rc || (rc = run_stage(g->dtype, p.jobs, st))) return rc;
   Epilogue e{};
   if (p.dx) {  // dx[m, k] = sum_n dz(m, n) w(n, k)
     e.out = g->dx;

@@ -225,27 +225,33 @@ __device__ __forceinline__ void act8(float (&v)[8], int act) {
   switch (act) {
     case FG_ACT_RELU:
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = 0.0f < v[i] ? v[i] : 0.0f;
+      for (int i = 0; i < 8; i++) {
+        float &x = v[i];
+        x = 0.0f < x ? x : 0.0f;
+      }
       break;
     case FG_ACT_GELU:
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const float b = bound_below(v[i], -32.0f);
-        v[i] = b * F::phi(b);
+        float &x = v[i];
+        x = bound_below(x, -32.0f);
+        x *= F::phi(x);
       }
       break;
     case FG_ACT_GELU_TANH:  // (1 + tanh u) / 2 = logistic(2u)
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const float b = bound_below(v[i], -32.0f);
-        v[i] = b * F::logistic(b * fmaf(2.0f * kGeluC * kGeluB, b * b, 2.0f * kGeluC));
+        float &x = v[i];
+        x = bound_below(x, -32.0f);
+        x *= F::logistic(x * fmaf(2.0f * kGeluC * kGeluB, x * x, 2.0f * kGeluC));
       }
       break;
     case FG_ACT_SILU:
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const float b = bound_below(v[i], -128.0f);
-        v[i] = b * F::logistic(b);
+        float &x = v[i];
+        x = bound_below(x, -128.0f);
+        x *= F::logistic(x);
       }
       break;
     default:
@@ -392,25 +398,25 @@ __device__ __forceinline__ void load8_smem(Chunk chunk, int c, float (&v)[8]) {
   }
 }
 
-// z (f32 sums, without the bias) for the columns col .. col+7 of a row ->
-// out (and pre).  Everything is f32 until the one rounding of each store; the
+// z (f32 sums, without the bias) for the columns col .. col+7 of a row -> out
+// (and pre).  Everything is f32 until the one rounding of each store; the
 // activation sees the unrounded z.
 template <typename T>
 __device__ __forceinline__ void epilogue8(const Epilogue &e, int row, int col, float (&v)[8]) {
-  const bool whole = col + 8 <= e.N;
-  const int n = whole ? 8 : e.N - col;
-  const bool vec = e.vec && whole;
-  bias8<T>(e, col, v);
-  if (e.pre) {
-    T *p = static_cast<T *>(e.pre) + (int64_t)row * e.ldp + col;
+  const int n = min(8, e.N - col);
+  const bool vec = e.vec && n == 8;
+  auto put = [&](void *base, int64_t ld) {
+    T *t = static_cast<T *>(base) + (int64_t)row * ld + col;
     if (vec) {
-      store8<T>(p, v);
+      store8<T>(t, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        if (i < n) p[i] = from_f32<T>(v[i]);
+        if (i < n) t[i] = from_f32<T>(v[i]);
     }
-  }
+  };
+  bias8<T>(e, col, v);
+  if (e.pre) put(e.pre, e.ldp);
   act8<sizeof(T) == 2>(v, e.act);
   if (e.drop.on) drop8(e.drop, row, col, v);
   if (e.residual) {
@@ -426,17 +432,75 @@ __device__ __forceinline__ void epilogue8(const Epilogue &e, int row, int col, f
         if (i < n) v[i] += to_f32<T>(r[i]);
     }
   }
-  T *o = static_cast<T *>(e.out) + (int64_t)row * e.ldo + col;
-  if (vec) {
-    store8<T>(o, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (i < n) o[i] = from_f32<T>(v[i]);
-  }
+  put(e.out, e.ldo);
 }
 
-// The same for one element.
+// A warp's R x C elements (R * C = 256, C = 2^lc) between global memory, neighbouring
+// lanes on neighbouring columns, and a slab of R rows of C + 4 floats in shared
+// memory, from which a lane takes eight columns of a row: for rows off 16-byte
+// boundaries, whose eight columns a lane would otherwise touch one by one, 32
+// sectors a time.  All lanes take part.
+template <typename T>
+__device__ __forceinline__ void slab_fetch(float *slab, int lc, const T *g, int64_t rs, int64_t cs,
+                                           int row0, int col0, int M, int N) {
+  const int lane = threadIdx.x & 31;
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int x = i * 32 + lane, r = x >> lc, c = x & ((1 << lc) - 1);
+    t[i] = row0 + r < M && col0 + c < N ? to_f32<T>(g[(row0 + r) * rs + (col0 + c) * cs]) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int x = i * 32 + lane;
+    slab[(x >> lc) * ((1 << lc) + 4) + (x & ((1 << lc) - 1))] = t[i];
+  }
+  __syncwarp();
+}
+template <typename T>
+__device__ __forceinline__ void slab_flush(const float *slab, int lc, T *g, int64_t ld, int row0,
+                                           int col0, int M, int N) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int x = i * 32 + lane, r = x >> lc, c = x & ((1 << lc) - 1);
+    if (row0 + r < M && col0 + c < N)
+      g[(int64_t)(row0 + r) * ld + col0 + c] = from_f32<T>(slab[r * ((1 << lc) + 4) + c]);
+  }
+  __syncwarp();
+}
+
+// epilogue8 for such rows: lane (r, c) of the R x C elements at (row0, col0).
+template <typename T>
+__device__ __forceinline__ void epilogue_slab(const Epilogue &e, float *slab, int lc, int row0,
+                                              int col0, int r, int c, float (&v)[8]) {
+  float *mine = slab + r * ((1 << lc) + 4) + c;
+  auto put = [&] {
+    __syncwarp();
+    reinterpret_cast<float4 *>(mine)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(mine)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  };
+  bias8<T>(e, col0 + c, v);
+  if (e.pre) {
+    put();
+    slab_flush<T>(slab, lc, static_cast<T *>(e.pre), e.ldp, row0, col0, e.M, e.N);
+  }
+  act8<sizeof(T) == 2>(v, e.act);
+  if (e.drop.on) drop8(e.drop, row0 + r, col0 + c, v);
+  if (e.residual) {
+    __syncwarp();
+    slab_fetch<T>(slab, lc, static_cast<const T *>(e.residual), e.ldr, 1, row0, col0, e.M, e.N);
+    float t[8];
+    load8<float>(mine, t);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] += t[i];
+  }
+  put();
+  slab_flush<T>(slab, lc, static_cast<T *>(e.out), e.ldo, row0, col0, e.M, e.N);
+}
+
+// epilogue8 for one element.
 template <typename T>
 __device__ __forceinline__ void epilogue1(const Epilogue &e, int row, int col, float z) {
   if (e.bias) z += to_f32<T>(static_cast<const T *>(e.bias)[col]);

@@ -63,7 +63,8 @@ struct ProductArgs {
   int M, N, nk;      // nk: k-blocks
   int chain;         // k-blocks of one accumulation chain
   int stages, split, group;
-  int join_at;       // split: offset from the ring of the joined sums
+  int join_at;       // split: offsets from the ring of the joined sums
+  int slab_at;       // and of the warps' slabs
   int bf16;
   OperandLayout a, b;
   unsigned int *err;
@@ -95,7 +96,8 @@ __device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int grou
 }
 
 constexpr int kBlockCols = 32;                 // IO: a warp's block
-constexpr int kSlabCols = 16, kSlabPitch = 20;  // floats; a warp's 32 x 16 transpose slab
+constexpr int kSlabCols = 16, kSlabPitch = 20;  // floats; a warp's 32 x 16 slab (pair)
+constexpr int kSplitSlab = 384;                 // floats; 8 x 36, 16 x 20 or 32 x 12 (split)
 
 // The block of each form.  RUN: the epilogue warps keep the running sums of the
 // chains in registers; without it a product is one chain and they read the
@@ -354,19 +356,17 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       return !dead;
     };
     // 16 columns of a pair's tile through the warp's slab, so that lanes hold
-    // eight neighbouring columns and two lanes a row's 16: 32-byte sectors
+    // eight neighbouring columns (rows off 16-byte boundaries)
     float *slab = reinterpret_cast<float *>(ring + S * stage_bytes) +
                   (warp - kFirstEpi) * (32 * kSlabPitch);
     auto finish16 = [&](int row0, int col0) {
       __syncwarp();
-#pragma unroll
+#pragma unroll 1
       for (int p = 0; p < 2; p++) {
-        const int r = p * 16 + lane / 2, cg = (lane & 1) * 8;
-        if (row0 + r < g.M && col0 + cg < g.N) {
-          float v[8];
-          load8<float>(slab + r * kSlabPitch + cg, v);
-          epilogue8<T>(e, row0 + r, col0 + cg, v);
-        }
+        float v[8];
+        load8<float>(slab + (p * 16 + lane / 2) * kSlabPitch + (lane & 1) * 8, v);
+        epilogue_slab<T>(e, slab + p * 16 * kSlabPitch, 4, row0 + 16 * p, col0, lane / 2,
+                         (lane & 1) * 8, v);
       }
     };
     // IO: this warp's block of 32 rows x 32 columns in shared memory (swizzled
@@ -600,12 +600,12 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
     // a warp takes gw groups of eight columns of 32 / gw rows at a time: eight
     // lanes read 128 neighbouring bytes, gw lanes write a row's
     const int gw = groups < 4 ? groups : 4, rw = 32 / gw, across = groups / gw;
-    for (int t = warp; t < (rows + rw - 1) / rw * across; t += Block<CG, RUN>::threads / 32) {
-      const int r = t / across * rw + lane % rw;
-      const int cg = (t % across * gw + lane / rw) * 8;
-      const int col = nb * BN + (int)rank * own + cg;
-      if (r >= rows || col >= g.N) continue;
-      float v[8] = {};
+    const int r_in = lane % rw, c_in = lane / rw * 8;
+    const int pieces = (rows + rw - 1) / rw * across;
+    constexpr int kWarps = Block<CG, RUN>::threads / 32;
+    auto gather = [&](int r, int cg, float(&v)[8]) {  // the ranks' sums, in order
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = 0.0f;
 #pragma unroll 4
       for (int k = 0; k < g.split; k++) {
         const float4 *x = joined + (k * (own / 4) + cg / 4) * pitch + r;
@@ -613,7 +613,18 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
         v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
         v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
       }
-      epilogue8<T>(e, mb * BM + r, col, v);
+    };
+    const int col0 = nb * BN + (int)rank * own;
+    float *slab = reinterpret_cast<float *>(ring + g.slab_at) + warp * kSplitSlab;
+    for (int t = warp; t < pieces; t += kWarps) {
+      const int r0 = t / across * rw, c0 = t % across * (gw * 8);
+      const int r = r0 + r_in, col = col0 + c0 + c_in;
+      float v[8];
+      gather(r < rows ? r : 0, c0 + c_in, v);
+      if (!e.vec)
+        epilogue_slab<T>(e, slab, 31 - __clz(gw * 8), mb * BM + r0, col0 + c0, r_in, c_in, v);
+      else if (r < rows && col < g.N)
+        epilogue8<T>(e, mb * BM + r, col, v);
     }
   }
   if (IO && warp >= kFirstEpi && lane == 0) bulk_wait_read();
@@ -633,19 +644,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
 // the contiguous direction innermost; f32 as three bf16 planes.
 // ---------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void stage8(const T *src, int64_t so, int64_t si, int64_t o, int64_t i,
-                                       int64_t inner, bool vec, uint4 *dst, int64_t plane16) {
-  float v[8];
-  if (vec && i + 8 <= inner) {
-    if (sizeof(T) == 2) {
-      dst[0] = *reinterpret_cast<const uint4 *>(src + o * so + i);
-      return;
-    }
-    load8<T>(src + o * so + i, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = i + j < inner ? to_f32<T>(src[o * so + (i + j) * si]) : 0.0f;
-  }
+__device__ __forceinline__ void stage_store(uint4 *dst, int64_t plane16, const float (&v)[8]) {
   if (sizeof(T) == 2) {
     store8<T>(reinterpret_cast<T *>(dst), v);
   } else {
@@ -665,12 +664,21 @@ __global__ void __launch_bounds__(256) k_stage(const StageJobs jobs) {
   const int64_t plane = groups * j.outer;
   const T *src = static_cast<const T *>(j.src);
   uint4 *dst = static_cast<uint4 *>(j.dst);
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
   grid_wait();
   grid_launch_next();
-  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
-  for (Walk at(j.outer, groups, first, step); at.inside(); at.next())
-    stage8<T>(src, j.so, j.si, at.row, (int64_t)at.group * 8, j.inner, j.vec,
-              dst + at.row * groups + at.group, plane);
+  for (Walk at(j.outer, groups, first, step); at.inside(); at.next()) {
+    const int64_t x = (int64_t)at.group * 8;
+    float v[8];
+    if (j.vec && x + 8 <= j.inner) {
+      load8<T>(src + at.row * j.so + x, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        v[k] = x + k < j.inner ? to_f32<T>(src[at.row * j.so + (x + k) * j.si]) : 0.0f;
+    }
+    stage_store<T>(dst + at.row * groups + at.group, plane, v);
+  }
 }
 
 int run_stage(int dtype, const StageJobs &jobs, cudaStream_t st) {
@@ -823,6 +831,8 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
     if (bytes < sums) bytes = sums;
     g.join_at = (int)((bytes + 127) & ~(size_t)127);
     if (g.split > 1) bytes = g.join_at + sums;
+    g.slab_at = (int)((bytes + 127) & ~(size_t)127);
+    if (!e.vec) bytes = g.slab_at + Block<CG, RUN>::threads / 32 * kSplitSlab * 4;
   }
   bytes += 2048;  // barriers, alignment
   if (bytes < tmem_share(2 * BN)) bytes = tmem_share(2 * BN);
