@@ -200,11 +200,10 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   // 256 x 216 and the others keep 128 x 64.
   if (warp < kFirstEpi) {
     if (CG == 2 && RUN) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    // Both loops below run in whole warps with one lane's instructions switched
-    // on, and are instantiated for each pair of layouts.  After a wait that
-    // gave up they run on with everything switched off, so that no branch of
-    // theirs hangs on a barrier's answer.
-    const uint32_t on = lane == 0;
+    // Both loops below run in whole warps and are instantiated for each pair of
+    // layouts.  After a wait that gave up they run on with everything switched
+    // off, so that no branch of theirs hangs on a barrier's answer.
+    const uint32_t on = 1;
     bool alive = true;
     const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), ring0 = smem_u32(ring);
     auto produce = [&](auto a_layout, auto b_layout) {
@@ -263,7 +262,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       const uint64_t db0 =
           desc_base<PLANES>(b_mn) + (((ring0 & 0x3ffffu) + PLANES * a_bytes) >> 4);
       // 16 elements further in k: 32 bytes inside a swizzled row, or 16 k-rows
-      constexpr uint32_t a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
+      constexpr int a_step = (a_mn ? 2048 : 32) >> 4, b_step = (b_mn ? 2048 : 32) >> 4;
       const uint32_t tmem_full0 = smem_u32(tmem_full), tmem_empty0 = smem_u32(tmem_empty);
       int s = 0, local = 0;
       uint32_t phase = 0, go = on;
@@ -282,11 +281,8 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
           auto products = [&](int st, int pa, int pb) {
             const uint64_t da = da0 + ((st * stage_bytes + pa * a_bytes) >> 4);
             const uint64_t db = db0 + ((st * stage_bytes + pb * b_bytes) >> 4);
-#pragma unroll
-            for (int k = 0; k < BK / 16; k++) {
-              mma_f16<CG>(go, d, da + k * a_step, db + k * b_step, idesc, acc);
-              acc = 1;
-            }
+            mma_f16_steps<CG, BK / 16, a_step, b_step>(go, d, da, db, idesc, acc);
+            acc = 1;
           };
           for (int kb = c0; kb < c1; kb++) {
             if (alive && !mbar_wait_suspended(full0 + 8 * s, phase, g.err, kErrLayer | 3))

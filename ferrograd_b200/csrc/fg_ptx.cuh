@@ -256,27 +256,42 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool a
          ((uint32_t)(M >> 4) << 24);
 }
 
-// The instructions below run in the lanes whose `on` is not 0 (one lane of a
-// warp that passes through them whole): predicated, not branched around, so
-// that the compiler keeps their operands in the warp's uniform registers.  A
-// loop in a branch of one lane took 600 cycles a step, mostly to move them.
+// The instructions below are for a warp that passes through them whole: one
+// elected lane (the same each time) runs them if `on`, the same in all lanes,
+// is not 0.  Elected and predicated in one piece, not branched around by the
+// caller, so that their operands stay in the warp's uniform registers: a loop
+// in a branch of one lane took 600 cycles a step, mostly to move them.
 
-// D[tmem] (+)= A * B, kind::f16, one CTA or a CTA pair (issued by its leader).
-template <int CG>
-__device__ __forceinline__ void mma_f16(uint32_t on, uint32_t d_tmem, uint64_t adesc,
-                                        uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  if (CG == 1)
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
-        : "memory");
+// D[tmem] (+)= A * B, kind::f16, one CTA or a CTA pair (issued by its leader):
+// STEPS k-steps of 16, the descriptors A_STEP and B_STEP apart; the first adds
+// to D if accumulate.
+template <int CG, int STEPS, int A_STEP, int B_STEP>
+__device__ __forceinline__ void mma_f16_steps(uint32_t on, uint32_t d_tmem, uint64_t adesc,
+                                              uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  static_assert(STEPS == 2 || STEPS == 4, "two or four steps");
+#define FG_MMA(cg, a, b, p) "@q tcgen05.mma.cta_group::" cg ".kind::f16 [%0], " a ", " b ", %3, " p ";\n\t"
+#define FG_MMA_STEPS(cg)                                                                          \
+  asm volatile(                                                                                   \
+      "{\n\t.reg .pred p, q, e, t;\n\t.reg .b64 a, b;\n\t"                                        \
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"              \
+      "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t" FG_MMA(cg, "%1", "%2", "p")         \
+      "add.s64 a, %1, %6;\n\tadd.s64 b, %2, %7;\n\t" FG_MMA(cg, "a", "b", "t")                    \
+      "}" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on),            \
+      "n"(A_STEP), "n"(B_STEP)                                                                    \
+      : "memory")
+#pragma unroll
+  for (int k = 0; k < STEPS; k += 2) {
+    if (CG == 1)
+      FG_MMA_STEPS("1");
+    else
+      FG_MMA_STEPS("2");
+    adesc += 2 * A_STEP;
+    bdesc += 2 * B_STEP;
+    accumulate = 1;
+  }
+#undef FG_MMA_STEPS
+#undef FG_MMA
 }
 
 // Arrive, once every tcgen05 op this thread issued so far completes, on the
@@ -285,14 +300,16 @@ template <int CG>
 __device__ __forceinline__ void mma_commit_cg(uint32_t on, uint32_t bar) {
   if (CG == 1)
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "{\n\t.reg .pred q, e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t"
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
             bar),
         "r"(on)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "{\n\t.reg .pred q, e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t"
         "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster"
         ".b64 [%0], %1;\n\t}" ::"r"(bar),
         "h"((uint16_t)3), "r"(on)
@@ -301,7 +318,8 @@ __device__ __forceinline__ void mma_commit_cg(uint32_t on, uint32_t bar) {
 
 __device__ __forceinline__ void mbar_expect_tx(uint32_t on, uint32_t bar, uint32_t bytes) {
   asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "{\n\t.reg .pred q, e;\n\tsetp.ne.b32 e, %2, 0;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t"
       "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
       "r"(bytes), "r"(on)
       : "memory");
@@ -380,14 +398,16 @@ __device__ __forceinline__ void tma_load_2d_cg(uint32_t on, uint32_t smem_dst,
                                                const CUtensorMap *map, uint32_t bar, int x, int y) {
   if (CG == 1)
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "{\n\t.reg .pred q, e;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t"
         "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(smem_dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar), "r"(on)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "{\n\t.reg .pred q, e;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t"
         "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier"
         "::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(smem_dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar), "r"(on)
@@ -399,14 +419,16 @@ __device__ __forceinline__ void tma_load_3d_cg(uint32_t on, uint32_t smem_dst,
                                                int z) {
   if (CG == 1)
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "{\n\t.reg .pred q, e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t"
         "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(smem_dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "{\n\t.reg .pred q, e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\tand.pred q, q, e;\n\t"
         "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier"
         "::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(smem_dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(on)
