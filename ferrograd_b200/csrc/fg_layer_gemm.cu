@@ -102,11 +102,14 @@ constexpr int kSplitSlab = 384;                 // floats; 8 x 36, 16 x 20 or 32
 // The block of each form.  RUN: the epilogue warps keep the running sums of the
 // chains in registers; without it a product is one chain and they read the
 // accumulator where they need it, which leaves registers for twice the warps.
+// split: four warps drain the accumulator, and all join in the epilogue, which
+// six left waiting on its latencies (5200 cycles for a plain 128 x 64 tile).
 template <int CG, bool RUN>
 struct Block {
   static constexpr int first_epi = CG == 2 ? 4 : 2;
   static constexpr int epi_warps = CG == 1 ? 4 : RUN ? 8 : 16;
-  static constexpr int threads = 32 * (first_epi + epi_warps);
+  static constexpr int warps = CG == 1 ? 12 : first_epi + epi_warps;
+  static constexpr int threads = 32 * warps;
 };
 
 // Case `at` of a switch: v = run[at .. at + 15].  The moves' texts differ, or the
@@ -129,7 +132,7 @@ struct Maps {
 // accesses to 32 rows cost it 32 passes; a TMA block costs 8 to write and 8 to
 // read.  It needs rows on 16-byte boundaries.
 template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO>
-__global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
+__global__ void __launch_bounds__(Block<CG, RUN>::threads, CG == 1 && !RUN ? 2 : 1)
     k_layer_product(const __grid_constant__ Maps maps, const ProductArgs g, const Epilogue e) {
   const CUtensorMap &tma = maps.a, &tmb = maps.b;
   constexpr int BK = Depth<PLANES>::BK;
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       by_layout(produce);
     else if (warp == 1 && leader)
       by_layout(multiply);
-  } else {
+  } else if (warp < kFirstEpi + kEpiWarps) {
     if (CG == 2 && RUN) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- epilogue ----------------
     const int q = warp & 3;  // the TMEM lanes this warp may read
@@ -452,6 +455,20 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
       if (kTwo && e.pre) block_store(&maps.pre, block + 32 * kRow, row0, col);
       block_store(&maps.out, block, row0, col);
     };
+    // split: sends each rank its share of this CTA's sums
+    auto share = [&](int pitch) {
+      if (g.split == 1) return;
+      fence_proxy_async_smem();
+      __syncwarp();
+      cluster_wait();  // the peers have started: their barriers are set up
+      if (!named_bar_or(1, 128, dead) && warp == kFirstEpi && lane < g.split) {
+        const uint32_t bytes = BN / g.split / 4 * pitch * 16;
+        if (lane == 0) mbar_arrive_expect_tx(join_bar, g.split * bytes);
+        bulk_copy_to_cta(map_to_rank(smem_u32(joined) + rank * bytes, lane),
+                         smem_u32(sums) + lane * bytes, bytes,
+                         map_to_rank(smem_u32(join_bar), lane));
+      }
+    };
     for (int tile = first; tile < num_m * num_n; tile += step) {
       int mb, nb;
       tile_at(tile, num_m, num_n, g.group, mb, nb);
@@ -479,6 +496,26 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
               release(buf);
           }
         }
+        continue;
+      }
+      if constexpr (!RUN && CG == 1) {
+        const int pitch = (min(128, g.M - mb * BM) + 7) & ~7, row = 32 * q + lane;
+        if (arrived(local++)) {
+#pragma unroll 1
+          for (int c = 0; c < COLS; c += 16) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(t_addr + c, r);
+            tmem_ld_wait();
+            if (row < pitch) {
+#pragma unroll
+              for (int j = 0; j < 16; j += 4)
+                sums[(c + j) / 4 * pitch + row] =
+                    make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
+                                __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+            }
+          }
+        }
+        share(pitch);
         continue;
       }
       if constexpr (!RUN) {
@@ -561,18 +598,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
             for (int j = 0; j < COLS; j += 4)
               sums[j / 4 * pitch + row] = make_float4(run[j], run[j + 1], run[j + 2], run[j + 3]);
           }
-          if (g.split > 1) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            cluster_wait();  // the peers have started: their barriers are set up
-            if (!named_bar_or(1, 128, dead) && warp == kFirstEpi && lane < g.split) {
-              const uint32_t bytes = BN / g.split / 4 * pitch * 16;
-              const uint32_t bar = smem_u32(join_bar);
-              if (lane == 0) mbar_arrive_expect_tx(join_bar, g.split * bytes);
-              bulk_copy_to_cta(map_to_rank(smem_u32(joined) + rank * bytes, lane),
-                               smem_u32(sums) + lane * bytes, bytes, map_to_rank(bar, lane));
-            }
-          }
+          share(pitch);
         }
       }
     }
@@ -581,7 +607,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
   if (CG == 1) {
     __syncwarp();
     if (g.split > 1) {
-      if (warp < kFirstEpi) cluster_wait();
+      if (warp < kFirstEpi || warp >= kFirstEpi + kEpiWarps) cluster_wait();
       mbar_wait(join_bar, 0, g.err, kErrLayer | 6);
       __syncwarp();
       cluster_arrive();  // (every copy into this CTA is done; waited for at the end)
@@ -592,33 +618,29 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, 1)
     int mb, nb;
     tile_at(first, num_m, num_n, g.group, mb, nb);
     const int rows = min(128, g.M - mb * BM), pitch = (rows + 7) & ~7;
-    const int own = BN / g.split, groups = own / 8;
-    // a warp takes gw groups of eight columns of 32 / gw rows at a time: eight
-    // lanes read 128 neighbouring bytes, gw lanes write a row's
-    const int gw = groups < 4 ? groups : 4, rw = 32 / gw, across = groups / gw;
-    const int r_in = lane % rw, c_in = lane / rw * 8;
-    const int pieces = (rows + rw - 1) / rw * across;
-    constexpr int kWarps = Block<CG, RUN>::threads / 32;
-    auto gather = [&](int r, int cg, float(&v)[8]) {  // the ranks' sums, in order
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = 0.0f;
+    // a warp takes a power of two, gw <= 4, groups of eight columns of 32 / gw
+    // rows at a time: eight lanes read 128 neighbouring bytes, gw lanes write a
+    // row's
+    const int own = BN / g.split, lgroups = 31 - __clz(own / 8);
+    const int lgw = min(lgroups, 2), lrw = 5 - lgw, lacross = lgroups - lgw;
+    const int r_in = lane & ((1 << lrw) - 1), c_in = (lane >> lrw) * 8;
+    const int pieces = ((rows + (1 << lrw) - 1) >> lrw) << lacross;
+    const int col0 = nb * BN + (int)rank * own;
+    float *slab = reinterpret_cast<float *>(ring + g.slab_at) + warp * kSplitSlab;
+    for (int t = warp; t < pieces; t += Block<CG, RUN>::warps) {
+      const int r0 = (t >> lacross) << lrw;
+      const int c0 = (t & ((1 << lacross) - 1)) << (lgw + 3);
+      const int r = r0 + r_in, col = col0 + c0 + c_in;
+      const float4 *x = joined + (c0 + c_in) / 4 * pitch + (r < rows ? r : 0);
+      float v[8] = {};
 #pragma unroll 4
-      for (int k = 0; k < g.split; k++) {
-        const float4 *x = joined + (k * (own / 4) + cg / 4) * pitch + r;
+      for (int k = 0; k < g.split; k++, x += own / 4 * pitch) {  // the ranks' sums, in order
         const float4 lo = x[0], hi = x[pitch];
         v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
         v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
       }
-    };
-    const int col0 = nb * BN + (int)rank * own;
-    float *slab = reinterpret_cast<float *>(ring + g.slab_at) + warp * kSplitSlab;
-    for (int t = warp; t < pieces; t += kWarps) {
-      const int r0 = t / across * rw, c0 = t % across * (gw * 8);
-      const int r = r0 + r_in, col = col0 + c0 + c_in;
-      float v[8];
-      gather(r < rows ? r : 0, c0 + c_in, v);
       if (!e.vec)
-        epilogue_slab<T>(e, slab, 31 - __clz(gw * 8), mb * BM + r0, col0 + c0, r_in, c_in, v);
+        epilogue_slab<T>(e, slab, lgw + 3, mb * BM + r0, col0 + c0, r_in, c_in, v);
       else if (r < rows && col < g.N)
         epilogue8<T>(e, mb * BM + r, col, v);
     }
@@ -828,7 +850,7 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
     g.join_at = (int)((bytes + 127) & ~(size_t)127);
     if (g.split > 1) bytes = g.join_at + sums;
     g.slab_at = (int)((bytes + 127) & ~(size_t)127);
-    if (!e.vec) bytes = g.slab_at + Block<CG, RUN>::threads / 32 * kSplitSlab * 4;
+    if (!e.vec) bytes = g.slab_at + Block<CG, RUN>::warps * kSplitSlab * 4;
   }
   bytes += 2048;  // barriers, alignment
   if (bytes < tmem_share(2 * BN)) bytes = tmem_share(2 * BN);
@@ -887,8 +909,13 @@ static int run_form(const Form &f, Maps &maps, ProductArgs g, const Epilogue &e,
   // more CTAs than SMs: two to an SM, so that one computes while the other joins
   size_t cap = (ctas > sms ? 92 : 190) * 1024;
   if (f.split > 1) cap -= (size_t)(g.M < 128 ? g.M : 128) * f.bn * 4;  // the joined sums
-  if (f.bn == 128) return launch<T, PLANES, 1, 128, true, false>(maps, g, e, (int)ctas, cap, st);
-  return launch<T, PLANES, 1, 64, true, false>(maps, g, e, (int)ctas, cap, st);
+  // one chain needs no running sums, except f32's, which are many
+  if (PLANES == 3 || (int64_t)g.chain * g.split < g.nk)
+    return launch<T, PLANES, 1, 64, true, false>(maps, g, e, (int)ctas, cap, st);
+  if constexpr (PLANES == 1) {
+    if (f.bn == 128) return launch<T, 1, 1, 128, false, false>(maps, g, e, (int)ctas, cap, st);
+    return launch<T, 1, 1, 64, false, false>(maps, g, e, (int)ctas, cap, st);
+  }
 }
 
 int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, const Epilogue &e,
@@ -947,8 +974,10 @@ Form pick_form(int M, int N, int K, int planes, int sms) {
   const int nk = (int)((K + (int64_t)bk - 1) / bk);
   const double rows = M < 128 ? M / 128.0 : 1.0;
   for (int bn = 64; bn <= 128; bn *= 2)
-    // (128-wide CTAs run one to an SM, and not enough clusters of 8 then fit)
+    // (128-wide CTAs take one chain of 16-bit products, and run one to an SM, so
+    // that not enough clusters of 8 fit)
     for (int split = 1; split <= (bn == 64 ? 8 : 4) && split <= nk; split *= 2) {
+      if (bn == 128 && (planes == 3 || nk > (int64_t)kChain16 * split)) continue;
       const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
       if (ctas > 1e8) continue;
       const double fixed = 1.8 + rows * (bn == 64 ? 2.8 : 4.8);
