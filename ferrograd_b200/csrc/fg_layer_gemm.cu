@@ -956,15 +956,15 @@ int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, con
   }
 }
 
-// The form with the least estimated time, in microseconds.  Measured on one
-// B200 over 17 shapes from 24 x 64 x 2048 to 2048 x 2048 x 2048 in bf16 and f32,
-// every form of each: an MMA step (16 deep) costs a pair 0.07 and a lone CTA
-// 0.052 at either width; around them a pair spends 6.8, a lone CTA 1.8 and its
-// epilogue 2.8 or 4.8 for 128 rows; joining a cluster's sums costs 1.  The
-// 64-wide CTAs run two to an SM and hide each other's fixed part.  It picks the
-// fastest form or one within 10% of it on 15 of the 17 (24 x 8192 x 2048 f16:
-// 64 wide, k over 8 CTAs, 10.6 against 32.3 unsplit; 1024 x 4096 x 4096: pairs,
-// 26.2 against 52.1).
+// The form with the least estimated time, in microseconds.  Fitted on one B200
+// to every form of 17 shapes from 24 x 64 x 2048 to 2048 x 2048 x 2048 in 16 bits
+// and f32: an MMA step (16 deep) costs a pair 0.07 and a lone CTA 0.038 at either
+// width; around them a pair spends 6.8, a lone CTA 1.8 and for 128 rows another
+// 1.9 (64 wide) or 3.4; joining a cluster's sums costs 0.7 and for 128 rows
+// another 1.1 or 3.1.  64-wide CTAs run two to an SM and hide each other's fixed
+// part.  It picks the fastest form or one within 10% of it on all 17 (24 x 8192 x
+// 2048 f16: 64 wide, k over 8 CTAs, 10.2 against 22.7 unsplit and 42.4 by pairs;
+// 1024 x 4096 x 4096 bf16: pairs, 27.6 against 35.1 and 48.3).
 Form pick_form(int M, int N, int K, int planes, int sms) {
   const double steps = K / 16.0 * (planes == 3 ? 6.0 : 1.0);
   Form best{true, 256, 256, 1};
@@ -980,11 +980,11 @@ Form pick_form(int M, int N, int K, int planes, int sms) {
       if (bn == 128 && (planes == 3 || nk > (int64_t)kChain16 * split)) continue;
       const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
       if (ctas > 1e8) continue;
-      const double fixed = 1.8 + rows * (bn == 64 ? 2.8 : 4.8);
-      const int resident = bn == 64 ? 2 : 1;
-      const double load = bn == 64 ? (ctas > sms ? ctas / sms : 1.0) : ceil(ctas / sms);
-      const double c = 1.5 + (split > 1 ? 1.0 : 0.0) + ceil(ctas / (resident * sms)) * fixed +
-                       load * steps / split * 0.052;
+      const double fixed = 1.8 + rows * (bn == 64 ? 1.9 : 3.4);
+      const double join = split > 1 ? 0.7 + rows * (bn == 64 ? 1.1 : 3.1) : 0.0;
+      const double per_sm = split > 1 || bn == 128 ? ceil(ctas / sms) : ctas > sms ? ctas / sms : 1.0;
+      const double turns = bn == 64 ? ceil(ctas / (2.0 * sms)) : per_sm;
+      const double c = 1.5 + join + turns * fixed + per_sm * steps / split * 0.038;
       if (c < cost) {
         cost = c;
         best = Form{false, 128, bn, split};
