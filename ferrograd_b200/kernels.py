@@ -134,17 +134,19 @@ ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GE
 _LAYER_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-def _layer_check(name: str, t: torch.Tensor, like: torch.Tensor, shape, unit_cols=False) -> None:
-    """``t`` is a tensor of this shape on ``like``'s device in its dtype (with
-    ``unit_cols``: its last dimension has stride 1)."""
-    if t.device != like.device:
-        raise ValueError(f"{name}: expected a CUDA tensor on {like.device}, got {t.device}")
-    if t.dtype is not like.dtype:
-        raise ValueError(f"{name}: expected {like.dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if unit_cols and t.stride()[-1] != 1 and t.shape[-1] > 1 and t.numel():
-        raise ValueError(f"{name}: expected unit stride in the last dimension")
+def _layer_check(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, shape,
+                 unit_cols: bool = False) -> None:
+    """``t`` is a tensor of this dtype, device and shape (with ``unit_cols``: its
+    last dimension has stride 1)."""
+    if t.dtype is dtype and t.device == device and t.shape == shape:
+        if unit_cols and t.stride()[-1] != 1 and t.shape[-1] > 1 and t.numel():
+            raise ValueError(f"{name}: expected unit stride in the last dimension")
+        return
+    if t.device != device:
+        raise ValueError(f"{name}: expected a CUDA tensor on {device}, got {t.device}")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _layer_dtype(t: torch.Tensor) -> int:
@@ -166,25 +168,25 @@ def _drop_spec(spec: _lib.DropoutC, drop: Dropout) -> None:
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _layer_run(name: str, args, x: torch.Tensor, stream: Optional[int]) -> None:
-    """Calls ``name`` with the workspace it asks for, on ``x``'s device."""
-    device = x.device.index
-    if device != torch.cuda.current_device():
+def _layer_run(ask, run, args, x: torch.Tensor, device: torch.device,
+               stream: Optional[int]) -> None:
+    """Calls ``run`` with the workspace that ``ask`` names, on ``device``."""
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _layer_run(name, args, x, stream)
-    lib = _lib.lib()
+            return _layer_run(ask, run, args, x, device, stream)
     ref = ctypes.byref(args)
     need = ctypes.c_size_t()
-    code = getattr(lib, name + "_workspace")(ref, ctypes.byref(need))
+    code = ask(ref, ctypes.byref(need))
     if code:
         _lib.check(code)
     if need.value:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(need.value, dtype=torch.uint8)
         if stream is not None:  # the allocator must not hand it out before that stream is done
-            ws.record_stream(torch.cuda.ExternalStream(stream, device=x.device))
+            ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
         args.workspace = ws.data_ptr()
         args.workspace_bytes = need.value
-    code = getattr(lib, name)(ref, _raw_stream(device) if stream is None else stream)
+    code = run(ref, _raw_stream(index) if stream is None else stream)
     if code:
         _lib.check(code)
 
@@ -213,24 +215,26 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     code = _layer_dtype(x)
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError("expected 2-D x and w")
-    if act not in ACTIVATIONS:
+    act_code = ACTIVATIONS.get(act)
+    if act_code is None:
         raise ValueError(f"unknown activation {act!r}")
+    dtype, device = x.dtype, x.device
     M, K = x.shape
     N = w.shape[0]
-    _layer_check("w", w, x, (N, K))
+    _layer_check("w", w, dtype, device, (N, K))
     a = _lib.LinearArgsC(code, M, N, K, x.data_ptr(), *x.stride(), w.data_ptr(), *w.stride())
-    a.act = ACTIVATIONS[act]
+    a.act = act_code
     if bias is not None:
-        _layer_check("bias", bias, x, (N,), True)
+        _layer_check("bias", bias, dtype, device, (N,), True)
         a.bias = bias.data_ptr()
     if residual is not None:
-        _layer_check("residual", residual, x, (M, N), True)
+        _layer_check("residual", residual, dtype, device, (M, N), True)
         a.residual, a.ld_residual = residual.data_ptr(), _ld(residual)
     if out is None:
         out = x.new_empty(M, N)
         a.ld_out = N
     else:
-        _layer_check("out", out, x, (M, N), True)
+        _layer_check("out", out, dtype, device, (M, N), True)
         a.ld_out = _ld(out)
     a.out = out.data_ptr()
     pre = None
@@ -239,7 +243,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
         a.pre, a.ld_pre = pre.data_ptr(), N
     if drop is not None:
         _drop_spec(a.drop, drop)
-    _layer_run("fg_linear", a, x, stream)
+    lib = _lib.lib()
+    _layer_run(lib.fg_linear_workspace, lib.fg_linear, a, x, device, stream)
     return (out, pre) if save_pre else out
 
 
@@ -257,26 +262,28 @@ def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
     code = _layer_dtype(x)
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError("expected 2-D x and w")
-    if act not in ACTIVATIONS:
+    act_code = ACTIVATIONS.get(act)
+    if act_code is None:
         raise ValueError(f"unknown activation {act!r}")
+    dtype, device = x.dtype, x.device
     M, K = x.shape
     N = w.shape[0]
-    _layer_check("w", w, x, (N, K))
-    _layer_check("dy", dy, x, (M, N))
+    _layer_check("w", w, dtype, device, (N, K))
+    _layer_check("dy", dy, dtype, device, (M, N))
     a = _lib.LinearGradArgsC(code, M, N, K, dy.data_ptr(), *dy.stride(), x.data_ptr(),
                              *x.stride(), w.data_ptr(), *w.stride())
-    a.act = ACTIVATIONS[act]
+    a.act = act_code
     if act != "none":
         if pre is None:
             raise ValueError(f"the gradient of {act} needs pre (linear(..., save_pre=True))")
-        _layer_check("pre", pre, x, (M, N), True)
+        _layer_check("pre", pre, dtype, device, (M, N), True)
         a.pre, a.ld_pre = pre.data_ptr(), _ld(pre)
     dx = dw = db = None
     if need_dx:
         dx = x.new_empty(M, K)
         a.dx, a.ld_dx = dx.data_ptr(), K
         if dx_residual is not None:
-            _layer_check("dx_residual", dx_residual, x, (M, K), True)
+            _layer_check("dx_residual", dx_residual, dtype, device, (M, K), True)
             a.dx_residual, a.ld_dx_residual = dx_residual.data_ptr(), _ld(dx_residual)
     elif dx_residual is not None:
         raise ValueError("dx_residual without dx")
@@ -288,7 +295,8 @@ def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
         a.db = db.data_ptr()
     if drop is not None:
         _drop_spec(a.drop, drop)
-    _layer_run("fg_linear_grad", a, x, stream)
+    lib = _lib.lib()
+    _layer_run(lib.fg_linear_grad_workspace, lib.fg_linear_grad, a, x, device, stream)
     return dx, dw, db
 
 
@@ -297,32 +305,35 @@ def dropout(x: torch.Tensor, drop: Optional[Dropout], *, residual: Optional[torc
     """``residual + dropout(x)`` on the last dimension's columns and the rows
     before it (a 1-D tensor is one row).  ``out`` may be ``x`` or the residual."""
     code = _layer_dtype(x)
-    shape = x.shape
-    if out is None:
-        out = x.new_empty(shape)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    flat = len(shape) != 2  # rows are then a contiguous tensor's
     cols = shape[-1] if shape else 1
     rows = x.numel() // cols if cols else 0
-    ptrs = []
-    for name, t in (("x", x), ("residual", residual), ("out", out)):
-        if t is None:
-            ptrs += (None, 0)
-            continue
-        _layer_check(name, t, x, shape, len(shape) > 0)
-        if len(shape) == 2:
-            ptrs += (t.data_ptr(), _ld(t))
-        elif t.is_contiguous():
-            ptrs += (t.data_ptr(), cols)
-        else:
+
+    def pitched(name: str, t: torch.Tensor):
+        _layer_check(name, t, dtype, device, shape, not flat)
+        if not flat:
+            return t.data_ptr(), _ld(t)
+        if not t.is_contiguous():
             raise ValueError(f"{name}: expected a 2-D or a contiguous tensor")
+        return t.data_ptr(), cols
+
+    ptrs = pitched("x", x)
+    ptrs += (None, 0) if residual is None else pitched("residual", residual)
+    if out is None:
+        out = x.new_empty(shape)
+        ptrs += (out.data_ptr(), cols)
+    else:
+        ptrs += pitched("out", out)
     spec = _lib.DropoutC()
     if drop is not None:
         _drop_spec(spec, drop)
-    device = x.device.index
-    if device != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return dropout(x, drop, residual=residual, out=out, stream=stream)
     code = _lib.lib().fg_dropout(code, rows, cols, *ptrs, ctypes.byref(spec),
-                                 _raw_stream(device) if stream is None else stream)
+                                 _raw_stream(index) if stream is None else stream)
     if code:
         _lib.check(code)
     return out
