@@ -34,9 +34,10 @@ def _stale(obj: str, deps: list[str]) -> bool:
 
 
 def build(verbose: bool = False) -> str:
-    """Build the CUDA library, then the front end on top of it."""
+    """Build the CUDA library, then the front end and the layer binding on top of it."""
     lib = build_cuda(verbose)
     build_front(verbose)
+    build_layer(verbose)
     return lib
 
 
@@ -104,6 +105,27 @@ def build_front(verbose: bool = False) -> str:
         cmd = [CXX, *CXXFLAGS, "-shared", f"-I{pybind11.get_include()}",
                f"-I{sysconfig.get_paths()['include']}", py_src, "-o", mod,
                "-L" + HERE, "-lferro_front", "-lferro_cuda", "-Wl,-rpath,$ORIGIN"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+    return mod
+
+
+def build_layer(verbose: bool = False) -> str:
+    """Build the Python module ``_layer`` (the layer operators on torch tensors,
+    linked to ``libferro_cuda.so`` and torch) with g++."""
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    mod = os.path.join(HERE, "_layer" + sysconfig.get_config_var("EXT_SUFFIX"))
+    src = os.path.join(CSRC, "layer_py.cpp")
+    if _stale(mod, [src, os.path.join(ROOT, "include", "ferro_cuda.h")]):
+        abi = int(torch.compiled_with_cxx11_abi())
+        cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+               *[f"-isystem{p}" for p in include_paths()], "-isystem/usr/local/cuda/include",
+               f"-I{sysconfig.get_paths()['include']}", src, "-o", mod, "-L" + HERE,
+               *[f"-L{p}" for p in library_paths()], "-lferro_cuda", "-ltorch_python", "-ltorch_cpu",
+               "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)

@@ -131,72 +131,29 @@ class Dropout(NamedTuple):
 
 ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
                "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
-_LAYER_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_NO_DROP = (0.0, 0, 0)
+_layer_module = None
 
 
-def _layer_check(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, shape,
-                 unit_cols: bool = False) -> None:
-    """``t`` is a tensor of this dtype, device and shape (with ``unit_cols``: its
-    last dimension has stride 1)."""
-    if t.dtype is dtype and t.device == device and t.shape == shape:
-        if unit_cols and t.stride()[-1] != 1 and t.shape[-1] > 1 and t.numel():
-            raise ValueError(f"{name}: expected unit stride in the last dimension")
-        return
-    if t.device != device:
-        raise ValueError(f"{name}: expected a CUDA tensor on {device}, got {t.device}")
-    if t.dtype is not dtype:
-        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
-    raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+def _layer():
+    """The binding of the layer operators (``csrc/layer_py.cpp``)."""
+    global _layer_module
+    if _layer_module is None:
+        _lib.lib()
+        try:
+            from . import _layer as module
+        except ImportError as e:  # pragma: no cover - build problem, fail loudly
+            raise ImportError(
+                "ferrograd_b200._layer is not built; run python -m ferrograd_b200.build") from e
+        _layer_module = module
+    return _layer_module
 
 
-def _layer_dtype(t: torch.Tensor) -> int:
-    if not t.is_cuda:
-        raise ValueError(f"expected a CUDA tensor, got {t.device}")
-    code = _LAYER_DTYPES.get(t.dtype)
+def _act_code(act: str) -> int:
+    code = ACTIVATIONS.get(act)
     if code is None:
-        raise ValueError(f"unsupported dtype {t.dtype}")
+        raise ValueError(f"unknown activation {act!r}")
     return code
-
-
-def _drop_spec(spec: _lib.DropoutC, drop: Dropout) -> None:
-    spec.p = drop.p
-    spec.seed = drop.seed & 0xFFFFFFFFFFFFFFFF
-    spec.offset = drop.offset & 0xFFFFFFFFFFFFFFFF
-
-
-# Handle of the current stream without building a torch.cuda.Stream for it (3 us).
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _layer_run(ask, run, args, x: torch.Tensor, device: torch.device,
-               stream: Optional[int]) -> None:
-    """Calls ``run`` with the workspace that ``ask`` names, on ``device``."""
-    index = device.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _layer_run(ask, run, args, x, device, stream)
-    ref = ctypes.byref(args)
-    need = ctypes.c_size_t()
-    code = ask(ref, ctypes.byref(need))
-    if code:
-        _lib.check(code)
-    if need.value:
-        ws = x.new_empty(need.value, dtype=torch.uint8)
-        if stream is not None:  # the allocator must not hand it out before that stream is done
-            ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
-        args.workspace = ws.data_ptr()
-        args.workspace_bytes = need.value
-    code = run(ref, _raw_stream(index) if stream is None else stream)
-    if code:
-        _lib.check(code)
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Row pitch of a 2-D tensor with unit column stride (rows of one row, or
-    of one element, may carry any stride)."""
-    rows, cols = t.shape
-    pitch = t.stride()[0]
-    return max(pitch, cols) if rows <= 1 else pitch
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -212,40 +169,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     ``(out, pre)``, ``pre`` being the pre-activations ``linear_grad`` needs
     for an activation.  ``out`` may be the residual.
     """
-    code = _layer_dtype(x)
-    if x.dim() != 2 or w.dim() != 2:
-        raise ValueError("expected 2-D x and w")
-    act_code = ACTIVATIONS.get(act)
-    if act_code is None:
-        raise ValueError(f"unknown activation {act!r}")
-    dtype, device = x.dtype, x.device
-    M, K = x.shape
-    N = w.shape[0]
-    _layer_check("w", w, dtype, device, (N, K))
-    a = _lib.LinearArgsC(code, M, N, K, x.data_ptr(), *x.stride(), w.data_ptr(), *w.stride())
-    a.act = act_code
-    if bias is not None:
-        _layer_check("bias", bias, dtype, device, (N,), True)
-        a.bias = bias.data_ptr()
-    if residual is not None:
-        _layer_check("residual", residual, dtype, device, (M, N), True)
-        a.residual, a.ld_residual = residual.data_ptr(), _ld(residual)
-    if out is None:
-        out = x.new_empty(M, N)
-        a.ld_out = N
-    else:
-        _layer_check("out", out, dtype, device, (M, N), True)
-        a.ld_out = _ld(out)
-    a.out = out.data_ptr()
-    pre = None
-    if save_pre:
-        pre = x.new_empty(M, N)
-        a.pre, a.ld_pre = pre.data_ptr(), N
-    if drop is not None:
-        _drop_spec(a.drop, drop)
-    lib = _lib.lib()
-    _layer_run(lib.fg_linear_workspace, lib.fg_linear, a, x, device, stream)
-    return (out, pre) if save_pre else out
+    p, seed, offset = _NO_DROP if drop is None else drop
+    return _layer().linear(x, w, bias, _act_code(act), residual, p, seed, offset, save_pre, out,
+                           stream)
 
 
 def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
@@ -257,86 +183,22 @@ def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
     gradient ``dy`` of its output; ``pre`` is what ``save_pre`` returned (not
     needed for ``act="none"``).  Gradients that are not wanted are ``None``.
     The residual's gradient is ``dy`` itself; ``dx_residual`` [M, K] is added to
-    ``dx`` in the product's epilogue.  With 16-bit types the gradient
-    at the pre-activations is rounded to that type before the two products."""
-    code = _layer_dtype(x)
-    if x.dim() != 2 or w.dim() != 2:
-        raise ValueError("expected 2-D x and w")
-    act_code = ACTIVATIONS.get(act)
-    if act_code is None:
-        raise ValueError(f"unknown activation {act!r}")
-    dtype, device = x.dtype, x.device
-    M, K = x.shape
-    N = w.shape[0]
-    _layer_check("w", w, dtype, device, (N, K))
-    _layer_check("dy", dy, dtype, device, (M, N))
-    a = _lib.LinearGradArgsC(code, M, N, K, dy.data_ptr(), *dy.stride(), x.data_ptr(),
-                             *x.stride(), w.data_ptr(), *w.stride())
-    a.act = act_code
-    if act != "none":
-        if pre is None:
-            raise ValueError(f"the gradient of {act} needs pre (linear(..., save_pre=True))")
-        _layer_check("pre", pre, dtype, device, (M, N), True)
-        a.pre, a.ld_pre = pre.data_ptr(), _ld(pre)
-    dx = dw = db = None
-    if need_dx:
-        dx = x.new_empty(M, K)
-        a.dx, a.ld_dx = dx.data_ptr(), K
-        if dx_residual is not None:
-            _layer_check("dx_residual", dx_residual, dtype, device, (M, K), True)
-            a.dx_residual, a.ld_dx_residual = dx_residual.data_ptr(), _ld(dx_residual)
-    elif dx_residual is not None:
-        raise ValueError("dx_residual without dx")
-    if need_dw:
-        dw = x.new_empty(N, K)
-        a.dw, a.ld_dw = dw.data_ptr(), K
-    if need_db:
-        db = x.new_empty(N)
-        a.db = db.data_ptr()
-    if drop is not None:
-        _drop_spec(a.drop, drop)
-    lib = _lib.lib()
-    _layer_run(lib.fg_linear_grad_workspace, lib.fg_linear_grad, a, x, device, stream)
-    return dx, dw, db
+    ``dx`` in the product's epilogue.  With 16-bit types the gradient at the
+    pre-activations is rounded to that type before the two products."""
+    code = _act_code(act)
+    if code and pre is None:
+        raise ValueError(f"the gradient of {act} needs pre (linear(..., save_pre=True))")
+    p, seed, offset = _NO_DROP if drop is None else drop
+    return _layer().linear_grad(dy, x, w, pre, code, p, seed, offset, need_dx, need_dw, need_db,
+                                dx_residual, stream)
 
 
 def dropout(x: torch.Tensor, drop: Optional[Dropout], *, residual: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
     """``residual + dropout(x)`` on the last dimension's columns and the rows
     before it (a 1-D tensor is one row).  ``out`` may be ``x`` or the residual."""
-    code = _layer_dtype(x)
-    shape, dtype, device = x.shape, x.dtype, x.device
-    flat = len(shape) != 2  # rows are then a contiguous tensor's
-    cols = shape[-1] if shape else 1
-    rows = x.numel() // cols if cols else 0
-
-    def pitched(name: str, t: torch.Tensor):
-        _layer_check(name, t, dtype, device, shape, not flat)
-        if not flat:
-            return t.data_ptr(), _ld(t)
-        if not t.is_contiguous():
-            raise ValueError(f"{name}: expected a 2-D or a contiguous tensor")
-        return t.data_ptr(), cols
-
-    ptrs = pitched("x", x)
-    ptrs += (None, 0) if residual is None else pitched("residual", residual)
-    if out is None:
-        out = x.new_empty(shape)
-        ptrs += (out.data_ptr(), cols)
-    else:
-        ptrs += pitched("out", out)
-    spec = _lib.DropoutC()
-    if drop is not None:
-        _drop_spec(spec, drop)
-    index = device.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return dropout(x, drop, residual=residual, out=out, stream=stream)
-    code = _lib.lib().fg_dropout(code, rows, cols, *ptrs, ctypes.byref(spec),
-                                 _raw_stream(index) if stream is None else stream)
-    if code:
-        _lib.check(code)
-    return out
+    p, seed, offset = _NO_DROP if drop is None else drop
+    return _layer().dropout(x, residual, p, seed, offset, out, stream)
 
 
 def dropout_grad(dy: torch.Tensor, drop: Optional[Dropout], *, out: Optional[torch.Tensor] = None,
