@@ -548,7 +548,7 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
   place_operand(&p.w, g->workspace);
   place_jobs(&p.jobs, g->workspace);
   if ((rc = run_stage(g->dtype, p.jobs, st))) return rc;
-  return run_tensor_product(g->dtype, p.x, p.w, g->K, e, st);
+  return run_tensor_product(g->dtype, {p.x, p.w, g->K, e}, st);
 }
 
 // How k_layer_dz is cut: blocks of 256 columns for large arrays (16384 x 16384
@@ -731,26 +731,24 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
     }
     if (rc) return rc;
   }
-  Epilogue e{};
-  if (p.dx) {  // dx[m, k] = sum_n dz(m, n) w(n, k)
-    e.out = g->dx;
-    e.ldo = g->ld_dx;
-    e.residual = g->dx_residual;
-    e.ldr = g->ld_dx_residual;
-    e.M = g->M;
-    e.N = g->K;
-    e.vec = rows16(e.out, e.ldo, es) && rows16(e.residual, e.ldr, es);
-    if ((rc = run_tensor_product(g->dtype, p.z_dx, p.w, g->N, e, st))) return rc;
-  }
-  if (p.dw) {  // dw[n, k] = sum_m dz(m, n) x(m, k)
-    e.residual = nullptr;
-    e.out = g->dw;
-    e.ldo = g->ld_dw;
-    e.M = g->N;
-    e.N = g->K;
-    e.vec = rows16(e.out, e.ldo, es);
-    if ((rc = run_tensor_product(g->dtype, p.z_dw, p.x, g->M, e, st))) return rc;
-  }
+  Product dx{p.z_dx, p.w, g->N, {}}, dw{p.z_dw, p.x, g->M, {}};
+  // dx[m, k] = sum_n dz(m, n) w(n, k)
+  dx.e.out = g->dx;
+  dx.e.ldo = g->ld_dx;
+  dx.e.residual = g->dx_residual;
+  dx.e.ldr = g->ld_dx_residual;
+  dx.e.M = g->M;
+  dx.e.N = g->K;
+  dx.e.vec = rows16(g->dx, g->ld_dx, es) && rows16(g->dx_residual, g->ld_dx_residual, es);
+  // dw[n, k] = sum_m dz(m, n) x(m, k)
+  dw.e.out = g->dw;
+  dw.e.ldo = g->ld_dw;
+  dw.e.M = g->N;
+  dw.e.N = g->K;
+  dw.e.vec = rows16(g->dw, g->ld_dw, es);
+  if (p.dx && p.dw) return run_tensor_products(g->dtype, dx, dw, st);
+  if (p.dx) return run_tensor_product(g->dtype, dx, st);
+  if (p.dw) return run_tensor_product(g->dtype, dw, st);
   return FG_OK;
 }
 

@@ -611,8 +611,14 @@ struct Form {
   int bm, bn, split;
 };
 Form pick_form(int M, int N, int K, int planes, int sms);
-int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, const Epilogue &e,
-                       cudaStream_t st);
+// A product of rows and columns e.M, e.N over K with its epilogue.
+struct Product {
+  Operand a, b;
+  int K;
+  Epilogue e;
+};
+int run_tensor_product(int dtype, const Product &x, cudaStream_t st);
+int run_tensor_products(int dtype, const Product &x, const Product &y, cudaStream_t st);
 
 // An f32 value as the sum of three bf16 values, each rest exact (an infinity
 // is its own first part; a value that would round up to infinity is cut).

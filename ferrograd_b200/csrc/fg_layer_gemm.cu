@@ -126,14 +126,33 @@ struct Maps {
   CUtensorMap a, b, out, pre, residual;
 };
 
+// What a launch computes: one product, or two (split form) of which the first
+// takes the first `ctas` CTAs.
+struct Problem {
+  Maps maps;
+  ProductArgs g;
+  Epilogue e;
+};
+template <bool TWO>
+struct Problems {
+  Problem at[TWO ? 2 : 1];
+  int ctas;
+};
+
 // IO (pair form): out, pre and the residual pass through shared memory by TMA.
 // At 64 bytes of operands in and 64 out a cycle, the MMAs of 16-bit operands
 // leave next to nothing of shared memory's 128, and a warp's 16-byte global
 // accesses to 32 rows cost it 32 passes; a TMA block costs 8 to write and 8 to
 // read.  It needs rows on 16-byte boundaries.
-template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO>
+template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO, bool TWO>
 __global__ void __launch_bounds__(Block<CG, RUN>::threads, CG == 1 && !RUN ? 2 : 1)
-    k_layer_product(const __grid_constant__ Maps maps, const ProductArgs g, const Epilogue e) {
+    k_layer_product(const __grid_constant__ Problems<TWO> ps) {
+  const bool other = TWO && blockIdx.x >= ps.ctas;
+  const Problem &pr = ps.at[TWO && other ? 1 : 0];
+  const int block_id = TWO && other ? blockIdx.x - ps.ctas : blockIdx.x;
+  const Maps &maps = pr.maps;
+  const ProductArgs &g = pr.g;
+  const Epilogue &e = pr.e;
   const CUtensorMap &tma = maps.a, &tmb = maps.b;
   constexpr int BK = Depth<PLANES>::BK;
   constexpr int kFirstEpi = Block<CG, RUN>::first_epi;  // first epilogue warp
@@ -162,13 +181,13 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, CG == 1 && !RUN ? 2 :
   // (the shuffle tells the compiler that a warp's index is the same in all its
   // lanes, and so the branches and operands that follow from it)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? blockIdx.x & 1 : blockIdx.x % g.split;  // in the cluster
+  const uint32_t rank = CG == 2 ? block_id & 1 : block_id % g.split;  // in the cluster
   const bool leader = CG == 1 || rank == 0;
   const int num_m = (g.M + BM - 1) / BM, num_n = (g.N + BN - 1) / BN;
   const int S = g.stages;
 
   // This CTA's work: whole tiles (pair), or one tile's share of k (split).
-  const int first = CG == 2 ? blockIdx.x / 2 : blockIdx.x / g.split;
+  const int first = CG == 2 ? block_id / 2 : block_id / g.split;
   const int step = CG == 2 ? gridDim.x / 2 : num_m * num_n;
   const int k0 = CG == 2 ? 0 : (int)((long long)g.nk * rank / g.split);
   const int k1 = CG == 2 ? g.nk : (int)((long long)g.nk * (rank + 1) / g.split);
@@ -824,11 +843,11 @@ static int make_io_map(CUtensorMap *map, const void *ptr, int M, int N, int64_t 
 // wait while its cluster's other CTAs hold theirs could wait for ever.
 static size_t tmem_share(int cols) { return (size_t)cols / 128 * 47 * 1024; }
 
-template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO>
-static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, size_t ring_cap,
-                  cudaStream_t st) {
+// Lays out a product's shared memory (its stages and what follows the ring);
+// returns the bytes.
+template <int PLANES, int CG, int BN, bool RUN, bool IO>
+static size_t lay_out(ProductArgs &g, const Epilogue &e, size_t ring_cap) {
   constexpr int BK = Depth<PLANES>::BK;
-  auto kern = k_layer_product<T, PLANES, CG, BN, RUN, IO>;
   const size_t stage = (size_t)PLANES * (g.a.rows + g.b.rows) * BK * 2;
   // past the ring: the pair's blocks or slabs, or what an MMA of 128 rows reads
   // beyond an A tile of fewer (it lands in unused accumulator rows)
@@ -853,7 +872,17 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
     if (!e.vec) bytes = g.slab_at + Block<CG, RUN>::warps * kSplitSlab * 4;
   }
   bytes += 2048;  // barriers, alignment
-  if (bytes < tmem_share(2 * BN)) bytes = tmem_share(2 * BN);
+  return bytes < tmem_share(2 * BN) ? tmem_share(2 * BN) : bytes;
+}
+
+template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO, bool TWO>
+static int launch(Problems<TWO> &ps, int ctas, size_t ring_cap, cudaStream_t st) {
+  auto kern = k_layer_product<T, PLANES, CG, BN, RUN, IO, TWO>;
+  size_t bytes = 0;
+  for (Problem &pr : ps.at) {
+    const size_t b = lay_out<PLANES, CG, BN, RUN, IO>(pr.g, pr.e, ring_cap);
+    if (bytes < b) bytes = b;
+  }
   static bool attr_done[64] = {};
   int dev = 0;
   FG_CUDA_TRY(cudaGetDevice(&dev));
@@ -869,22 +898,35 @@ static int launch(const Maps &maps, ProductArgs g, const Epilogue &e, int ctas, 
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG == 2 ? 2 : g.split;
+  attr[0].val.clusterDim.x = CG == 2 ? 2 : ps.at[0].g.split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, g, e));
+  FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ps));
   count_launch();
   return FG_OK;
 }
 
+static int64_t tiles_of(const Epilogue &e, int bm, int bn) {
+  return (e.M + (int64_t)bm - 1) / bm * ((e.N + (int64_t)bn - 1) / bn);
+}
+
+// Shared memory of a split CTA's ring: with more CTAs than SMs two fit an SM, so
+// that one computes while the other joins; less the joined sums.
+static size_t split_ring(int64_t ctas, int sms, int M, int bn, int split) {
+  const size_t cap = (ctas > sms ? 92 : 190) * 1024;
+  return split > 1 ? cap - (size_t)(M < 128 ? M : 128) * bn * 4 : cap;
+}
+
 template <typename T, int PLANES>
-static int run_form(const Form &f, Maps &maps, ProductArgs g, const Epilogue &e, int sms,
-                    cudaStream_t st) {
-  const int64_t tiles = (int64_t)((g.M + f.bm - 1) / f.bm) * ((g.N + f.bn - 1) / f.bn);
+static int run_form(const Form &f, Problems<false> &ps, int sms, cudaStream_t st) {
+  Maps &maps = ps.at[0].maps;
+  const ProductArgs &g = ps.at[0].g;
+  const Epilogue &e = ps.at[0].e;
+  const int64_t tiles = tiles_of(e, f.bm, f.bn);
   if (f.pair) {
     const int pairs = sms / 2;
     const int ctas = 2 * (int)(tiles < pairs ? tiles : pairs);
@@ -897,62 +939,107 @@ static int run_form(const Form &f, Maps &maps, ProductArgs g, const Epilogue &e,
       if (!rc && e.pre) rc = make_io_map<T>(&maps.pre, e.pre, e.M, e.N, e.ldp);
       if (!rc && e.residual) rc = make_io_map<T>(&maps.residual, e.residual, e.M, e.N, e.ldr);
       if (rc) return rc;
-      if (g.chain >= g.nk)
-        return launch<T, PLANES, 2, 256, kLong, true>(maps, g, e, ctas, ring, st);
-      return launch<T, PLANES, 2, 256, true, true>(maps, g, e, ctas, 192 * 1024, st);
+      if (g.chain >= g.nk) return launch<T, PLANES, 2, 256, kLong, true, false>(ps, ctas, ring, st);
+      return launch<T, PLANES, 2, 256, true, true, false>(ps, ctas, 192 * 1024, st);
     }
-    if (g.chain >= g.nk)
-      return launch<T, PLANES, 2, 256, kLong, false>(maps, g, e, ctas, ring, st);
-    return launch<T, PLANES, 2, 256, true, false>(maps, g, e, ctas, 192 * 1024, st);
+    if (g.chain >= g.nk) return launch<T, PLANES, 2, 256, kLong, false, false>(ps, ctas, ring, st);
+    return launch<T, PLANES, 2, 256, true, false, false>(ps, ctas, 192 * 1024, st);
   }
   const int64_t ctas = tiles * f.split;
-  // more CTAs than SMs: two to an SM, so that one computes while the other joins
-  size_t cap = (ctas > sms ? 92 : 190) * 1024;
-  if (f.split > 1) cap -= (size_t)(g.M < 128 ? g.M : 128) * f.bn * 4;  // the joined sums
+  const size_t ring = split_ring(ctas, sms, g.M, f.bn, f.split);
   // one chain needs no running sums, except f32's, which are many
   if (PLANES == 3 || (int64_t)g.chain * g.split < g.nk)
-    return launch<T, PLANES, 1, 64, true, false>(maps, g, e, (int)ctas, cap, st);
+    return launch<T, PLANES, 1, 64, true, false, false>(ps, (int)ctas, ring, st);
   if constexpr (PLANES == 1) {
-    if (f.bn == 128) return launch<T, 1, 1, 128, false, false>(maps, g, e, (int)ctas, cap, st);
-    return launch<T, 1, 1, 64, false, false>(maps, g, e, (int)ctas, cap, st);
+    if (f.bn == 128) return launch<T, 1, 1, 128, false, false, false>(ps, (int)ctas, ring, st);
+    return launch<T, 1, 1, 64, false, false, false>(ps, (int)ctas, ring, st);
   }
 }
 
-int run_tensor_product(int dtype, const Operand &a, const Operand &b, int K, const Epilogue &e,
-                       cudaStream_t st) {
-  DevCtx *ctx = ctx_current();
-  if (!ctx) return set_error(FG_ERR_CUDA, "no CUDA device context");
-  const int sms = ctx->num_sms ? ctx->num_sms : 148;
-  const int planes = dtype == FG_F32 ? 3 : 1;
-  const bool bf16 = dtype != FG_F16;
+// Two products whose tiles do not fill the SMs by themselves, in one launch of
+// 64-wide split tiles with the same split.
+template <typename T, int PLANES>
+static int run_two(Problems<true> &ps, int64_t ctas, int sms, cudaStream_t st) {
+  const int m = ps.at[0].g.M > ps.at[1].g.M ? ps.at[0].g.M : ps.at[1].g.M;
+  const size_t ring = split_ring(ctas, sms, m, 64, ps.at[0].g.split);
+  return launch<T, PLANES, 1, 64, PLANES == 3, false, true>(ps, (int)ctas, ring, st);
+}
+
+static int k_blocks(int K, int planes) {
   const int bk = planes == 3 ? 32 : 64;
-  const Form f = pick_form(e.M, e.N, K, planes, sms);
-  ProductArgs g{};
+  return (int)((K + (int64_t)bk - 1) / bk);
+}
+
+static int make_problem(Problem *pr, int dtype, const Operand &a, const Operand &b, int K,
+                        const Epilogue &e, const Form &f, unsigned int *err) {
+  const int planes = dtype == FG_F32 ? 3 : 1, bk = planes == 3 ? 32 : 64;
+  const bool bf16 = dtype != FG_F16;
+  ProductArgs &g = pr->g;
   g.M = e.M;
   g.N = e.N;
-  g.nk = (int)((K + (int64_t)bk - 1) / bk);
+  g.nk = k_blocks(K, planes);
   g.chain = planes == 3 ? 2 : kChain16;
   g.split = f.split;
   g.group = f.pair ? 16 : 8;
   g.bf16 = bf16;
-  g.err = ctx->d_err;
+  g.err = err;
   const int unit_a = a.mn_major ? 64 : 16;
   g.a.mn_major = a.mn_major;
-  g.a.rows = e.M >= 128 ? 128 : (e.M + unit_a - 1) / unit_a * unit_a;
+  g.a.rows = f.pair || e.M >= 128 ? 128 : (e.M + unit_a - 1) / unit_a * unit_a;
   g.b.mn_major = b.mn_major;
   g.b.rows = f.pair ? 128 : f.bn;
-  if (f.pair) g.a.rows = 128;
-  Maps maps = {};
-  int rc = make_map(&maps.a, a, bk, g.a.rows, bf16);
+  pr->e = e;
+  int rc = make_map(&pr->maps.a, a, bk, g.a.rows, bf16);
+  return rc ? rc : make_map(&pr->maps.b, b, bk, g.b.rows, bf16);
+}
+
+int run_tensor_product(int dtype, const Product &x, cudaStream_t st) {
+  DevCtx *ctx = ctx_current();
+  if (!ctx) return set_error(FG_ERR_CUDA, "no CUDA device context");
+  const int sms = ctx->num_sms ? ctx->num_sms : 148;
+  const Form f = pick_form(x.e.M, x.e.N, x.K, dtype == FG_F32 ? 3 : 1, sms);
+  Problems<false> ps = {};
+  int rc = make_problem(&ps.at[0], dtype, x.a, x.b, x.K, x.e, f, ctx->d_err);
   if (rc) return rc;
-  if ((rc = make_map(&maps.b, b, bk, g.b.rows, bf16))) return rc;
   switch (dtype) {
     case FG_F32:
-      return run_form<float, 3>(f, maps, g, e, sms, st);
+      return run_form<float, 3>(f, ps, sms, st);
     case FG_BF16:
-      return run_form<__nv_bfloat16, 1>(f, maps, g, e, sms, st);
+      return run_form<__nv_bfloat16, 1>(f, ps, sms, st);
     default:
-      return run_form<__half, 1>(f, maps, g, e, sms, st);
+      return run_form<__half, 1>(f, ps, sms, st);
+  }
+}
+
+// Two independent products (a gradient's dx and dw): in one launch where each
+// alone would leave SMs idle and the 64-wide tiles of both fit them twice over.
+int run_tensor_products(int dtype, const Product &x, const Product &y, cudaStream_t st) {
+  DevCtx *ctx = ctx_current();
+  if (!ctx) return set_error(FG_ERR_CUDA, "no CUDA device context");
+  const int sms = ctx->num_sms ? ctx->num_sms : 148;
+  const int planes = dtype == FG_F32 ? 3 : 1;
+  const int nkx = k_blocks(x.K, planes), nky = k_blocks(y.K, planes);
+  const int64_t tiles = tiles_of(x.e, 128, 64) + tiles_of(y.e, 128, 64);
+  int split = 1;  // as far as both have k-blocks and the CTAs one turn
+  while (split < 8 && 2 * split <= nkx && 2 * split <= nky && tiles * 2 * split <= sms) split *= 2;
+  const bool one_chain = planes == 3 || (nkx <= kChain16 * split && nky <= kChain16 * split);
+  if (!one_chain || tiles > 2 * sms) {
+    int rc = run_tensor_product(dtype, x, st);
+    return rc ? rc : run_tensor_product(dtype, y, st);
+  }
+  const Form f{false, 128, 64, split};
+  Problems<true> ps = {};
+  ps.ctas = (int)(tiles_of(x.e, 128, 64) * split);
+  int rc = make_problem(&ps.at[0], dtype, x.a, x.b, x.K, x.e, f, ctx->d_err);
+  if (rc) return rc;
+  if ((rc = make_problem(&ps.at[1], dtype, y.a, y.b, y.K, y.e, f, ctx->d_err))) return rc;
+  switch (dtype) {
+    case FG_F32:
+      return run_two<float, 3>(ps, tiles * split, sms, st);
+    case FG_BF16:
+      return run_two<__nv_bfloat16, 1>(ps, tiles * split, sms, st);
+    default:
+      return run_two<__half, 1>(ps, tiles * split, sms, st);
   }
 }
 
