@@ -127,6 +127,32 @@ __device__ __forceinline__ void store8<float>(float *p, const float (&v)[8]) {
   reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
+// Eight consecutive elements from any address.  16-bit types come as 4-byte words,
+// shifted together where the address is odd among them; the words then reach
+// one element to either side, so an address nearer than that to the ends of the
+// array [lo, hi) is read element by element.
+template <typename T>
+__device__ __forceinline__ void load8_off(const T *p, const T *lo, const T *hi, float (&v)[8]) {
+  if (sizeof(T) == 2 && p - 1 >= lo && p + 9 <= hi) {
+    const bool odd = (reinterpret_cast<uintptr_t>(p) & 2) != 0;
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(p - odd);
+    uint32_t t[5];
+#pragma unroll
+    for (int i = 0; i < 4; i++) t[i] = w[i];
+    t[4] = odd ? w[4] : 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t u = odd ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
+      const float2 f = unpack2(u, typename Half16<T>::type{});
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = to_f32<T>(p[i]);
+  }
+}
+
 // ---- activations ------------------------------------------------------------
 // ReLU is the framework's (0 < z) ? z : 0, so a NaN gives 0.  The others pass
 // NaN on and take their limits (0 and z) far from 0: the formulas' products

@@ -709,6 +709,8 @@ __global__ void __launch_bounds__(256) k_stage(const StageJobs jobs) {
     float v[8];
     if (j.vec && x + 8 <= j.inner) {
       load8<T>(src + at.row * j.so + x, v);
+    } else if (j.si == 1 && x + 8 <= j.inner) {
+      load8_off<T>(src + at.row * j.so + x, src, src + (j.outer - 1) * j.so + j.inner, v);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; k++)
