@@ -64,18 +64,28 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------------------
 // Up to 8 rows of x: C = x w^T with w's rows contiguous, in f32 on the CUDA
-// cores.  The weight is read once, a warp two of its rows at a time, each lane
-// 16 bytes of a row; what bounds it is that stream, so a lane asks for the next
-// four steps before it multiplies.  The warp's sums meet by shuffles in a
+// cores.  The weight is read once, a warp one or two of its rows at a time, each
+// lane 16 bytes of a row; what bounds it is that stream, so a lane asks for the
+// next four steps before it multiplies.  The warp's sums meet by shuffles in a
 // fixed order.  (A tensor-core tile of so few rows first fills and drains
-// accumulators, and joins its k-ranges across CTAs: 1 x 4096 x 4096 bf16 11.0
-// us against 7.6 us here.)  VEC: every row starts on a 16-byte boundary;
+// accumulators, and joins its k-ranges across CTAs: 1 x 4096 x 4096 bf16, the
+// weight from HBM, 11.6 us against 8.3 us here, 4.0 TB/s.)  VEC: every row starts on a 16-byte boundary;
 // without it elements are read one by one, still in neighbouring lanes.
 // ---------------------------------------------------------------------------
 using ptx::grid_launch_next;
 using ptx::grid_wait;
 
 constexpr int kRowsMax = 8;
+
+// For MR rows of x: the weight's rows a warp takes, and the steps it has in
+// flight.  One 16-bit row of 4096 by itself is 1 x 4096 x 4096 from HBM in 8.3 us,
+// two together 11.6; two f32 rows 15.5, one 16.2.
+template <typename T, int MR>
+struct RowsShape {
+  static constexpr int rows = sizeof(T) == 2 ? 1 : 2;
+  static constexpr int steps = MR <= 4 ? 4 : 2;
+};
+
 // Rows up to which it beats the tensor cores' few-row tiles (4096 x 4096): in
 // f32 8 (22 us against 56, which has to split the weight into planes first),
 // in 16 bits 2, or 4 where the weight would have to be copied to be aligned.
@@ -124,19 +134,22 @@ __global__ void __launch_bounds__(256)
     k_linear_rows(const T *__restrict__ x, int64_t xr, const T *__restrict__ w, int64_t wr, int K,
                   const Epilogue e) {
   constexpr int V = VEC ? 16 / sizeof(T) : 1;  // elements a lane reads at once
-  constexpr int U = MR == 1 ? 8 : MR <= 4 ? 4 : 2;  // steps in flight (rows past M repeat the last)
+  constexpr int R = RowsShape<T, MR>::rows, U = RowsShape<T, MR>::steps;
   const int lane = threadIdx.x & 31;
-  const int n0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 2;
+  const int n0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * R;
+  grid_wait();
+  grid_launch_next();
   if (n0 >= e.N) return;
-  const T *w0 = w + n0 * wr;
-  const T *w1 = n0 + 1 < e.N ? w0 + wr : w0;
-  float acc[MR][2] = {};
+  const T *wp[R];
+#pragma unroll
+  for (int c = 0; c < R; c++) wp[c] = w + min(n0 + c, e.N - 1) * wr;
+  float acc[MR][R] = {};
   using Raw = typename RawOf<T, VEC>::type;
   auto read = [](const T *p) { return __ldg(reinterpret_cast<const Raw *>(p)); };
-  auto step = [&](int64_t k, const Raw &ra, const Raw &rb) {
-    float a[V], b[V];
-    unraw<T>(ra, a);
-    unraw<T>(rb, b);
+  auto step = [&](int64_t k, const Raw(&rw)[R]) {
+    float b[R][V];
+#pragma unroll
+    for (int c = 0; c < R; c++) unraw<T>(rw[c], b[c]);
     Raw rx[MR];
 #pragma unroll
     for (int m = 0; m < MR; m++) rx[m] = read(x + min(m, e.M - 1) * xr + k);
@@ -145,59 +158,59 @@ __global__ void __launch_bounds__(256)
       float t[V];
       unraw<T>(rx[m], t);
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        acc[m][0] = fmaf(t[i], a[i], acc[m][0]);
-        acc[m][1] = fmaf(t[i], b[i], acc[m][1]);
-      }
+      for (int i = 0; i < V; i++)
+#pragma unroll
+        for (int c = 0; c < R; c++) acc[m][c] = fmaf(t[i], b[c][i], acc[m][c]);
     }
   };
   constexpr int S = 32 * V;  // elements of a row in one step of the warp
   int64_t k = lane * V;
   for (; k + (U - 1) * S + V <= K; k += U * S) {
-    Raw a[U], b[U];
+    Raw r[U][R];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      a[u] = read(w0 + k + u * S);
-      b[u] = read(w1 + k + u * S);
-    }
+    for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int u = 0; u < U; u++) step(k + u * S, a[u], b[u]);
+      for (int c = 0; c < R; c++) r[u][c] = read(wp[c] + k + u * S);
+#pragma unroll
+    for (int u = 0; u < U; u++) step(k + u * S, r[u]);
   }
-  for (; k + V <= K; k += S) step(k, read(w0 + k), read(w1 + k));
+  for (; k + V <= K; k += S) {
+    Raw r[R];
+#pragma unroll
+    for (int c = 0; c < R; c++) r[c] = read(wp[c] + k);
+    step(k, r);
+  }
   if (VEC && k < K)  // the row's last elements, fewer than V (one lane has them)
     for (; k < K; k++)
 #pragma unroll
       for (int m = 0; m < MR; m++) {
         const float t = to_f32<T>(x[min(m, e.M - 1) * xr + k]);
-        acc[m][0] = fmaf(t, to_f32<T>(w0[k]), acc[m][0]);
-        acc[m][1] = fmaf(t, to_f32<T>(w1[k]), acc[m][1]);
+#pragma unroll
+        for (int c = 0; c < R; c++) acc[m][c] = fmaf(t, to_f32<T>(wp[c][k]), acc[m][c]);
       }
 #pragma unroll
   for (int m = 0; m < MR; m++)
 #pragma unroll
-    for (int c = 0; c < 2; c++) {
+    for (int c = 0; c < R; c++) {
       float s = acc[m][c];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == m * 2 + c && m < e.M && n0 + c < e.N) epilogue1<T>(e, m, n0 + c, s);
+      if (lane == m * R + c && m < e.M && n0 + c < e.N) epilogue1<T>(e, m, n0 + c, s);
     }
 }
 
 template <typename T>
 static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaStream_t st) {
-  const unsigned grid = (unsigned)((g->N + 15LL) / 16);
   const T *x = static_cast<const T *>(g->x), *w = static_cast<const T *>(g->w);
-  auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(x, g->x_row, w, g->w_row, g->K, e); };
-  if (g->M == 1)
-    vec ? go(k_linear_rows<T, 1, true>) : go(k_linear_rows<T, 1, false>);
-  else if (g->M == 2)
-    vec ? go(k_linear_rows<T, 2, true>) : go(k_linear_rows<T, 2, false>);
-  else if (g->M <= 4)
-    vec ? go(k_linear_rows<T, 4, true>) : go(k_linear_rows<T, 4, false>);
-  else
-    vec ? go(k_linear_rows<T, 8, true>) : go(k_linear_rows<T, 8, false>);
-  FG_LAUNCH_TRY();
-  return FG_OK;
+  auto go = [&](auto kern) {
+    const int per = 8 * RowsShape<T, 1>::rows;
+    const unsigned grid = (unsigned)((g->N + (int64_t)per - 1) / per);
+    return launch_early(kern, dim3(grid), 256, st, x, g->x_row, w, g->w_row, g->K, e);
+  };
+  if (g->M == 1) return vec ? go(k_linear_rows<T, 1, true>) : go(k_linear_rows<T, 1, false>);
+  if (g->M == 2) return vec ? go(k_linear_rows<T, 2, true>) : go(k_linear_rows<T, 2, false>);
+  if (g->M <= 4) return vec ? go(k_linear_rows<T, 4, true>) : go(k_linear_rows<T, 4, false>);
+  return vec ? go(k_linear_rows<T, 8, true>) : go(k_linear_rows<T, 8, false>);
 }
 
 // ---------------------------------------------------------------------------
