@@ -530,3 +530,95 @@ def test_refusals():
     kernels.linear(both[:, :6], torch.ones((5, 6), device="cuda"), out=both[:, 6:11])
     assert torch.equal(both[:, 6:11], torch.full((4, 5), 6.0, device="cuda"))
     assert torch.equal(both[:, :6], torch.ones((4, 6), device="cuda"))
+
+
+# ---- large sizes, against 64 bits on the device ----------------------------------------
+
+
+def device_check(got, ref, tol, what):
+    bad = ~((got.double() - ref).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:4], ref[bad][:4])
+
+
+def device_act(z, act):
+    if act == "gelu":
+        return z * 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    return z.clamp(min=0.0) if act == "relu" else z
+
+
+LARGE = [(2560, 2304, 320), (2501, 2311, 333), (2050, 4100, 1031), (4097, 1280, 4104),
+         (1024, 1024, 20480), (2048, 2304, 17000), (96, 72, 40000), (130, 77, 33001)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_linear_large(dtype, m, n, k):
+    """The same bounds as above; every form of the product, chains of 16384 and
+    longer among them."""
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+    dt = TYPES[dtype]
+    new = lambda r, c, s: torch.empty((r, c), dtype=dt, device="cuda").normal_(  # noqa: E731
+        0, s, generator=gen)
+    x, w, b, r = new(m, k, 1), new(n, k, 1 / math.sqrt(k)), new(1, n, 1)[0], new(m, n, 1)
+    act = "gelu" if k % 2 else "relu"
+    spec = (0.2, 31, 1 << 35)
+    out, pre = kernels.linear(x, w, b, act=act, residual=r, drop=kernels.Dropout(*spec),
+                              save_pre=True)
+    z = x.double() @ w.double().t() + b.double()
+    size = x.double().abs() @ w.double().abs().t() + b.double().abs()
+    tz = (k + 16) * STEP * size
+    u, tiny = ROUND[dtype], TINY[dtype]
+    device_check(pre, z, tz + u * z.abs() + tiny, "pre")
+    keep = torch.from_numpy(keep_mask(m, n, *spec)).cuda()
+    scale = 65536.0 / (65536 - math.floor(spec[0] * 65536 + 0.5))
+    ref = torch.where(keep, device_act(z, act) * scale, 0.0) + r.double()
+    tol = scale * (1.13 * tz + CURVE * z.abs()) + u * ref.abs() + tiny + 2 * STEP * r.double().abs()
+    device_check(out, ref, tol, "out")
+    # without the worst case's slack: random errors are far smaller than the bound
+    limit = {"f32": 2.0 ** -19, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
+    assert float((pre.double() - z).norm() / z.norm()) <= limit
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(2560, 2304, 1320), (2501, 2311, 1333), (20000, 264, 520),
+                                   (260, 20008, 136)])
+def test_grad_large(dtype, m, n, k):
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+    dt = TYPES[dtype]
+    new = lambda r, c, s: torch.empty((r, c), dtype=dt, device="cuda").normal_(  # noqa: E731
+        0, s, generator=gen)
+    dy, x, w = new(m, n, 0.1), new(m, k, 1), new(n, k, 1 / math.sqrt(k))
+    pre = new(m, n, 1.5)
+    dx, dw, db = kernels.linear_grad(dy, x, w, pre=pre, act="relu")
+    dz = torch.where(pre > 0, dy, 0.0).double()  # exact in every type
+    u, tiny = ROUND[dtype], TINY[dtype]
+    for got, a, b, terms, name in ((dx, dz, w.double(), n, "dx"), (dw, dz.t(), x.double(), m, "dw")):
+        ref = a @ b
+        tol = (terms + 16) * STEP * (a.abs() @ b.abs()) + u * ref.abs() + tiny
+        device_check(got, ref, tol, name)
+        limit = {"f32": 2.0 ** -19, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
+        assert float((got.double() - ref).norm() / ref.norm()) <= limit, name
+    ref = dz.sum(0)
+    device_check(db, ref, (m + 16) * STEP * dz.abs().sum(0) + u * ref.abs() + tiny, "db")
+
+
+def test_offsets_beyond_32_bits():
+    """Outputs of more than 2^32 elements: the last rows are what they are by
+    themselves (the mask goes by the row's number, so dropout is shifted by hand)."""
+    rows, cols = 70000, 66008
+    x = torch.empty((rows, 16), dtype=torch.bfloat16, device="cuda").normal_()
+    w = torch.empty((cols, 16), dtype=torch.bfloat16, device="cuda").normal_()
+    out = kernels.linear(x, w, act="silu")
+    assert out.numel() > 1 << 32
+    for part in (slice(0, 100), slice(rows // 2, rows // 2 + 100), slice(rows - 100, rows)):
+        assert torch.equal(out[part], kernels.linear(x[part], w, act="silu"))
+    drop = kernels.Dropout(0.5, 3, 4)
+    kernels.dropout(out, drop, out=out)
+    tail = kernels.linear(x[-7:], w, act="silu")
+    # the last rows' mask from the definition
+    blocks = cols // 8
+    col, row = np.meshgrid(np.arange(blocks), np.arange(rows - 7, rows))
+    words = philox4x32((col, row, np.full_like(col, 4), np.full_like(col, 0)), (3, 0))
+    r16 = np.stack([h for v in words for h in (v & np.uint64(0xFFFF), v >> np.uint64(16))], axis=2)
+    keep = torch.from_numpy(r16.reshape(7, cols) >= 32768).cuda()
+    assert torch.equal(out[-7:], torch.where(keep, tail * 2, torch.zeros_like(tail)))
