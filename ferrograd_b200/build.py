@@ -121,11 +121,12 @@ def build_layer(verbose: bool = False) -> str:
     src = os.path.join(CSRC, "layer_py.cpp")
     if _stale(mod, [src, os.path.join(ROOT, "include", "ferro_cuda.h")]):
         abi = int(torch.compiled_with_cxx11_abi())
-        cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+        cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+               f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
                *[f"-isystem{p}" for p in include_paths()], "-isystem/usr/local/cuda/include",
                f"-I{sysconfig.get_paths()['include']}", src, "-o", mod, "-L" + HERE,
-               *[f"-L{p}" for p in library_paths()], "-lferro_cuda", "-ltorch_python", "-ltorch_cpu",
-               "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
+               *[f"-L{p}" for p in library_paths()], "-lferro_cuda", "-ltorch_python",
+               "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)

@@ -17,48 +17,21 @@
 namespace fg {
 namespace layer {
 
+using ptx::grid_launch_next;
+using ptx::grid_wait;
+
 // ---------------------------------------------------------------------------
-// C[m, n] = sum_k A(m, k) B(n, k), any strides and sizes (K = 0 included),
-// on the CUDA cores in f32: 64 x 64 tiles, 16-deep steps through shared
-// memory, 2 rows x 8 columns a thread.
+// K = 0: there is nothing to read, every sum is 0 and the epilogue remains.
+// Bound by the output's writes; a thread has eight columns of a row a step.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256)
-    k_linear_tile(const T *__restrict__ a, int64_t ar, int64_t ac, const T *__restrict__ b,
-                  int64_t br, int64_t bc, int K, const Epilogue e) {
-  __shared__ float sa[16][64 + 4], sb[16][64 + 4];
-  const int m0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
-  for (int n0 = blockIdx.y * 64; n0 < e.N; n0 += gridDim.y * 64) {
-    float acc[2][8] = {};
-    for (int k0 = 0; k0 < K; k0 += 16) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-        // neighbouring threads walk the operand's contiguous direction
-        const int ak = ac == 1 ? i & 15 : i >> 6, am = ac == 1 ? i >> 4 : i & 63;
-        const int bk = bc == 1 ? i & 15 : i >> 6, bn = bc == 1 ? i >> 4 : i & 63;
-        sa[ak][am] = m0 + am < e.M && k0 + ak < K
-                         ? to_f32<T>(a[(m0 + am) * ar + (k0 + ak) * ac]) : 0.0f;
-        sb[bk][bn] = n0 + bn < e.N && k0 + bk < K
-                         ? to_f32<T>(b[(n0 + bn) * br + (k0 + bk) * bc]) : 0.0f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 16; k++) {
-        const float a0 = sa[k][ty], a1 = sa[k][ty + 32];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float bj = sb[k][tx * 8 + j];
-          acc[0][j] = fmaf(a0, bj, acc[0][j]);
-          acc[1][j] = fmaf(a1, bj, acc[1][j]);
-        }
-      }
-    }
-    const int col = n0 + tx * 8;
-    if (col < e.N) {
-      if (m0 + ty < e.M) epilogue8<T>(e, m0 + ty, col, acc[0]);
-      if (m0 + ty + 32 < e.M) epilogue8<T>(e, m0 + ty + 32, col, acc[1]);
-    }
+__global__ void __launch_bounds__(256) k_linear_empty(const Epilogue e) {
+  grid_wait();
+  grid_launch_next();
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  for (Walk at(e.M, (e.N + 7) / 8, first, step); at.inside(); at.next()) {
+    float v[8] = {};
+    epilogue8<T>(e, (int)at.row, at.group * 8, v);
   }
 }
 
@@ -69,12 +42,10 @@ __global__ void __launch_bounds__(256)
 // next four steps before it multiplies.  The warp's sums meet by shuffles in a
 // fixed order.  (A tensor-core tile of so few rows first fills and drains
 // accumulators, and joins its k-ranges across CTAs: 1 x 4096 x 4096 bf16, the
-// weight from HBM, 11.6 us against 8.3 us here, 4.0 TB/s.)  VEC: every row starts on a 16-byte boundary;
-// without it elements are read one by one, still in neighbouring lanes.
+// weight from HBM, 11.6 us against 8.3 us here, 4.0 TB/s: 33 MB are too few for
+// the copy rate.)  VEC: every row starts on a 16-byte boundary; without it
+// elements are read one by one, still in neighbouring lanes.
 // ---------------------------------------------------------------------------
-using ptx::grid_launch_next;
-using ptx::grid_wait;
-
 constexpr int kRowsMax = 8;
 
 // For MR rows of x: the weight's rows a warp takes, and the steps it has in
@@ -203,20 +174,30 @@ template <typename T>
 static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaStream_t st) {
   const T *x = static_cast<const T *>(g->x), *w = static_cast<const T *>(g->w);
   auto go = [&](auto kern) {
-    const int per = 8 * RowsShape<T, 1>::rows;
+    const int per = 8 * RowsShape<T, 1>::rows;  // the same for every MR
     const unsigned grid = (unsigned)((g->N + (int64_t)per - 1) / per);
     return launch_early(kern, dim3(grid), 256, st, x, g->x_row, w, g->w_row, g->K, e);
   };
   if (g->M == 1) return vec ? go(k_linear_rows<T, 1, true>) : go(k_linear_rows<T, 1, false>);
   if (g->M == 2) return vec ? go(k_linear_rows<T, 2, true>) : go(k_linear_rows<T, 2, false>);
-  if (g->M <= 4) return vec ? go(k_linear_rows<T, 4, true>) : go(k_linear_rows<T, 4, false>);
-  return vec ? go(k_linear_rows<T, 8, true>) : go(k_linear_rows<T, 8, false>);
+  // 16-bit rows of 16-byte reads end at two, others at four (rows_limit)
+  if constexpr (sizeof(T) == 2) {
+    return go(k_linear_rows<T, 4, false>);
+  } else {
+    if (g->M <= 4) return vec ? go(k_linear_rows<T, 4, true>) : go(k_linear_rows<T, 4, false>);
+    return vec ? go(k_linear_rows<T, 8, true>) : go(k_linear_rows<T, 8, false>);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // dz = D(dy) * act'(pre), and the column sums of dz over this block's rows
 // (f32, one row of `part` a block; k_bias_grad adds them up in order).
 // dz may be null (only the sums are wanted).
+// It reads dy and pre once and writes dz once: 1.6 GB at 16384 x 16384 bf16, GELU,
+// 246 us at the copy rate, measured 391 us: with the slope's exponential and the
+// conversions 36 instructions an element, the issue slots bound it, not HBM.  A
+// thread keeps its eight columns down the rows, so the column sums need no
+// exchange until the end, and asks for the next rows before it computes.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void store_dz(void *dz, int64_t at, int64_t, const float (&v)[8]) {
@@ -308,6 +289,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
   }
 }
 
+// db = the blocks' sums, a thread a column, in the order of the rows.  At most 128
+// a column (dz_shape): 8 MB at 16384 columns, a few microseconds.
 template <typename T>
 __global__ void __launch_bounds__(256)
     k_bias_grad(const float *__restrict__ part, int chunks, int N, T *__restrict__ db) {
@@ -322,7 +305,10 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------
-// out = residual + D(x): eight columns of a row a step.
+// out = residual + D(x): eight columns of a row a step, one Philox call for them.
+// Bound by HBM, with the issue slots close behind: 16384 x 16384 bf16 with a
+// residual in 271 us, 5.9 TB/s or 0.91 of a copy's rate (an addition of the two
+// arrays alone takes 236 us).  A thread asks for all its groups before it draws.
 // ---------------------------------------------------------------------------
 // Groups of eight columns a thread takes, 256 groups apart.
 template <typename T>
@@ -446,27 +432,12 @@ static bool overlap(const void *w, int64_t rows, int64_t cols, int64_t ld, const
   return true;
 }
 
-template <typename T>
-static int run_tile(const Mat &a, const Mat &b, int K, const Epilogue &e, cudaStream_t st) {
-  const unsigned gx = (unsigned)((e.M + 63LL) / 64), ny = (unsigned)((e.N + 63LL) / 64);
-  k_linear_tile<T><<<dim3(gx, ny < 65535 ? ny : 65535), 256, 0, st>>>(
-      static_cast<const T *>(a.ptr), a.row, a.col, static_cast<const T *>(b.ptr), b.row, b.col, K,
-      e);
-  FG_LAUNCH_TRY();
-  return FG_OK;
-}
-
-// A K of 0 has nothing to load: the tile kernel's sums are 0.
 static int run_empty_product(int dtype, const Epilogue &e, cudaStream_t st) {
-  const Mat none{};
-  switch (dtype) {
-    case FG_F32:
-      return run_tile<float>(none, none, 0, e, st);
-    case FG_BF16:
-      return run_tile<__nv_bfloat16>(none, none, 0, e, st);
-    default:
-      return run_tile<__half>(none, none, 0, e, st);
-  }
+  const int64_t blocks = ((int64_t)e.M * ((e.N + 7LL) / 8) + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+  if (dtype == FG_F32) return launch_early(k_linear_empty<float>, grid, 256, st, e);
+  if (dtype == FG_BF16) return launch_early(k_linear_empty<__nv_bfloat16>, grid, 256, st, e);
+  return launch_early(k_linear_empty<__half>, grid, 256, st, e);
 }
 
 static int check_common(const char *who, int dtype, int M, int N, int K, int act) {

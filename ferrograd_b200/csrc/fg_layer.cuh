@@ -93,7 +93,8 @@ struct Raw8 {
   uint4 q[sizeof(T) / 2];
   __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) q[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    for (int i = 0; i < (int)sizeof(T) / 2; i++)
+      q[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll

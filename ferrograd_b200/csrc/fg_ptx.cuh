@@ -270,7 +270,8 @@ __device__ __forceinline__ void mma_f16_steps(uint32_t on, uint32_t d_tmem, uint
                                               uint64_t bdesc, uint32_t idesc,
                                               uint32_t accumulate) {
   static_assert(STEPS == 2 || STEPS == 4, "two or four steps");
-#define FG_MMA(cg, a, b, p) "@q tcgen05.mma.cta_group::" cg ".kind::f16 [%0], " a ", " b ", %3, " p ";\n\t"
+#define FG_MMA(cg, a, b, p) \
+  "@q tcgen05.mma.cta_group::" cg ".kind::f16 [%0], " a ", " b ", %3, " p ";\n\t"
 #define FG_MMA_STEPS(cg)                                                                          \
   asm volatile(                                                                                   \
       "{\n\t.reg .pred p, q, e, t;\n\t.reg .b64 a, b;\n\t"                                        \
@@ -369,7 +370,8 @@ __device__ __forceinline__ void cluster_wait() {
 __device__ __forceinline__ void bulk_copy_to_cta(uint32_t dst_cluster, uint32_t src, uint32_t bytes,
                                                  uint32_t bar_cluster) {
   asm volatile(
-      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes "
+      "[%0], [%1], %2, [%3];" ::
           "r"(dst_cluster),
       "r"(src), "r"(bytes), "r"(bar_cluster)
       : "memory");

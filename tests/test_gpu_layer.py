@@ -622,3 +622,23 @@ def test_offsets_beyond_32_bits():
     r16 = np.stack([h for v in words for h in (v & np.uint64(0xFFFF), v >> np.uint64(16))], axis=2)
     keep = torch.from_numpy(r16.reshape(7, cols) >= 32768).cuda()
     assert torch.equal(out[-7:], torch.where(keep, tail * 2, torch.zeros_like(tail)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(2, 264, 320), (40, 264, 320), (2560, 2304, 320)])
+def test_repeated_and_overlapping_rows(dtype, m, n, k):
+    """A residual expanded over the rows and an x whose rows overlap (stride 8)
+    give what their copies give."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    new = lambda *s: torch.empty(s, dtype=TYPES[dtype], device="cuda").normal_(  # noqa: E731
+        generator=gen)
+    w, r = new(n, k), new(1, n).expand(m, n)
+    x = new(8 * m + k).as_strided((m, k), (8, 1))
+    drop = kernels.Dropout(0.3, 1, 2)
+    got = kernels.linear(x, w, act="relu", residual=r, drop=drop)
+    want = kernels.linear(x.contiguous(), w, act="relu", residual=r.contiguous(), drop=drop)
+    assert torch.equal(got, want)
+    dy, base = new(m, n), new(1, k).expand(m, k)
+    got = kernels.linear_grad(dy, x, w, dx_residual=base)
+    want = kernels.linear_grad(dy, x.contiguous(), w, dx_residual=base.contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
