@@ -632,12 +632,6 @@ void place_operand(Operand *o, void *ws);
 void place_jobs(StageJobs *jobs, void *ws);
 int run_stage(int dtype, const StageJobs &jobs, cudaStream_t st);
 
-// How the tensor-core kernel cuts a product up (fg_layer_gemm.cu).
-struct Form {
-  bool pair;
-  int bm, bn, split;
-};
-Form pick_form(int M, int N, int K, int planes, int sms);
 // A product of rows and columns e.M, e.N over K with its epilogue.
 struct Product {
   Operand a, b;

@@ -42,6 +42,7 @@
 
 #include "fg_internal.h"
 #include "fg_layer.cuh"
+#include "fg_layer_plan.h"
 #include "fg_ptx.cuh"
 
 namespace fg {
@@ -52,11 +53,6 @@ using namespace fg::ptx;
 using True = std::true_type;
 using False = std::false_type;
 
-constexpr int kMaxStages = 16;
-// k-blocks of a chain of 16-bit products: 16384 deep, 1024 truncated additions
-// of 2^-24 of the sum each at most.  Outputs of 8 or 11 bits do not show that
-// (f16 rounds by up to 2^-11).
-constexpr int kChain16 = 256;
 constexpr unsigned kErrLayer = 5u << 16;  // device error word: role 5
 
 // How an operand's tile lies in shared memory.  K-major: rows of BK elements
@@ -103,9 +99,8 @@ __device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int grou
   nb = r / gm;
 }
 
-constexpr int kBlockCols = 32;                 // IO: a warp's block
-constexpr int kSlabCols = 16, kSlabPitch = 20;  // floats; a warp's 32 x 16 slab (pair)
-constexpr int kSplitSlab = 384;                 // floats; 8 x 36, 16 x 20 or 32 x 12 (split)
+constexpr int kBlockCols = 32;  // IO: a warp's block
+constexpr int kSlabCols = 16;   // a warp's 32 x 16 slab (pair)
 
 // The block of each form.  RUN: the epilogue warps keep the running sums of the
 // chains in registers; without it a product is one chain and they read the
@@ -114,9 +109,9 @@ constexpr int kSplitSlab = 384;                 // floats; 8 x 36, 16 x 20 or 32
 // six left waiting on its latencies (5200 cycles for a plain 128 x 64 tile).
 template <int CG, bool RUN>
 struct Block {
-  static constexpr int first_epi = CG == 2 ? 4 : 2;
-  static constexpr int epi_warps = CG == 1 ? 4 : RUN ? 8 : 16;
-  static constexpr int warps = CG == 1 ? 12 : first_epi + epi_warps;
+  static constexpr int first_epi = block_first_epi(CG);
+  static constexpr int epi_warps = block_epi_warps(CG, RUN);
+  static constexpr int warps = block_warps(CG, RUN);
   static constexpr int threads = 32 * warps;
 };
 
@@ -855,57 +850,26 @@ static int make_io_map(CUtensorMap *map, const void *ptr, int M, int N, int64_t 
   return FG_OK;
 }
 
-// Shared memory a CTA must ask for so that the CTAs that fit on an SM never
-// need more than its 512 TMEM columns between them: an allocation that had to
-// wait while its cluster's other CTAs hold theirs could wait for ever.
-static size_t tmem_share(int cols) { return (size_t)cols / 128 * 47 * 1024; }
-
-// Lays out a product's shared memory (its stages and what follows the ring);
-// returns the bytes.
-template <int PLANES, int CG, int BN, bool RUN, bool IO>
-static size_t lay_out(ProductArgs &g, const Epilogue &e, size_t ring_cap) {
-  constexpr int BK = Depth<PLANES>::BK;
-  const size_t stage = (size_t)PLANES * (g.a.rows + g.b.rows) * BK * 2;
-  // past the ring: the pair's blocks or slabs, or what an MMA of 128 rows reads
-  // beyond an A tile of fewer (it lands in unused accumulator rows)
-  const size_t tail = CG == 2 ? Block<CG, RUN>::epi_warps * (IO ? 4096 : 32 * kSlabPitch * 4)
-                              : 128 * BK * 2;
-  int64_t stages = (int64_t)(ring_cap / stage);
-  if (stages > kMaxStages) stages = kMaxStages;
-  if (CG == 1) {
-    const int64_t per = (g.nk + g.split - 1) / g.split;
-    if (stages > per) stages = per;
-  }
-  const int64_t least = PLANES == 3 ? 2 : 1;  // an f32 chain holds two k-blocks at once
-  if (stages < least) stages = least;
-  g.stages = (int)stages;
-  size_t bytes = stages * stage + tail;
-  if (CG == 1) {
-    const size_t sums = (size_t)((g.M < 128 ? g.M + 7 : 128) & ~7) * BN * 4;
-    if (bytes < sums) bytes = sums;
-    g.join_at = (int)((bytes + 127) & ~(size_t)127);
-    if (g.split > 1) bytes = g.join_at + sums;
-    g.slab_at = (int)((bytes + 127) & ~(size_t)127);
-    if (!e.vec) bytes = g.slab_at + Block<CG, RUN>::warps * kSplitSlab * 4;
-  }
-  bytes += 2048;  // barriers, alignment
-  return bytes < tmem_share(2 * BN) ? tmem_share(2 * BN) : bytes;
-}
-
 template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO, bool TWO>
 static int launch(Problems<TWO> &ps, int ctas, size_t ring_cap, cudaStream_t st) {
   auto kern = k_layer_product<T, PLANES, CG, BN, RUN, IO, TWO>;
   size_t bytes = 0;
   for (Problem &pr : ps.at) {
-    const size_t b = lay_out<PLANES, CG, BN, RUN, IO>(pr.g, pr.e, ring_cap);
-    if (bytes < b) bytes = b;
+    ProductArgs &g = pr.g;
+    const SharedPlan p = lay_out({PLANES, CG, BN, RUN, IO, g.M, g.a.rows, g.b.rows, g.nk, g.split,
+                                  pr.e.vec != 0},
+                                 ring_cap);
+    g.stages = p.stages;
+    g.join_at = p.join_at;
+    g.slab_at = p.slab_at;
+    if (bytes < p.bytes) bytes = p.bytes;
   }
   static bool attr_done[64] = {};
   int dev = 0;
   FG_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
     FG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     227 * 1024));
+                                     (int)kSharedMax));
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -929,13 +893,6 @@ static int launch(Problems<TWO> &ps, int ctas, size_t ring_cap, cudaStream_t st)
 
 static int64_t tiles_of(const Epilogue &e, int bm, int bn) {
   return (e.M + (int64_t)bm - 1) / bm * ((e.N + (int64_t)bn - 1) / bn);
-}
-
-// Shared memory of a split CTA's ring: with more CTAs than SMs two fit an SM, so
-// that one computes while the other joins; less the joined sums.
-static size_t split_ring(int64_t ctas, int sms, int M, int bn, int split) {
-  const size_t cap = (ctas > sms ? 92 : 190) * 1024;
-  return split > 1 ? cap - (size_t)(M < 128 ? M : 128) * bn * 4 : cap;
 }
 
 template <typename T, int PLANES>
@@ -1058,44 +1015,6 @@ int run_tensor_products(int dtype, const Product &x, const Product &y, cudaStrea
     default:
       return run_two<__half, 1>(ps, tiles * split, sms, st);
   }
-}
-
-// The form with the least estimated time, in microseconds.  Fitted on one B200
-// to every form of 17 shapes from 24 x 64 x 2048 to 2048 x 2048 x 2048 in 16 bits
-// and f32: an MMA step (16 deep) costs a pair 0.07 and a lone CTA 0.038 at either
-// width; around them a pair spends 6.8, a lone CTA 1.8 and for 128 rows another
-// 1.9 (64 wide) or 3.4; joining a cluster's sums costs 0.7 and for 128 rows
-// another 1.1 or 3.1.  64-wide CTAs run two to an SM and hide each other's fixed
-// part.  It picks the fastest form or one within 10% of it on all 17 (24 x 8192 x
-// 2048 f16: 64 wide, k over 8 CTAs, 10.2 against 22.7 unsplit and 42.4 by pairs;
-// 1024 x 4096 x 4096 bf16: pairs, 27.6 against 35.1 and 48.3).
-Form pick_form(int M, int N, int K, int planes, int sms) {
-  const double steps = K / 16.0 * (planes == 3 ? 6.0 : 1.0);
-  Form best{true, 256, 256, 1};
-  const double pairs = ceil(M / 256.0) * ceil(N / 256.0);
-  double cost = ceil(pairs / (sms / 2)) * steps * 0.07 + 6.8;
-  const int bk = planes == 3 ? 32 : 64;
-  const int nk = (int)((K + (int64_t)bk - 1) / bk);
-  const double rows = M < 128 ? M / 128.0 : 1.0;
-  for (int bn = 64; bn <= 128; bn *= 2)
-    // (128-wide CTAs take one chain of 16-bit products, and run one to an SM, so
-    // that not enough clusters of 8 fit)
-    for (int split = 1; split <= (bn == 64 ? 8 : 4) && split <= nk; split *= 2) {
-      if (bn == 128 && (planes == 3 || nk > (int64_t)kChain16 * split)) continue;
-      const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
-      if (ctas > 1e8) continue;
-      const double fixed = 1.8 + rows * (bn == 64 ? 1.9 : 3.4);
-      const double join = split > 1 ? 0.7 + rows * (bn == 64 ? 1.1 : 3.1) : 0.0;
-      const double per_sm =
-          split > 1 || bn == 128 ? ceil(ctas / sms) : ctas > sms ? ctas / sms : 1.0;
-      const double turns = bn == 64 ? ceil(ctas / (2.0 * sms)) : per_sm;
-      const double c = 1.5 + join + turns * fixed + per_sm * steps / split * 0.038;
-      if (c < cost) {
-        cost = c;
-        best = Form{false, 128, bn, split};
-      }
-    }
-  return best;
 }
 
 }  // namespace layer

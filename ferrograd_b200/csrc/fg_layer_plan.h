@@ -1,0 +1,137 @@
+// How a product of the layer's tensor-core kernel is cut up and laid out in
+// shared memory (host code without CUDA, so that it can be swept over every
+// shape on the CPU).
+#pragma once
+#include <math.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace fg {
+namespace layer {
+
+constexpr int kMaxStages = 16;
+// k-blocks of a chain of 16-bit products: 16384 deep, 1024 truncated additions
+// of 2^-24 of the sum each at most.  Outputs of 8 or 11 bits do not show that
+// (f16 rounds by up to 2^-11).
+constexpr int kChain16 = 256;
+constexpr size_t kSharedMax = 227 * 1024;  // what a CTA may ask for
+
+constexpr int kSlabPitch = 20;   // floats; of a warp's 32 x 16 slab (pair)
+constexpr int kSplitSlab = 384;  // floats; 8 x 36, 16 x 20 or 32 x 12 (split)
+
+// Warps of a block (Block in fg_layer_gemm.cu).
+constexpr int block_first_epi(int cg) { return cg == 2 ? 4 : 2; }
+constexpr int block_epi_warps(int cg, bool run) { return cg == 1 ? 4 : run ? 8 : 16; }
+constexpr int block_warps(int cg, bool run) {
+  return cg == 1 ? 12 : block_first_epi(cg) + block_epi_warps(cg, run);
+}
+
+struct Form {
+  bool pair;
+  int bm, bn, split;
+};
+
+// Shared memory a CTA must ask for so that the CTAs that fit on an SM never
+// need more than its 512 TMEM columns between them: an allocation that had to
+// wait while its cluster's other CTAs hold theirs could wait for ever.
+inline size_t tmem_share(int cols) { return (size_t)cols / 128 * 47 * 1024; }
+
+// Shared memory of a split CTA's ring: with more CTAs than SMs two fit an SM, so
+// that one computes while the other joins; less the joined sums.
+inline size_t split_ring(int64_t ctas, int sms, int M, int bn, int split) {
+  const size_t cap = (ctas > sms ? 92 : 190) * 1024;
+  return split > 1 ? cap - (size_t)(M < 128 ? M : 128) * bn * 4 : cap;
+}
+
+// What a launch's shared memory depends on (vec: the outputs' rows start on
+// 16-byte boundaries, so that the split form needs no slabs).
+struct SharedShape {
+  int planes, cg, bn;
+  bool run, io;
+  int M, a_rows, b_rows, nk, split;
+  bool vec;
+};
+struct SharedPlan {
+  int stages;
+  int join_at, slab_at;  // split: offsets from the ring
+  size_t bytes;
+};
+
+// Lays out a product's shared memory: its stages, as many as ring_cap holds
+// and the rest leaves room for, and what follows the ring.
+inline SharedPlan lay_out(const SharedShape &s, size_t ring_cap) {
+  const int bk = s.planes == 3 ? 32 : 64;
+  const size_t stage = (size_t)s.planes * (s.a_rows + s.b_rows) * bk * 2;
+  // past the ring: the pair's blocks or slabs, or what an MMA of 128 rows reads
+  // beyond an A tile of fewer (it lands in unused accumulator rows)
+  const size_t tail =
+      s.cg == 2 ? (size_t)block_epi_warps(s.cg, s.run) * (s.io ? 4096 : 32 * kSlabPitch * 4)
+                : (size_t)128 * bk * 2;
+  int64_t stages = (int64_t)(ring_cap / stage);
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (s.cg == 1) {
+    const int64_t per = ((int64_t)s.nk + s.split - 1) / s.split;
+    if (stages > per) stages = per;
+  }
+  const int64_t least = s.planes == 3 ? 2 : 1;  // an f32 chain holds two k-blocks at once
+  if (stages < least) stages = least;
+  SharedPlan p{};
+  for (;; stages--) {
+    size_t bytes = stages * stage + tail;
+    if (s.cg == 1) {
+      const size_t sums = (size_t)((s.M < 128 ? s.M + 7 : 128) & ~7) * s.bn * 4;
+      if (bytes < sums) bytes = sums;
+      p.join_at = (int)((bytes + 127) & ~(size_t)127);
+      if (s.split > 1) bytes = p.join_at + sums;
+      p.slab_at = (int)((bytes + 127) & ~(size_t)127);
+      if (!s.vec) bytes = p.slab_at + (size_t)block_warps(s.cg, s.run) * kSplitSlab * 4;
+    }
+    p.stages = (int)stages;
+    p.bytes = bytes + 2048;  // barriers, alignment
+    if (p.bytes <= kSharedMax || stages == least) break;
+  }
+  const size_t share = tmem_share(2 * s.bn);
+  if (p.bytes < share) p.bytes = share;
+  return p;
+}
+
+// The form with the least estimated time, in microseconds.  Fitted on one B200
+// to every form of 17 shapes from 24 x 64 x 2048 to 2048 x 2048 x 2048 in 16 bits
+// and f32: an MMA step (16 deep) costs a pair 0.07 and a lone CTA 0.038 at either
+// width; around them a pair spends 6.8, a lone CTA 1.8 and for 128 rows another
+// 1.9 (64 wide) or 3.4; joining a cluster's sums costs 0.7 and for 128 rows
+// another 1.1 or 3.1.  64-wide CTAs run two to an SM and hide each other's fixed
+// part.  It picks the fastest form or one within 10% of it on all 17 (24 x 8192 x
+// 2048 f16: 64 wide, k over 8 CTAs, 10.2 against 22.7 unsplit and 42.4 by pairs;
+// 1024 x 4096 x 4096 bf16: pairs, 27.6 against 35.1 and 48.3).
+inline Form pick_form(int M, int N, int K, int planes, int sms) {
+  const double steps = K / 16.0 * (planes == 3 ? 6.0 : 1.0);
+  Form best{true, 256, 256, 1};
+  const double pairs = ceil(M / 256.0) * ceil(N / 256.0);
+  double cost = ceil(pairs / (sms / 2)) * steps * 0.07 + 6.8;
+  const int bk = planes == 3 ? 32 : 64;
+  const int nk = (int)((K + (int64_t)bk - 1) / bk);
+  const double rows = M < 128 ? M / 128.0 : 1.0;
+  for (int bn = 64; bn <= 128; bn *= 2)
+    // (128-wide CTAs take one chain of 16-bit products, and run one to an SM, so
+    // that not enough clusters of 8 fit)
+    for (int split = 1; split <= (bn == 64 ? 8 : 4) && split <= nk; split *= 2) {
+      if (bn == 128 && (planes == 3 || nk > (int64_t)kChain16 * split)) continue;
+      const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
+      if (ctas > 1e8) continue;
+      const double fixed = 1.8 + rows * (bn == 64 ? 1.9 : 3.4);
+      const double join = split > 1 ? 0.7 + rows * (bn == 64 ? 1.1 : 3.1) : 0.0;
+      const double per_sm =
+          split > 1 || bn == 128 ? ceil(ctas / sms) : ctas > sms ? ctas / sms : 1.0;
+      const double turns = bn == 64 ? ceil(ctas / (2.0 * sms)) : per_sm;
+      const double c = 1.5 + join + turns * fixed + per_sm * steps / split * 0.038;
+      if (c < cost) {
+        cost = c;
+        best = Form{false, 128, bn, split};
+      }
+    }
+  return best;
+}
+
+}  // namespace layer
+}  // namespace fg
