@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <string>
 
 #include "../../include/ferro_cuda.h"
@@ -121,26 +122,53 @@ at::Tensor empty(const at::Tensor &x, at::IntArrayRef shape) {
   return at::empty(shape, x.options().memory_format(at::MemoryFormat::Contiguous));
 }
 
-// Runs a C-ABI call with the workspace it asks for, on x's device and on the
-// given stream (None: torch's current one).
+// The stream of a call: torch's current one, or the one given.  On another
+// stream than the current one the call's memory has to be that stream's own:
+// the allocator hands out blocks whose last use is over in the order of the
+// stream they are allocated for, and of no other.  So everything is allocated
+// with that stream current; arguments are kept from reuse until it is done with
+// them, and results until the caller's stream is.
+class Launch {
+ public:
+  cudaStream_t st;
+
+  Launch(const at::Tensor &x, PyObject *stream)
+      : device_(x.device()), caller_(c10::cuda::getCurrentCUDAStream(x.device().index())) {
+    st = caller_.stream();
+    if (stream == Py_None) return;
+    cudaStream_t given = (cudaStream_t)word(stream);
+    if (given == cudaStreamLegacy) given = nullptr;  // the same stream by its other name
+    if (given == st) return;
+    st = given;
+    guard_.reset_stream(c10::cuda::getStreamFromExternal(st, x.device().index()));
+  }
+  void uses(const at::Tensor &t) {
+    if (guard_.current_stream().has_value())
+      t.record_stream(guard_.current_stream().value().unwrap());
+  }
+  void gives(const at::Tensor &t) {
+    if (guard_.current_stream().has_value() && t.defined()) t.record_stream(caller_.unwrap());
+  }
+
+ private:
+  c10::cuda::CUDAGuard device_;
+  c10::cuda::CUDAStream caller_;
+  c10::cuda::OptionalCUDAStreamGuard guard_;
+};
+
+// Runs a C-ABI call with the workspace it asks for.
 template <typename Args>
-void run(const at::Tensor &x, PyObject *stream, Args &a, int (*ask)(const Args *, size_t *),
+void run(const at::Tensor &x, const Launch &on, Args &a, int (*ask)(const Args *, size_t *),
          int (*call)(const Args *, void *)) {
   size_t need = 0;
   check(ask(&a, &need));
-  const bool current = stream == Py_None;
-  const auto index = x.device().index();
-  cudaStream_t st =
-      current ? c10::cuda::getCurrentCUDAStream(index).stream() : (cudaStream_t)word(stream);
   at::Tensor ws;
   if (need) {
     ws = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
-    // the allocator must not hand it out before that stream is done
-    if (!current) ws.record_stream(c10::cuda::getStreamFromExternal(st, index).unwrap());
     a.workspace = ws.data_ptr();
     a.workspace_bytes = need;
   }
-  check(call(&a, st));
+  check(call(&a, on.st));
 }
 
 void set_drop(fg_dropout_spec &d, PyObject *p, PyObject *seed, PyObject *offset) {
@@ -164,7 +192,8 @@ PyObject *linear(PyObject *const *o) {
   const at::Tensor &x = tensor(o[0], "x"), &w = tensor(o[1], "w");
   const Like like(x);
   const Product s = product(like, x, w);
-  c10::cuda::CUDAGuard guard(x.device());
+  Launch on(x, o[10]);
+  on.uses(x), on.uses(w);
   fg_linear_args a{};
   a.dtype = like.code;
   a.M = extent(s.M), a.N = extent(s.N), a.K = extent(s.K);
@@ -173,12 +202,14 @@ PyObject *linear(PyObject *const *o) {
   if (o[2] != Py_None) {
     const at::Tensor &bias = tensor(o[2], "bias");
     like.check("bias", bias, {s.N}, true);
+    on.uses(bias);
     a.bias = bias.data_ptr();
   }
   a.act = integer(o[3]);
   if (o[4] != Py_None) {
     const at::Tensor &r = tensor(o[4], "residual");
     like.check("residual", r, {s.M, s.N}, true);
+    on.uses(r);
     a.residual = r.data_ptr(), a.ld_residual = pitch(r);
   }
   set_drop(a.drop, o[5], o[6], o[7]);
@@ -186,16 +217,19 @@ PyObject *linear(PyObject *const *o) {
   at::Tensor out, pre;
   if (o[9] == Py_None) {
     out = empty(x, {s.M, s.N});
+    on.gives(out);
   } else {
     out = tensor(o[9], "out");
     like.check("out", out, {s.M, s.N}, true);
+    on.uses(out);
   }
   a.out = out.data_ptr(), a.ld_out = pitch(out);
   if (save_pre) {
     pre = empty(x, {s.M, s.N});
+    on.gives(pre);
     a.pre = pre.data_ptr(), a.ld_pre = s.N;
   }
-  run(x, o[10], a, fg_linear_workspace, fg_linear);
+  run(x, on, a, fg_linear_workspace, fg_linear);
   PyObject *result = o[9] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(o[9]);
   if (!save_pre) return result;
   return Py_BuildValue("(NN)", result, THPVariable_Wrap(pre));
@@ -208,7 +242,8 @@ PyObject *linear_grad(PyObject *const *o) {
   const Like like(x);
   const Product s = product(like, x, w);
   like.check("dy", dy, {s.M, s.N}, false);
-  c10::cuda::CUDAGuard guard(x.device());
+  Launch on(x, o[12]);
+  on.uses(dy), on.uses(x), on.uses(w);
   fg_linear_grad_args a{};
   a.dtype = like.code;
   a.M = extent(s.M), a.N = extent(s.N), a.K = extent(s.K);
@@ -219,6 +254,7 @@ PyObject *linear_grad(PyObject *const *o) {
   if (a.act != FG_ACT_NONE) {
     const at::Tensor &pre = tensor(o[3], "pre");
     like.check("pre", pre, {s.M, s.N}, true);
+    on.uses(pre);
     a.pre = pre.data_ptr(), a.ld_pre = pitch(pre);
   }
   set_drop(a.drop, o[5], o[6], o[7]);
@@ -229,6 +265,7 @@ PyObject *linear_grad(PyObject *const *o) {
     if (o[11] != Py_None) {
       const at::Tensor &r = tensor(o[11], "dx_residual");
       like.check("dx_residual", r, {s.M, s.K}, true);
+      on.uses(r);
       a.dx_residual = r.data_ptr(), a.ld_dx_residual = pitch(r);
     }
   } else if (o[11] != Py_None) {
@@ -242,7 +279,8 @@ PyObject *linear_grad(PyObject *const *o) {
     db = empty(x, {s.N});
     a.db = db.data_ptr();
   }
-  run(x, o[12], a, fg_linear_grad_workspace, fg_linear_grad);
+  on.gives(dx), on.gives(dw), on.gives(db);
+  run(x, on, a, fg_linear_grad_workspace, fg_linear_grad);
   // an undefined tensor wraps as None
   return Py_BuildValue("(NNN)", THPVariable_Wrap(dx), THPVariable_Wrap(dw), THPVariable_Wrap(db));
 }
@@ -251,7 +289,8 @@ PyObject *linear_grad(PyObject *const *o) {
 PyObject *dropout(PyObject *const *o) {
   const at::Tensor &x = tensor(o[0], "x");
   const Like like(x);
-  c10::cuda::CUDAGuard guard(x.device());
+  Launch on(x, o[6]);
+  on.uses(x);
   const auto shape = x.sizes();
   const bool flat = shape.size() != 2;  // rows are then a contiguous tensor's
   const int64_t cols = shape.empty() ? 1 : shape.back();
@@ -268,15 +307,15 @@ PyObject *dropout(PyObject *const *o) {
   if (o[1] != Py_None) {
     r = tensor(o[1], "residual");
     ldr = rows_of("residual", r);
+    on.uses(r);
   }
   fg_dropout_spec drop{};
   set_drop(drop, o[2], o[3], o[4]);
   out = o[5] == Py_None ? empty(x, shape) : tensor(o[5], "out");
   const int64_t ldo = rows_of("out", out);
-  void *st = o[6] == Py_None ? (void *)c10::cuda::getCurrentCUDAStream(x.device().index()).stream()
-                             : (void *)word(o[6]);
+  o[5] == Py_None ? on.gives(out) : on.uses(out);
   check(fg_dropout(like.code, (size_t)rows, (size_t)cols, x.data_ptr(), ldx,
-                   r.defined() ? r.data_ptr() : nullptr, ldr, out.data_ptr(), ldo, &drop, st));
+                   r.defined() ? r.data_ptr() : nullptr, ldr, out.data_ptr(), ldo, &drop, on.st));
   return o[5] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(o[5]);
 }
 

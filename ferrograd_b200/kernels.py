@@ -168,6 +168,12 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     [M, N].  ``act`` is one of ``ACTIVATIONS``.  With ``save_pre`` returns
     ``(out, pre)``, ``pre`` being the pre-activations ``linear_grad`` needs
     for an activation.  ``out`` may be the residual.
+
+    ``stream`` is a ``cudaStream_t`` as an integer (None: torch's current
+    stream).  On another stream than the current one the call allocates its
+    results and workspace there; what comes before and after it on other
+    streams is for the caller to order (wait for an event), as in torch.  The
+    same goes for ``linear_grad`` and ``dropout``.
     """
     p, seed, offset = _NO_DROP if drop is None else drop
     return _layer().linear(x, w, bias, _act_code(act), residual, p, seed, offset, save_pre, out,
