@@ -102,7 +102,7 @@ __device__ __forceinline__ void unraw(const R &r, float (&v)[1]) {
 
 template <typename T, int MR, bool VEC>
 __global__ void __launch_bounds__(256)
-    k_linear_rows(const T *__restrict__ x, int64_t xr, const T *__restrict__ w, int64_t wr, int K,
+    k_linear_rows(const T *x, int64_t xr, const T *w, int64_t wr, int K,
                   const Epilogue e) {
   constexpr int V = VEC ? 16 / sizeof(T) : 1;  // elements a lane reads at once
   constexpr int R = RowsShape<T, MR>::rows, U = RowsShape<T, MR>::steps;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256)
   for (int c = 0; c < R; c++) wp[c] = w + min(n0 + c, e.N - 1) * wr;
   float acc[MR][R] = {};
   using Raw = typename RawOf<T, VEC>::type;
-  auto read = [](const T *p) { return __ldg(reinterpret_cast<const Raw *>(p)); };
+  auto read = [](const T *p) { return *reinterpret_cast<const Raw *>(p); };
   auto step = [&](int64_t k, const Raw(&rw)[R]) {
     float b[R][V];
 #pragma unroll
@@ -218,9 +218,9 @@ __device__ __forceinline__ void store_dz<float>(void *dz, int64_t at, int64_t pl
 // itself.
 template <typename T, int TX>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
-    k_layer_dz(const T *__restrict__ dy, int64_t yr, int64_t yc, const T *__restrict__ pre,
-               int64_t ldp, int act, const DropParams drop, void *__restrict__ dz, int64_t ldz,
-               float *__restrict__ part, T *__restrict__ db, int M, int N, int rows, int vec) {
+    k_layer_dz(const T *dy, int64_t yr, int64_t yc, const T *pre,
+               int64_t ldp, int act, const DropParams drop, void *dz, int64_t ldz,
+               float *part, T *db, int M, int N, int rows, int vec) {
   constexpr int TY = 256 / TX;
   __shared__ float red[TY][TX * 8];
   constexpr int U = 2;  // rows in flight, and as many again asked for
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 // columns of 128, beside products of a millisecond.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    k_bias_grad(const float *__restrict__ part, int chunks, int N, T *__restrict__ db) {
+    k_bias_grad(const float *part, int chunks, int N, T *db) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   grid_wait();
   grid_launch_next();

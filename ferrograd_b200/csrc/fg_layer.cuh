@@ -579,7 +579,10 @@ struct Walk {
 };
 
 // Launches a kernel whose blocks begin with grid_wait() (fg_ptx.cuh), so that
-// it may start while the stream's previous kernel ends.
+// it may start while the stream's previous kernel ends.  Its inputs may then
+// still be written while it runs, so none of it reads through the path for data
+// that is constant over a kernel's life (no __ldg, no __restrict__: such loads
+// may also be moved above the wait).
 template <typename... P, typename... A>
 int launch_early(void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
