@@ -644,14 +644,32 @@ struct Product {
 int run_tensor_product(int dtype, const Product &x, cudaStream_t st);
 int run_tensor_products(int dtype, const Product &x, const Product &y, cudaStream_t st);
 
-// An f32 value as the sum of three bf16 values, each rest exact (an infinity
-// is its own first part; a value that would round up to infinity is cut).
+// An f32 value as the sum of three bf16 values, each rest exact, such that the six
+// products of two values' parts add up to what f32 arithmetic gives beyond its
+// range too:
+//  * An infinity is (+-1, 0, +-inf).  Against a finite value only its last part
+//    meets the other's first, so the sum is +-inf, or NaN for 0; against another
+//    infinity 1 meets inf twice.  (inf in front would meet rests of either sign:
+//    inf - inf.)
+//  * From 4 upwards the parts are cut, not rounded, and so have the value's sign.
+//    Below, a part may be rounded up and leave a rest of the other sign, 2^-7 at
+//    most: the 64 products of a chain with such rests stay below 2^127.  (With
+//    every part rounded, 1e21 * 1e21 came out as -inf.)
+// What six products leave out of one is at most 2^-24 of it, and 2^-21 where both
+// values are cut.  Below 2^-110 the rests run out of bf16's exponents: the last
+// bits are lost.
 __device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
-  a = __bfloat162float(__float2bfloat16_rn(v));
-  if (isinf(a) && !isinf(v)) a = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-  const float r = isinf(v) ? 0.0f : v - a;
-  b = __bfloat162float(__float2bfloat16_rn(r));
+  const uint32_t top = 0xffff0000u;
+  const bool cut = fabsf(v) >= 4.0f;
+  a = cut ? __uint_as_float(__float_as_uint(v) & top) : __bfloat162float(__float2bfloat16_rn(v));
+  const float r = v - a;
+  b = cut ? __uint_as_float(__float_as_uint(r) & top) : __bfloat162float(__float2bfloat16_rn(r));
   c = r - b;
+  if (!isfinite(v)) {
+    a = isinf(v) ? copysignf(1.0f, v) : v;
+    b = 0.0f;
+    c = isinf(v) ? v : 0.0f;
+  }
 }
 
 }  // namespace layer

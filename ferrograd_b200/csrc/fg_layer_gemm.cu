@@ -7,7 +7,7 @@
 // an aligned layout (k_stage).  f32 operands are split into three bf16 planes,
 // x = x0 + x1 + x2 with each rest exact, and a product runs as the six bf16
 // products whose size is at least 2^-16 of the largest; what is dropped is
-// below 2^-24 of a product.
+// 2^-24 of a product at most, or 2^-21 of one of large values (split3).
 //
 // The tensor cores truncate each addition to their f32 accumulator, so a long
 // chain drifts towards 0.  A chain is therefore cut after `chain` k-blocks and

@@ -231,8 +231,8 @@ typedef struct fg_dropout_spec {
  * (receives z, for fg_linear_grad) may be NULL; drop.p = 0 for no dropout.
  * out may be the residual itself (same pointer and pitch); no other output
  * may overlap an input.  Products run on the tensor cores, f32 ones as sums of
- * bf16 products to f32 accuracy (an infinity in an f32 operand may give NaN
- * where f32 arithmetic gives infinity).  workspace: at least
+ * bf16 products to f32 accuracy, infinities and overflow as f32 arithmetic
+ * gives them (f32 operands below 2^-110 lose bits).  workspace: at least
  * fg_linear_workspace() bytes of device memory, 256-byte aligned, free for
  * reuse once the call's work on the stream is done. */
 typedef struct fg_linear_args {

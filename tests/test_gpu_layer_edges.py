@@ -1,10 +1,12 @@
 """The layer operators at the edges of their range: the bounds are those of
 test_gpu_layer.py unless a test derives its own."""
+import numpy as np
 import pytest
 import torch
 
 from ferrograd_b200 import kernels
-from test_gpu_layer import forward_case, grad_case
+from layer_ref import act as ref_act
+from test_gpu_layer import f64, forward_case, grad_case, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -49,8 +51,9 @@ def test_given_stream_leaves_the_current_ones_memory_alone(name):
     does that work reach the call's results, nor the call that work's input."""
     side = torch.cuda.Stream()
     call = one_of_each(side.cuda_stream)[name]
-    want = [t.clone() for t in call()]
+    want = call()
     torch.cuda.synchronize()
+    want = [t.clone() for t in want]
     for _ in range(2):  # the results of 4 MB, then the workspaces of 3 to 13
         torch.cuda.empty_cache()
         later = torch.empty_like(want[0])
@@ -76,7 +79,9 @@ def test_given_stream_keeps_what_the_call_still_uses(name):
     handed to the current stream before it is done with them."""
     side = torch.cuda.Stream()
     calls = one_of_each(side.cuda_stream)
-    want = [t.clone() for t in calls[name]()]
+    want = calls[name]()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in want]
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
     calls = one_of_each(side.cuda_stream)
@@ -130,3 +135,55 @@ def test_two_streams_at_once(explicit):
     torch.cuda.synchronize()
     for i, r in got:
         assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+# ---- infinities and overflow in f32 ------------------------------------------------------
+
+
+ROWS = [(5, 40, 72), (40, 96, 200), (300, 264, 136), (2560, 2304, 96)]
+
+
+def same_class(got, ref, what):
+    """Equal infinities and NaN; finite where the definition is."""
+    got = f64(got)
+    for of in (np.isnan, np.isposinf, np.isneginf):
+        assert np.array_equal(of(got), of(ref)), (what, of.__name__)
+
+
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("m,n,k", ROWS)
+def test_f32_infinities_are_f32s(m, n, k, act):
+    """Infinities of both signs in x and in w, zeros opposite some, and two
+    opposite each other: every element is what the 64-bit formula gives."""
+    rng = np.random.default_rng(m)
+    x, w, dy = (randn(rng, *s, torch.float32) for s in ((m, k), (n, k), (m, n)))
+    x[1, 5], x[m - 1, 7], w[2, 9], w[n - 1, 5] = np.inf, -np.inf, -np.inf, np.inf
+    w[3, 5] = w[4, 7] = x[0, 9] = 0.0
+    x[2, 11] = x[2, 12] = np.inf
+    w[6, 11], w[6, 12] = 1.0, -1.0
+    with np.errstate(invalid="ignore"):
+        z = f64(x) @ f64(w).T
+        same_class(kernels.linear(x, w, act=act), ref_act(z, act), "out")
+        dy[1, 3], dy[3, 3] = np.inf, -np.inf
+        got = kernels.linear_grad(dy, x, w)
+        for g, r, name in zip(got, (f64(dy) @ f64(w), f64(dy).T @ f64(x), f64(dy).sum(0)),
+                              ("dx", "dw", "db")):
+            same_class(g, r, name)
+
+
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("m,n,k", ROWS)
+def test_f32_overflow_keeps_its_sign(m, n, k, act):
+    """Finite operands whose products are beyond f32: infinite, of the sum's sign.
+    In each row of x the terms are of one sign, so no order of summation gives
+    NaN; the last column is small enough to stay finite."""
+    rng = np.random.default_rng(n)
+    for big_x, big_w in ((1.5e21, 1.5e21), (3e38, 3.9), (3e38, 40.0), (1e30, 1e9)):
+        x = torch.from_numpy(rng.uniform(0.5, 1.0, (m, k)) * big_x).float().cuda()
+        w = torch.from_numpy(rng.uniform(0.5, 1.0, (n, k)) * big_w).float().cuda()
+        x[1::2] *= -1
+        w[n - 1] = torch.from_numpy(rng.uniform(0.0, 1e-3 / k, k)).float()
+        z = f64(x) @ f64(w).T
+        z[np.abs(z) > 3.5e38] *= np.inf
+        assert np.isinf(z[:, :n - 1]).all() and np.isfinite(z[:, n - 1]).all()
+        same_class(kernels.linear(x, w, act=act), ref_act(z, act), (big_x, big_w))
