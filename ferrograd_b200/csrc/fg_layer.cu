@@ -192,7 +192,9 @@ static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaSt
 // ---------------------------------------------------------------------------
 // dz = D(dy) * act'(pre), and the column sums of dz over this block's rows
 // (f32, one row of `part` a block; k_bias_grad adds them up in order).
-// dz may be null (only the sums are wanted).
+// dz may be null (only the sums are wanted).  What it writes is dz * unit / scale
+// (DzScale): without dropout's scale the 16-bit types hold dy itself where no
+// slope multiplies it, and f16 does not overflow.
 // It reads dy and pre once and writes dz once: 1.6 GB at 16384 x 16384 bf16, GELU,
 // 246 us at the copy rate, measured 391 us: with the slope's exponential and the
 // conversions 36 instructions an element, the issue slots bound it, not HBM.  A
@@ -213,14 +215,18 @@ __device__ __forceinline__ void store_dz<float>(void *dz, int64_t at, int64_t pl
 #pragma unroll
   for (int k = 0; k < 3; k++) store8(static_cast<__nv_bfloat16 *>(dz) + k * plane + at, p[k]);
 }
+// How dz is scaled where it is stored, and what its sums are multiplied by.
+struct DzScale {
+  float unit, after;
+};
 // TX: groups of eight columns across a block, 32 or 4 (small matrices); 256 /
 // TX rows down it.  Where one block has all rows of its columns it writes db
 // itself.
 template <typename T, int TX>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
     k_layer_dz(const T *dy, int64_t yr, int64_t yc, const T *pre,
-               int64_t ldp, int act, const DropParams drop, void *dz, int64_t ldz,
-               float *part, T *db, int M, int N, int rows, int vec) {
+               int64_t ldp, int act, const DropParams drop, const DzScale by, void *dz,
+               int64_t ldz, float *part, T *db, int M, int N, int rows, int vec) {
   constexpr int TY = 256 / TX;
   __shared__ float red[TY][TX * 8];
   constexpr int U = 2;  // rows in flight, and as many again asked for
@@ -231,7 +237,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
   grid_wait();
   grid_launch_next();
   auto one = [&](int r, float(&v)[8], const float(&z)[8]) {
-    if (drop.on) drop8(drop, r, col, v);
+    if (drop.on) {  // whose scale is by.unit
+      drop8(drop, r, col, v);
+    } else if (by.unit != 1.0f) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] *= by.unit;
+    }
     slope8<sizeof(T) == 2>(v, z, act);
 #pragma unroll
     for (int i = 0; i < 8; i++) sum[i] += v[i];
@@ -282,6 +293,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
     float s = 0.0f;
 #pragma unroll 8
     for (int w = 0; w < TY; w++) s += red[w][threadIdx.x];
+    s *= by.after;
     if (gridDim.y == 1)
       db[c] = from_f32<T>(s);
     else
@@ -612,14 +624,14 @@ static GradPlan plan_grad(const fg_linear_grad_args *g) {
 
 template <typename T>
 static int run_dz(const fg_linear_grad_args *g, const GradPlan &p, const DropParams &drop,
-                  cudaStream_t st) {
+                  const DzScale &by, cudaStream_t st) {
   char *ws = static_cast<char *>(g->workspace);
   const DzShape &d = p.shape;
   float *part = g->db && d.chunks > 1 ? reinterpret_cast<float *>(ws + p.part_off) : nullptr;
   const dim3 grid((unsigned)((g->N + 8LL * d.tx - 1) / (8 * d.tx)), d.chunks);
   int rc = launch_early(d.tx == 32 ? k_layer_dz<T, 32> : k_layer_dz<T, 4>, grid, 256, st,
                         static_cast<const T *>(g->dy), g->dy_row, g->dy_col,
-                        static_cast<const T *>(g->pre), g->ld_pre, g->act, drop,
+                        static_cast<const T *>(g->pre), g->ld_pre, g->act, drop, by,
                         p.make_dz ? ws + p.dz_off : nullptr, p.ldz, part, static_cast<T *>(g->db),
                         g->M, g->N, d.rows, d.vec);
   if (rc || !part) return rc;
@@ -703,20 +715,28 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
   place_operand(&p.x, g->workspace);
   place_jobs(&p.jobs, g->workspace);
   if ((rc = run_stage(g->dtype, p.jobs, st))) return rc;
+  // Dropout's scale multiplies the sums, and GELU's and SiLU's slopes, which reach
+  // 1.13, act on halves in f16: the stored dz is finite where dy is.  (A half
+  // costs values below 2^-13 a bit.)
+  const bool steep = g->act != FG_ACT_NONE && g->act != FG_ACT_RELU;
+  const float unit = g->dtype == FG_F16 && steep ? 0.5f : 1.0f;
+  const DzScale by{unit, (drop.on && drop.some ? drop.scale : 1.0f) / unit};
+  drop.scale = unit;
   if (p.make_dz || g->db) {
     switch (g->dtype) {
       case FG_F32:
-        rc = run_dz<float>(g, p, drop, st);
+        rc = run_dz<float>(g, p, drop, by, st);
         break;
       case FG_BF16:
-        rc = run_dz<__nv_bfloat16>(g, p, drop, st);
+        rc = run_dz<__nv_bfloat16>(g, p, drop, by, st);
         break;
       default:
-        rc = run_dz<__half>(g, p, drop, st);
+        rc = run_dz<__half>(g, p, drop, by, st);
     }
     if (rc) return rc;
   }
   Product dx{p.z_dx, p.w, g->N, {}}, dw{p.z_dw, p.x, g->M, {}};
+  dx.e.scale = dw.e.scale = p.make_dz ? by.after : 1.0f;
   // dx[m, k] = sum_n dz(m, n) w(n, k)
   dx.e.out = g->dx;
   dx.e.ldo = g->ld_dx;

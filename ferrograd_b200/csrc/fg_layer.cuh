@@ -384,11 +384,16 @@ struct Epilogue {
   int64_t ldr, ldp, ldo;
   int M, N;
   int vec;  // every array's rows start on 16-byte boundaries: 16-byte accesses
+  float scale = 1.0f;  // of the sums, before the bias (a gradient's products)
 };
 
-// v += bias for the columns col .. col+7 (those beyond N keep v).
+// v = scale v + bias for the columns col .. col+7 (those beyond N get no bias).
 template <typename T>
-__device__ __forceinline__ void bias8(const Epilogue &e, int col, float (&v)[8]) {
+__device__ __forceinline__ void affine8(const Epilogue &e, int col, float (&v)[8]) {
+  if (e.scale != 1.0f) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= e.scale;
+  }
   if (!e.bias) return;
   const T *b = static_cast<const T *>(e.bias) + col;
   if (e.vec && col + 8 <= e.N) {
@@ -442,7 +447,7 @@ __device__ __forceinline__ void epilogue8(const Epilogue &e, int row, int col, f
         if (i < n) t[i] = from_f32<T>(v[i]);
     }
   };
-  bias8<T>(e, col, v);
+  affine8<T>(e, col, v);
   if (e.pre) put(e.pre, e.ldp);
   act8<sizeof(T) == 2>(v, e.act);
   if (e.drop.on) drop8(e.drop, row, col, v);
@@ -508,7 +513,7 @@ __device__ __forceinline__ void epilogue_slab(const Epilogue &e, float *slab, in
     reinterpret_cast<float4 *>(mine)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4 *>(mine)[1] = make_float4(v[4], v[5], v[6], v[7]);
   };
-  bias8<T>(e, col0 + c, v);
+  affine8<T>(e, col0 + c, v);
   if (e.pre) {
     put();
     slab_flush<T>(slab, lc, static_cast<T *>(e.pre), e.ldp, row0, col0, e.M, e.N);
@@ -527,7 +532,7 @@ __device__ __forceinline__ void epilogue_slab(const Epilogue &e, float *slab, in
   slab_flush<T>(slab, lc, static_cast<T *>(e.out), e.ldo, row0, col0, e.M, e.N);
 }
 
-// epilogue8 for one element.
+// epilogue8 for one element (of a product with scale 1).
 template <typename T>
 __device__ __forceinline__ void epilogue1(const Epilogue &e, int row, int col, float z) {
   if (e.bias) z += to_f32<T>(static_cast<const T *>(e.bias)[col]);

@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, CG == 1 && !RUN ? 2 :
           sums(c, false, v);
 #pragma unroll
           for (int p = 0; p < 2; p++) {
-            bias8<T>(e, col + c + 8 * p, v[p]);
+            affine8<T>(e, col + c + 8 * p, v[p]);
             store8_smem<T>(pre_chunk, c + 8 * p, v[p]);
           }
         }
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(Block<CG, RUN>::threads, CG == 1 && !RUN ? 2 :
         sums(c, true, v);
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-          bias8<T>(e, col + c + 8 * p, v[p]);
+          affine8<T>(e, col + c + 8 * p, v[p]);
           if (kTwo && e.pre) store8_smem<T>(pre_chunk, c + 8 * p, v[p]);
           act8<sizeof(T) == 2>(v[p], e.act);
           if (e.drop.on) drop8(e.drop, row, col + c + 8 * p, v[p]);

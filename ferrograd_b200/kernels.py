@@ -190,7 +190,8 @@ def linear_grad(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
     needed for ``act="none"``).  Gradients that are not wanted are ``None``.
     The residual's gradient is ``dy`` itself; ``dx_residual`` [M, K] is added to
     ``dx`` in the product's epilogue.  With 16-bit types the gradient at the
-    pre-activations is rounded to that type before the two products."""
+    pre-activations is rounded to that type before the two products (exact for
+    ``"none"`` and ``"relu"``: dropout's scale multiplies the sums)."""
     code = _act_code(act)
     if code and pre is None:
         raise ValueError(f"the gradient of {act} needs pre (linear(..., save_pre=True))")

@@ -262,8 +262,10 @@ int fg_linear(const fg_linear_args *args, void *stream);
  * dz^T x [N, K]; db = column sums of dz [N].  dx, dw and db may each be NULL
  * (not wanted); dx_residual [M, K] may be NULL, or dx itself (same pointer and
  * pitch): where x also went round the layer, the gradient that came that way.
- * For the 16-bit types dz is rounded to that type before the two products; db is summed from the unrounded dz.  Sums
- * run in a fixed order: the same inputs give the same bits. */
+ * For the 16-bit types dz, without dropout's scale (which multiplies the sums), is
+ * rounded to that type before the two products: exact for no activation and ReLU,
+ * one rounding for the others.  db is summed from the unrounded dz.  Sums run in a
+ * fixed order: the same inputs give the same bits. */
 typedef struct fg_linear_grad_args {
   int32_t dtype, M, N, K;
   const void *dy;

@@ -5,8 +5,9 @@ import pytest
 import torch
 
 from ferrograd_b200 import kernels
-from layer_ref import act as ref_act
-from test_gpu_layer import f64, forward_case, grad_case, randn
+from layer_ref import act as ref_act, linear_grad as ref_grad
+from test_gpu_layer import CURVE, ROUND, STEP, TINY, TYPES, check, f64, forward_case, grad_case, \
+    randn
 
 pytestmark = pytest.mark.gpu
 
@@ -187,3 +188,49 @@ def test_f32_overflow_keeps_its_sign(m, n, k, act):
         z[np.abs(z) > 3.5e38] *= np.inf
         assert np.isinf(z[:, :n - 1]).all() and np.isfinite(z[:, n - 1]).all()
         same_class(kernels.linear(x, w, act=act), ref_act(z, act), (big_x, big_w))
+
+
+# ---- dz in 16 bits -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("m,n,k", [(90, 72, 56), (300, 512, 264), (2560, 2304, 320)])
+def test_grad_without_a_slope_is_rounded_once(dtype, act, m, n, k):
+    """Dropout's scale 1/(1 - p) is no 16-bit value; the products see dy all the
+    same.  One rounding of normally distributed values to bf16 is off by 0.85 2^-9
+    in the 2-norm (f16: 2^-12), two in a row by 1.2; between them lies the bound
+    for dx and dw.  db, of fewer values, is held to the largest error."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    dt = TYPES[dtype]
+    new = lambda r, c, s=1.0: torch.empty((r, c), dtype=dt, device="cuda").normal_(  # noqa: E731
+        0, s, generator=gen)
+    dy, x, w, pre = new(m, n), new(m, k), new(n, k, 0.1), new(m, n)
+    spec = (0.3, 3, 1 << 40)
+    got = kernels.linear_grad(dy, x, w, pre=pre, act=act, drop=kernels.Dropout(*spec))
+    dx, dw, db, dz = ref_grad(f64(dy), f64(x), f64(w), f64(pre), act, spec)
+    for g, r, most in zip(got, (dx, dw, db), (0.5, 0.5, 1.0)):
+        assert np.linalg.norm(f64(g) - r) <= most * ROUND[dtype] * np.linalg.norm(r)
+
+
+@pytest.mark.parametrize("act,at", [("none", 0.0), ("relu", 1.0), ("gelu", 1.4), ("gelu_tanh", 1.4),
+                                    ("silu", 2.4)])
+@pytest.mark.parametrize("m,n,k", [(40, 64, 72), (300, 264, 136), (2560, 2304, 96)])
+def test_f16_grad_beyond_f16s_range(act, at, m, n, k):
+    """dz is up to 1.13 * 65504 / (1 - p), the gradients are not: no infinity.
+    The bounds are grad_case's; a slope near its maximum."""
+    rng = np.random.default_rng(m + n)
+    spec = (0.5, 5, 6) if m != 300 else None
+    dy = torch.from_numpy(rng.choice([-65504.0, 65504.0, 60000.0], (m, n))).half().cuda()
+    x, w = randn(rng, m, k, torch.float16, 1e-3), randn(rng, n, k, torch.float16, 1e-3)
+    pre = torch.full((m, n), at, dtype=torch.float16, device="cuda")
+    got = kernels.linear_grad(dy, x, w, pre=pre, act=act, need_db=False,
+                              drop=kernels.Dropout(*spec) if spec else None)
+    dx, dw, _, dz = ref_grad(f64(dy), f64(x), f64(w), f64(pre), act, spec)
+    u, tiny = ROUND["f16"], TINY["f16"]
+    r = (CURVE * 2 + 2 * STEP + u) * np.abs(dz)
+    for g, ref, left, right, terms, rr in ((got[0], dx, np.abs(dz), np.abs(f64(w)), n, r),
+                                           (got[1], dw, np.abs(dz).T, np.abs(f64(x)), m, r.T)):
+        assert np.abs(ref).max() < 65504
+        check(g, ref, (terms + 16) * STEP * (left @ right) + rr @ right + u * np.abs(ref) + tiny,
+              act)
