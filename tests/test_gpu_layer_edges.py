@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from ferrograd_b200 import kernels
-from layer_ref import act as ref_act, linear_grad as ref_grad
+from layer_ref import act as ref_act, linear_grad as ref_grad, slope as ref_slope
 from test_gpu_layer import CURVE, ROUND, STEP, TINY, TYPES, check, f64, forward_case, grad_case, \
     randn
 
@@ -234,3 +234,28 @@ def test_f16_grad_beyond_f16s_range(act, at, m, n, k):
         assert np.abs(ref).max() < 65504
         check(g, ref, (terms + 16) * STEP * (left @ right) + rr @ right + u * np.abs(ref) + tiny,
               act)
+
+
+# ---- the activations' tails ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [3, 2000])
+def test_left_tails_keep_their_digits(dtype, act, rows):
+    """act and its slope for z in [-8, -1.5], through w = 1, relative to their
+    value.  Phi by its polynomial is good to 2^-15.  An exponential's argument is at
+    most 49 (the tanh form's at -8) and three times rounded, 2^-24 each: 2^-16.8 of
+    the value; f32's functions add little, so 2^-16.5 there and 2^-14 in 16 bits.
+    The slopes are differences that shrink by at most 5 (SiLU's zero is at -1.28):
+    2^-14 and 2^-11.5.  Then the output's rounding; f16 adds one unit among
+    subnormals to each rounding, of which the slope has two, the first of a half."""
+    z = torch.linspace(-8, -1.5, rows, device="cuda").to(TYPES[dtype]).view(-1, 1)
+    one = torch.ones((1, 1), dtype=TYPES[dtype], device="cuda")
+    near, steep = (2.0 ** -16.5, 2.0 ** -14) if dtype == "f32" else (2.0 ** -14, 2.0 ** -11.5)
+    ref = ref_act(f64(z), act)
+    check(kernels.linear(z, one, act=act), ref, (near + ROUND[dtype]) * np.abs(ref) + TINY[dtype],
+          act)
+    ref = ref_slope(f64(z), act)
+    dx = kernels.linear_grad(torch.ones_like(z), z, one, pre=z, act=act)[0]
+    check(dx, ref, (steep + 2 * ROUND[dtype]) * np.abs(ref) + 2 * TINY[dtype], act)
