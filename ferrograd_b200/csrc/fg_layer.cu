@@ -191,7 +191,7 @@ static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaSt
 
 // ---------------------------------------------------------------------------
 // dz = D(dy) * act'(pre), and the column sums of dz over this block's rows
-// (f32, one row of `part` a block; k_bias_grad adds them up in order).
+// (f32, one row of `part` a block; k_bias_grad adds them up).
 // dz may be null (only the sums are wanted).  What it writes is dz * unit / scale
 // (DzScale): without dropout's scale the 16-bit types hold dy itself where no
 // slope multiplies it, and f16 does not overflow.
@@ -285,15 +285,19 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
       one(r, v, z);
     }
   }
+  if (!db) return;
 #pragma unroll
   for (int i = 0; i < 8; i++) red[ty][tx * 8 + i] = sum[i];
   __syncthreads();
   const int c = blockIdx.x * (TX * 8) + threadIdx.x;
-  if (db && threadIdx.x < TX * 8 && c < N) {
-    float s = 0.0f;
-#pragma unroll 8
-    for (int w = 0; w < TY; w++) s += red[w][threadIdx.x];
-    s *= by.after;
+#pragma unroll
+  for (int half = TY / 2; half > 0; half /= 2) {  // a tree: TY terms, log2 TY roundings
+    for (int i = threadIdx.x; i < half * TX * 8; i += 256)
+      red[i / (TX * 8)][i % (TX * 8)] += red[i / (TX * 8) + half][i % (TX * 8)];
+    __syncthreads();
+  }
+  if (threadIdx.x < TX * 8 && c < N) {
+    const float s = red[0][threadIdx.x] * by.after;
     if (gridDim.y == 1)
       db[c] = from_f32<T>(s);
     else
@@ -301,20 +305,34 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
   }
 }
 
-// db = the blocks' sums, a thread a column, in the order of the rows.  At most 128
-// a column (dz_shape); bound by the latency of that chain of reads, 14 us for 8192
-// columns of 128, beside products of a millisecond.
+// db = the blocks' sums, in a fixed order: 32 columns a block, a column's sums dealt
+// to 32 threads, each of which carries the rounding of its additions along (W.
+// Kahan, "Further remarks on reducing truncation errors", 1965), and joined as a
+// tree.  Latency of a few reads.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     k_bias_grad(const float *part, int chunks, int N, T *db) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  __shared__ float red[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + x;
   grid_wait();
   grid_launch_next();
-  if (c >= N) return;
-  float s = 0.0f;
-#pragma unroll 8
-  for (int i = 0; i < chunks; i++) s += part[(size_t)i * N + c];
-  db[c] = from_f32<T>(s);
+  float s = 0.0f, lost = 0.0f;
+  if (c < N) {
+#pragma unroll 4
+    for (int i = y; i < chunks; i += 32) {
+      const float v = part[(size_t)i * N + c] - lost, t = s + v;
+      lost = isfinite(t) ? (t - s) - v : 0.0f;
+      s = t;
+    }
+  }
+  red[y][x] = s;
+#pragma unroll
+  for (int half = 16; half > 0; half /= 2) {
+    __syncthreads();
+    if (y < half) red[y][x] += red[y + half][x];
+  }
+  if (y == 0 && c < N) db[c] = from_f32<T>(red[0][x]);
 }
 
 // ---------------------------------------------------------------------------
@@ -550,9 +568,11 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
 
 // How k_layer_dz is cut: blocks of 256 columns for large arrays (16384 x 16384
 // bf16: 391 us), of 32 columns x 64 rows for small ones; rows a
-// block such that there are several waves of blocks but at most 128 partial sums
-// a column, and one block for all rows where eight passes do (then it writes db
-// itself and a launch is saved).
+// block such that there are several waves of blocks and a thread adds no more than
+// 16 rows one after another for an f32 sum (64 for a 16-bit one), and one block for
+// all rows where eight passes do (then it writes db itself and a launch is saved).
+// f32 db is off by 2^-23 of random sums' norm then; with 128 chains added in
+// turn it was 2^-22.
 struct DzShape {
   int vec, tx, rows, chunks;
 };
@@ -566,6 +586,9 @@ static DzShape dz_shape(const fg_linear_grad_args *g) {
   const int64_t blocks = d.tx == 32 ? 4096 : 592;
   int64_t chunks = g->M <= 8 * down ? 1 : strips >= blocks ? 1 : blocks / strips;
   if (chunks > 128) chunks = 128;
+  const int64_t deep = down * (es == 4 ? 16 : 64);
+  if (g->M > 8 * down && chunks < (g->M + deep - 1) / deep) chunks = (g->M + deep - 1) / deep;
+  if (chunks > 65535) chunks = 65535;  // of a grid's y
   const int64_t rows = ((g->M + chunks - 1) / chunks + down - 1) / down * down;
   d.rows = (int)(rows < 0x7fffff00 ? rows : 0x7fffff00);
   d.chunks = (int)((g->M + (int64_t)d.rows - 1) / d.rows);
@@ -635,7 +658,7 @@ static int run_dz(const fg_linear_grad_args *g, const GradPlan &p, const DropPar
                         p.make_dz ? ws + p.dz_off : nullptr, p.ldz, part, static_cast<T *>(g->db),
                         g->M, g->N, d.rows, d.vec);
   if (rc || !part) return rc;
-  return launch_early(k_bias_grad<T>, dim3((unsigned)((g->N + 255LL) / 256)), 256, st, part,
+  return launch_early(k_bias_grad<T>, dim3((unsigned)((g->N + 31LL) / 32)), 1024, st, part,
                       d.chunks, g->N, static_cast<T *>(g->db));
 }
 
