@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
   constexpr int U = 2;  // rows in flight, and as many again asked for
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const int col = blockIdx.x * (TX * 8) + tx * 8;
-  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
+  const int r0 = blockIdx.y * rows, r1 = r0 + min(rows, M - r0);  // (r0 + rows may pass 2^31)
   float sum[8] = {};
   grid_wait();
   grid_launch_next();

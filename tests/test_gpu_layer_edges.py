@@ -281,3 +281,15 @@ def test_f32_bias_gradient_is_summed_as_a_tree(m, n, most):
     assert float((db - ref).norm() / ref.norm()) <= 2.0 ** most
     again = kernels.linear_grad(dy, x, w, need_dx=False, need_dw=False)[2]
     assert torch.equal(db, again)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_bias_gradient_of_the_longest_batch(dtype):
+    """2^31 - 256 rows: the last block of rows ends where an int does."""
+    m = 0x7fffff00
+    dy = torch.zeros((m, 1), dtype=TYPES[dtype], device="cuda")
+    for at in (0, m // 2, m - 1):
+        dy[at] = 1.0
+    one = torch.ones((1, 1), dtype=TYPES[dtype], device="cuda")
+    db = kernels.linear_grad(dy, one.expand(m, 1), one, need_dx=False, need_dw=False)[2]
+    assert float(db) == 3.0
