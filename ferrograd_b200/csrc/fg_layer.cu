@@ -21,7 +21,7 @@ using ptx::grid_launch_next;
 using ptx::grid_wait;
 
 // ---------------------------------------------------------------------------
-// K = 0: there is nothing to read, every sum is 0 and the epilogue remains.
+// Sums over nothing (K = 0, or a gradient's N = 0): all are 0 and the epilogue remains.
 // Bound by the output's writes; a thread has eight columns of a row a step.
 // ---------------------------------------------------------------------------
 template <typename T>
@@ -717,13 +717,13 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
   if (rc) return rc;
   const int es = elem_size(g->dtype);
   if (g->M == 0 || g->N == 0) {  // sums over nothing
-    if (g->dx_residual && g->dx && g->M > 0 && g->K > 0) {
-      if (g->dx_residual != g->dx)
-        FG_CUDA_TRY(cudaMemcpy2DAsync(g->dx, g->ld_dx * es, g->dx_residual,
-                                      g->ld_dx_residual * es, (size_t)g->K * es, g->M,
-                                      cudaMemcpyDeviceToDevice, st));
-    } else if ((rc = zero_rows(g->dx, g->ld_dx, g->M, g->K, es, st))) {
-      return rc;
+    if (g->dx && g->M > 0 && g->K > 0) {
+      Epilogue e{};
+      e.out = g->dx, e.ldo = g->ld_dx;
+      e.residual = g->dx_residual, e.ldr = g->ld_dx_residual;
+      e.M = g->M, e.N = g->K;
+      e.vec = rows16(e.out, e.ldo, es) && rows16(e.residual, e.ldr, es);
+      if ((rc = run_empty_product(g->dtype, e, st))) return rc;
     }
     if ((rc = zero_rows(g->dw, g->ld_dw, g->N, g->K, es, st))) return rc;
     return zero_rows(g->db, g->N, 1, g->N, es, st);

@@ -293,3 +293,17 @@ def test_bias_gradient_of_the_longest_batch(dtype):
     one = torch.ones((1, 1), dtype=TYPES[dtype], device="cuda")
     db = kernels.linear_grad(dy, one.expand(m, 1), one, need_dx=False, need_dw=False)[2]
     assert float(db) == 3.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(5, 8), (70, 33)])
+def test_no_outputs_leave_the_gradient_that_went_round(dtype, m, k):
+    """N = 0: dx is dx_residual, whatever its rows' stride (repeated, overlapping, wide)."""
+    dt = TYPES[dtype]
+    new = lambda *s: torch.empty(s, dtype=dt, device="cuda").normal_()  # noqa: E731
+    dy, x, w = new(m, 0), new(m, k), new(0, k)
+    for r in (new(1, k).expand(m, k), new(m + k).as_strided((m, k), (1, 1)), new(m, k + 3)[:, 2:2 + k],
+              new(m, k)):
+        dx, dw, db = kernels.linear_grad(dy, x, w, dx_residual=r)
+        assert torch.equal(dx, r) and dw.shape == (0, k) and db.shape == (0,)
+    assert not kernels.linear_grad(dy, x, w)[0].any()
