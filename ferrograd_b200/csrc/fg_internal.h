@@ -36,12 +36,17 @@ void count_launch(int n = 1);
 
 }  // namespace fg
 
+// (A failed call also leaves its error with the runtime, where the caller's own
+// next check, torch's after a launch for one, would take it for its own; it is
+// returned here and cleared there.  Errors that end a context stay.)
 #define FG_CUDA_TRY(expr)                                                                   \
   do {                                                                                      \
     cudaError_t fg_e_ = (expr);                                                             \
-    if (fg_e_ != cudaSuccess)                                                               \
+    if (fg_e_ != cudaSuccess) {                                                             \
+      cudaGetLastError();                                                                   \
       return fg::set_error(FG_ERR_CUDA, "%s failed: %s (%s:%d)", #expr,                     \
                            cudaGetErrorString(fg_e_), __FILE__, __LINE__);                 \
+    }                                                                                       \
   } while (0)
 
 #define FG_LAUNCH_TRY()                                                                     \

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from ferrograd_b200 import kernels
+from ferrograd_b200 import CudaDevice, kernels
+from ferrograd_b200.device import Event
 from layer_ref import act as ref_act, linear_grad as ref_grad, slope as ref_slope
 from test_gpu_layer import CURVE, ROUND, STEP, TINY, TYPES, check, f64, forward_case, grad_case, \
     randn
@@ -307,3 +308,13 @@ def test_no_outputs_leave_the_gradient_that_went_round(dtype, m, k):
         dx, dw, db = kernels.linear_grad(dy, x, w, dx_residual=r)
         assert torch.equal(dx, r) and dw.shape == (0, k) and db.shape == (0,)
     assert not kernels.linear_grad(dy, x, w)[0].any()
+
+
+def test_a_failed_call_leaves_no_error_behind():
+    """The runtime's last error after a refused call is not there for torch's next
+    launch to find (two events that were never recorded have no time between)."""
+    device = CudaDevice()
+    start, end = Event(device), Event(device)
+    with pytest.raises(kernels._lib.FerroError):
+        Event.elapsed_ms(start, end)
+    assert float((torch.ones(8, device="cuda") + 1).sum()) == 16
