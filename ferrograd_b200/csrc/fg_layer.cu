@@ -434,6 +434,13 @@ static bool rows16(const void *p, int64_t ld, int es) {
   return !p || ((uintptr_t)p % 16 == 0 && ld * es % 16 == 0);
 }
 
+// Every address is a multiple of the element's size (an odd one would be a
+// misaligned access on the device).
+template <typename... P>
+static bool whole(int es, const P *...p) {
+  return (((uintptr_t)p % es == 0) && ...);
+}
+
 // A rows x cols array's bytes [lo, hi), strides of either sign included.
 struct Span {
   uintptr_t lo, hi;
@@ -509,6 +516,8 @@ static int check_linear(const fg_linear_args *g, DropParams *drop) {
   if (g->M == 0 || g->N == 0) return FG_OK;
   const int es = elem_size(g->dtype);
   FG_REQUIRE(g->out && (g->K == 0 || (g->x && g->w)), "%s: null operand", who);
+  FG_REQUIRE(whole(es, g->x, g->w, g->bias, g->residual, g->pre, g->out),
+             "%s: an address is not a multiple of the element's size", who);
   FG_REQUIRE(g->ld_out >= g->N && (!g->pre || g->ld_pre >= g->N), "%s: output pitch too small",
              who);
   for (int i = 0; i < 2; i++) {
@@ -535,6 +544,8 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
   LinearPlan p = plan_linear(g);
   FG_REQUIRE(g->workspace_bytes >= p.bytes && (p.bytes == 0 || g->workspace),
              "fg_linear: %zu bytes of workspace needed, got %zu", p.bytes, g->workspace_bytes);
+  FG_REQUIRE(p.bytes == 0 || whole(256, g->workspace),
+             "fg_linear: the workspace is not on a 256-byte boundary");
   const int es = elem_size(g->dtype);
   e.act = g->act;
   e.bias = g->bias;
@@ -677,6 +688,9 @@ static int check_grad(const fg_linear_grad_args *g, DropParams *drop) {
   FG_REQUIRE((!g->dx || g->ld_dx >= g->K) && (!g->dw || g->ld_dw >= g->K),
              "%s: output pitch too small", who);
   const int es = elem_size(g->dtype);
+  FG_REQUIRE(whole(es, g->dy, g->x, g->w, g->act ? g->pre : nullptr, g->dx,
+                   g->dx ? g->dx_residual : nullptr, g->dw, g->db),
+             "%s: an address is not a multiple of the element's size", who);
   struct Out {
     const char *name;
     const void *p;
@@ -732,6 +746,8 @@ static int linear_grad(const fg_linear_grad_args *g, cudaStream_t st) {
   FG_REQUIRE(g->workspace_bytes >= p.bytes && (p.bytes == 0 || g->workspace),
              "fg_linear_grad: %zu bytes of workspace needed, got %zu", p.bytes,
              g->workspace_bytes);
+  FG_REQUIRE(p.bytes == 0 || whole(256, g->workspace),
+             "fg_linear_grad: the workspace is not on a 256-byte boundary");
   place_operand(&p.z_dx, g->workspace);
   place_operand(&p.z_dw, g->workspace);
   place_operand(&p.w, g->workspace);
@@ -793,6 +809,8 @@ static int dropout(int dtype, int64_t rows, int64_t cols, const void *x, int64_t
   if (rc) return rc;
   if (rows == 0 || cols == 0) return FG_OK;
   FG_REQUIRE(x && out, "%s: null operand", who);
+  FG_REQUIRE(whole(es, x, residual, out), "%s: an address is not a multiple of the element's size",
+             who);
   FG_REQUIRE(ldo >= cols || rows == 1, "%s: output pitch too small", who);
   FG_REQUIRE((x == out && ldx == ldo) || !overlap(out, rows, cols, ldo, x, rows, cols, ldx, 1, es),
              "%s: out overlaps x (it may only be all of it)", who);
