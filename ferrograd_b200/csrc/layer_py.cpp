@@ -40,7 +40,11 @@ void check(int code) {
 
 const at::Tensor &tensor(PyObject *o, const char *name) {
   if (!THPVariable_Check(o)) value_error(std::string(name) + ": expected a tensor");
-  return THPVariable_Unpack(o);
+  const at::Tensor &t = THPVariable_Unpack(o);
+  // (such a view's memory holds the values before the sign, or nothing)
+  if (t.is_neg() || t._is_zerotensor())
+    value_error(std::string(name) + ": a lazily negated or zero tensor (see resolve_neg)");
+  return t;
 }
 
 double real(PyObject *o) {

@@ -318,3 +318,20 @@ def test_a_failed_call_leaves_no_error_behind():
     with pytest.raises(kernels._lib.FerroError):
         Event.elapsed_ms(start, end)
     assert float((torch.ones(8, device="cuda") + 1).sum()) == 16
+
+
+# ---- what the binding refuses or passes on ---------------------------------------------------
+
+
+def test_lazily_negated_views_are_refused():
+    """The imaginary part of a conjugate shares memory that holds its negative."""
+    z = torch.randn((6, 6), device="cuda", dtype=torch.complex64).conj().imag
+    assert z.is_neg()
+    w = torch.randn((6, 6), device="cuda")
+    for call in (lambda t: kernels.linear(t, w), lambda t: kernels.linear(w, t),
+                 lambda t: kernels.linear(w, w, residual=t), lambda t: kernels.linear(w, w, out=t),
+                 lambda t: kernels.linear_grad(t, w, w), lambda t: kernels.linear_grad(w, w, t),
+                 lambda t: kernels.dropout(t, kernels.Dropout(0.5, 1))):
+        with pytest.raises(ValueError):
+            call(z)
+        call(z.resolve_neg())
