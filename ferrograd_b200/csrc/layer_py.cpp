@@ -323,6 +323,15 @@ PyObject *dropout(PyObject *const *o) {
   return o[5] == Py_None ? THPVariable_Wrap(out) : Py_NewRef(o[5]);
 }
 
+// Sets the error module.name(message).
+void raise(const char *module, const char *name, const char *message) {
+  PyObject *mod = PyImport_ImportModule(module);
+  PyObject *cls = mod ? PyObject_GetAttrString(mod, name) : nullptr;
+  if (cls) PyErr_SetString(cls, message);
+  Py_XDECREF(cls);
+  Py_XDECREF(mod);
+}
+
 // No C++ exception leaves the module.
 template <PyObject *(*F)(PyObject *const *), Py_ssize_t N>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -334,6 +343,8 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     return F(args);
   } catch (const Raised &) {
     return nullptr;
+  } catch (const c10::OutOfMemoryError &e) {
+    raise("torch", "OutOfMemoryError", e.what_without_backtrace());
   } catch (const c10::Error &e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception &e) {

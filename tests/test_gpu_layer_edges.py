@@ -335,3 +335,15 @@ def test_lazily_negated_views_are_refused():
         with pytest.raises(ValueError):
             call(z)
         call(z.resolve_neg())
+
+
+def test_out_of_memory_is_torchs():
+    """Outputs of 8 TB: the allocator refuses before anything is launched."""
+    one = torch.ones((1, 1), dtype=torch.bfloat16, device="cuda")
+    x, w = one.expand(1 << 21, 1), one.expand(1 << 21, 1)
+    with pytest.raises(torch.OutOfMemoryError):
+        kernels.linear(x, w)
+    with pytest.raises(torch.OutOfMemoryError):
+        kernels.dropout(torch.ones((1, 1 << 21), dtype=torch.bfloat16, device="cuda")
+                        .expand(1 << 21, 1 << 21), None)
+    assert float(kernels.linear(one, one)) == 1.0
