@@ -113,14 +113,18 @@ def build_front(verbose: bool = False) -> str:
 
 def build_layer(verbose: bool = False) -> str:
     """Build the Python module ``_layer`` (the layer operators on torch tensors,
-    linked to ``libferro_cuda.so`` and torch) with g++."""
+    linked to ``libferro_cuda.so`` and torch) with g++.  It is tied to the torch it
+    was compiled against, so another torch rebuilds it."""
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
+    os.makedirs(OBJDIR, exist_ok=True)
     mod = os.path.join(HERE, "_layer" + sysconfig.get_config_var("EXT_SUFFIX"))
     src = os.path.join(CSRC, "layer_py.cpp")
-    if _stale(mod, [src, os.path.join(ROOT, "include", "ferro_cuda.h")]):
-        abi = int(torch.compiled_with_cxx11_abi())
+    abi = int(torch.compiled_with_cxx11_abi())
+    built_for = f"{torch.__version__} {torch.version.git_version} abi {abi}"
+    stamp = os.path.join(OBJDIR, "layer_torch")
+    if _stale(mod, [src, os.path.join(ROOT, "include", "ferro_cuda.h")]) or _read(stamp) != built_for:
         cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
                f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
                *[f"-isystem{p}" for p in include_paths()], "-isystem/usr/local/cuda/include",
@@ -130,7 +134,16 @@ def build_layer(verbose: bool = False) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+        with open(stamp, "w") as f:
+            f.write(built_for)
     return mod
+
+
+def _read(path: str) -> str:
+    if not os.path.exists(path):
+        return ""
+    with open(path) as f:
+        return f.read()
 
 
 if __name__ == "__main__":
