@@ -5,6 +5,7 @@ Run ``python -m ferrograd_b200.build`` (or ``__graft_entry__.build()``).
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
@@ -37,7 +38,8 @@ def build(verbose: bool = False) -> str:
     """Build the CUDA library, then the front end and the layer binding on top of it."""
     lib = build_cuda(verbose)
     build_front(verbose)
-    build_layer(verbose)
+    if importlib.util.find_spec("torch") is not None:  # the rest does without it
+        build_layer(verbose)
     return lib
 
 

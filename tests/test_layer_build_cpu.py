@@ -1,5 +1,7 @@
 """When the layer operators' binding is compiled."""
 import os
+import subprocess
+import sys
 
 import torch
 
@@ -22,3 +24,11 @@ def test_another_torch_rebuilds_the_binding(monkeypatch, tmp_path):
     assert len(ran) == 1 and any(a.endswith("layer_py.cpp") for a in ran[0])
     build.build_layer()
     assert len(ran) == 1
+
+
+def test_the_libraries_build_without_torch():
+    code = ("import sys; sys.modules['torch'] = None; from ferrograd_b200 import build; "
+            "print(build.build())")
+    got = subprocess.run([sys.executable, "-c", code], cwd=build.ROOT, capture_output=True, text=True)
+    assert got.returncode == 0, got.stderr
+    assert got.stdout.strip() == build.LIB
