@@ -38,6 +38,13 @@ static DevCtx g_ctx[64];
 DevCtx *ctx_current() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  // A thread's first use of a device binds its context: the driver calls that
+  // describe tensors to TMA need one, and not every path launches a kernel first.
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return nullptr;
+    bound = dev;
+  }
   std::lock_guard<std::mutex> lock(g_ctx_mu);
   DevCtx &c = g_ctx[dev];
   if (c.ordinal < 0) {

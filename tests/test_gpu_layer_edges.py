@@ -1,5 +1,7 @@
 """The layer operators at the edges of their range: the bounds are those of
 test_gpu_layer.py unless a test derives its own."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -347,3 +349,22 @@ def test_out_of_memory_is_torchs():
         kernels.dropout(torch.ones((1, 1 << 21), dtype=torch.bfloat16, device="cuda")
                         .expand(1 << 21, 1 << 21), None)
     assert float(kernels.linear(one, one)) == 1.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_new_threads_first_call(dtype):
+    """A thread that has made no CUDA call yet has no context bound to it."""
+    dt = TYPES[dtype]
+    x, w = torch.randn((300, 264), device="cuda").to(dt), torch.randn((136, 264), device="cuda").to(dt)
+    dy = torch.randn((300, 136), device="cuda").to(dt)
+    calls = [lambda: kernels.linear(x, w), lambda: kernels.linear_grad(dy, x, w)[0],
+             lambda: kernels.linear(x[:1], w), lambda: kernels.dropout(x, kernels.Dropout(0.5, 1))]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    for call, ref in zip(calls, want):
+        got = []
+        thread = threading.Thread(target=lambda: got.append(call()))
+        thread.start()
+        thread.join()
+        torch.cuda.synchronize()
+        assert got and torch.equal(got[0], ref)
