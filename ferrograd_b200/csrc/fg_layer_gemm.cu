@@ -37,6 +37,7 @@
 
 #include <math.h>
 
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -864,7 +865,7 @@ static int launch(Problems<TWO> &ps, int ctas, size_t ring_cap, cudaStream_t st)
     g.slab_at = p.slab_at;
     if (bytes < p.bytes) bytes = p.bytes;
   }
-  static bool attr_done[64] = {};
+  static std::atomic<bool> attr_done[64];  // (callers on several threads)
   int dev = 0;
   FG_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {

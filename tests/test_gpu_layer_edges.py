@@ -1,5 +1,6 @@
 """The layer operators at the edges of their range: the bounds are those of
 test_gpu_layer.py unless a test derives its own."""
+import ctypes
 import threading
 
 import numpy as np
@@ -368,3 +369,42 @@ def test_a_new_threads_first_call(dtype):
         thread.join()
         torch.cuda.synchronize()
         assert got and torch.equal(got[0], ref)
+
+
+def test_threads_call_at_once():
+    """The C entry point from eight threads, each with its stream and buffers (ctypes
+    lets go of the interpreter's lock), the first calls of their kernels among them."""
+    L = kernels._lib.lib()
+    shapes = [(200, 136, 264, torch.float32), (64, 72, 2048, torch.float16),
+              (40, 8200, 512, torch.bfloat16), (2600, 2312, 96, torch.float32)]
+    codes = {torch.float32: kernels._lib.F32, torch.bfloat16: kernels._lib.BF16,
+             torch.float16: kernels._lib.F16}
+    jobs = []
+    for i in range(8):
+        m, n, k, dt = shapes[i % 4]
+        x, w = torch.randn((m, k), device="cuda").to(dt), torch.randn((n, k), device="cuda").to(dt)
+        out, ws = torch.zeros((m, n), dtype=dt, device="cuda"), torch.empty(1 << 26, dtype=torch.uint8,
+                                                                           device="cuda")
+        a = kernels._lib.LinearArgsC(dtype=codes[dt], M=m, N=n, K=k, x=x.data_ptr(), x_row=k, x_col=1,
+                                     w=w.data_ptr(), w_row=k, w_col=1, out=out.data_ptr(), ld_out=n,
+                                     workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+        jobs.append((a, torch.cuda.Stream(), x, w, out, ws))
+    torch.cuda.synchronize()
+    start, failed, done = threading.Barrier(8), [], []
+
+    def work(a, stream):
+        start.wait()
+        for _ in range(50):
+            if L.fg_linear(ctypes.byref(a), stream.cuda_stream):
+                failed.append(L.fg_last_error())
+        done.append(1)
+
+    threads = [threading.Thread(target=work, args=job[:2]) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(done) == 8 and not failed, failed[:1]
+    for a, _, x, w, out, _ in jobs:
+        assert torch.equal(out, kernels.linear(x, w))
