@@ -13,7 +13,8 @@ pass recomputes it from ``(seed, offset)``.
 
 Weights are initialised as ``Linear::new`` (src/nn.rs:77-85).  With a 16-bit
 ``dtype`` the layers compute in that type from f32 master weights, which
-``Sgd::step`` (src/optim.rs:60-71) updates.
+``Sgd::step`` (src/optim.rs:60-71) updates.  The loss is not scaled: in f16,
+gradients below 2^-24 are lost, so bf16 is the type for large batches.
 """
 from __future__ import annotations
 
@@ -89,15 +90,16 @@ class ResidualMlp:
                        for _ in range(blocks)]
         self.last = make(width, classes)
         self.steps = 0
+        self.draws = 0  # training forward passes so far
 
     def layers(self) -> List[Layer]:
         return [self.first, *[layer for block in self.blocks for layer in block], self.last]
 
     def _drop(self, layer: Layer, index: int, train: bool) -> Optional[kernels.Dropout]:
-        """The layer's draw of this step: every layer and step has its own offset."""
+        """The layer's draw of this pass: every layer and training pass has its own offset."""
         if not train or layer.p == 0.0:
             return None
-        return kernels.Dropout(layer.p, self.seed, self.steps * 2 * len(self.blocks) + index)
+        return kernels.Dropout(layer.p, self.seed, self.draws * 2 * len(self.blocks) + index)
 
     def forward(self, x: torch.Tensor, train: bool = False) -> torch.Tensor:
         """Logits [rows, classes]; a single row to serve is ``x`` of one row."""
@@ -105,12 +107,15 @@ class ResidualMlp:
         for i, (up, down) in enumerate(self.blocks):
             a = up.forward(h, drop=self._drop(up, 2 * i, train), train=train)
             h = down.forward(a, residual=h, drop=self._drop(down, 2 * i + 1, train), train=train)
+        if train:
+            self.draws += 1
         return self.last.forward(h, train=train)
 
     __call__ = forward
 
     def backward(self, dlogits: torch.Tensor) -> None:
-        """Gradients of every parameter into the layers' ``grads``."""
+        """Gradients of every parameter, for the last training forward pass, into the
+        layers' ``grads`` (in place of what was there)."""
         dh = self.last.backward(dlogits.to(self.dtype))
         for up, down in reversed(self.blocks):
             # the residual passes dh on unchanged, next to the block's own path
