@@ -458,7 +458,7 @@ static Span span(const void *p, int64_t rows, int64_t cols, int64_t rs, int64_t 
 // one pitched buffer (equal pitch, disjoint columns) do not.
 static bool overlap(const void *w, int64_t rows, int64_t cols, int64_t ld, const void *q,
                     int64_t qrows, int64_t qcols, int64_t qrs, int64_t qcs, int es) {
-  if (!w || !q) return false;
+  if (!w || !q || rows <= 0 || cols <= 0 || qrows <= 0 || qcols <= 0) return false;
   const Span a = span(w, rows, cols, ld, 1, es), b = span(q, qrows, qcols, qrs, qcs, es);
   if (a.lo >= b.hi || b.lo >= a.hi) return false;
   if (ld == qrs && qcs == 1 && ld > 0) {

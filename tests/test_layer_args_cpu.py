@@ -47,3 +47,17 @@ def test_workspace_boundary():
         for off in (1, 2, 4, 8, 16, 128):
             a.workspace = BASE + 0x80000 + off
             refused(call(ctypes.byref(a), None), "boundary")
+
+
+def test_nothing_overlaps_an_empty_array():
+    """No bytes are shared with an array of no elements, wherever it points.  (Past
+    the refusals the call asks for a device, which is another error, or has one.)"""
+    L = _lib.lib()
+    need = ctypes.c_size_t()
+    a = linear_args(K=0, x=BASE + 0x20010, w=BASE + 0x20020)
+    assert L.fg_linear_workspace(ctypes.byref(a), ctypes.byref(need)) == 0
+    for kw in (dict(N=0, dy=BASE + 0x30010, db=BASE + 0x30020, dw=BASE + 0x30030),
+               dict(K=0, x=BASE + 0x50000, w=BASE + 0x50002, dx=BASE + 0x50004),
+               dict(M=0, dy=BASE + 0x40010, x=BASE + 0x40020, dx=BASE + 0x40040)):
+        g = grad_args(**kw)
+        assert L.fg_linear_grad_workspace(ctypes.byref(g), ctypes.byref(need)) == 0, kw
