@@ -953,7 +953,7 @@ static int make_problem(Problem *pr, int dtype, const Operand &a, const Operand 
   g.M = e.M;
   g.N = e.N;
   g.nk = k_blocks(K, planes);
-  g.chain = planes == 3 ? 2 : kChain16;
+  g.chain = chain_blocks(planes, bf16);
   g.split = f.split;
   g.group = f.pair ? 16 : 8;
   g.bf16 = bf16;
@@ -972,7 +972,8 @@ int run_tensor_product(int dtype, const Product &x, cudaStream_t st) {
   DevCtx *ctx = ctx_current();
   if (!ctx) return set_error(FG_ERR_CUDA, "no CUDA device context");
   const int sms = ctx->num_sms ? ctx->num_sms : 148;
-  const Form f = pick_form(x.e.M, x.e.N, x.K, dtype == FG_F32 ? 3 : 1, sms);
+  const int planes = dtype == FG_F32 ? 3 : 1;
+  const Form f = pick_form(x.e.M, x.e.N, x.K, planes, chain_blocks(planes, dtype != FG_F16), sms);
   Problems<false> ps = {};
   int rc = make_problem(&ps.at[0], dtype, x.a, x.b, x.K, x.e, f, ctx->d_err);
   if (rc) return rc;
@@ -997,7 +998,8 @@ int run_tensor_products(int dtype, const Product &x, const Product &y, cudaStrea
   const int64_t tiles = tiles_of(x.e, 128, 64) + tiles_of(y.e, 128, 64);
   int split = 1;  // as far as both have k-blocks and the CTAs one turn
   while (split < 8 && 2 * split <= nkx && 2 * split <= nky && tiles * 2 * split <= sms) split *= 2;
-  const bool one_chain = planes == 3 || (nkx <= kChain16 * split && nky <= kChain16 * split);
+  const int chain = chain_blocks(planes, dtype != FG_F16);
+  const bool one_chain = planes == 3 || (nkx <= chain * split && nky <= chain * split);
   if (!one_chain || tiles > 2 * sms) {
     int rc = run_tensor_product(dtype, x, st);
     return rc ? rc : run_tensor_product(dtype, y, st);

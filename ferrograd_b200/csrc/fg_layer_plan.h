@@ -10,10 +10,13 @@ namespace fg {
 namespace layer {
 
 constexpr int kMaxStages = 16;
-// k-blocks of a chain of 16-bit products: 16384 deep, 1024 truncated additions
-// of 2^-24 of the sum each at most.  Outputs of 8 or 11 bits do not show that
-// (f16 rounds by up to 2^-11).
-constexpr int kChain16 = 256;
+// k-blocks of one accumulation chain.  The tensor cores cut the sum at each
+// addition, so a chain drifts towards 0: measured on products of one sign, by
+// 2^-15.3 of the sum over 4096 terms and 2^-13.3 over 16384.  A rounding to f16 is off
+// by 2^-12.3 on average, to bf16 by 2^-9.3: the longer chain does not show in bf16,
+// in f16 it makes the whole error 12% larger and the shorter one 1%.  f32 takes 64
+// terms.
+inline int chain_blocks(int planes, bool bf16) { return planes == 3 ? 2 : bf16 ? 256 : 64; }
 constexpr size_t kSharedMax = 227 * 1024;  // what a CTA may ask for
 
 constexpr int kSlabPitch = 20;   // floats; of a warp's 32 x 16 slab (pair)
@@ -104,7 +107,7 @@ inline SharedPlan lay_out(const SharedShape &s, size_t ring_cap) {
 // part.  It picks the fastest form or one within 10% of it on all 17 (24 x 8192 x
 // 2048 f16: 64 wide, k over 8 CTAs, 10.2 against 22.7 unsplit and 42.4 by pairs;
 // 1024 x 4096 x 4096 bf16: pairs, 27.6 against 35.1 and 48.3).
-inline Form pick_form(int M, int N, int K, int planes, int sms) {
+inline Form pick_form(int M, int N, int K, int planes, int chain, int sms) {
   const double steps = K / 16.0 * (planes == 3 ? 6.0 : 1.0);
   Form best{true, 256, 256, 1};
   const double pairs = ceil(M / 256.0) * ceil(N / 256.0);
@@ -116,7 +119,7 @@ inline Form pick_form(int M, int N, int K, int planes, int sms) {
     // (128-wide CTAs take one chain of 16-bit products, and run one to an SM, so
     // that not enough clusters of 8 fit)
     for (int split = 1; split <= (bn == 64 ? 8 : 4) && split <= nk; split *= 2) {
-      if (bn == 128 && (planes == 3 || nk > (int64_t)kChain16 * split)) continue;
+      if (bn == 128 && (planes == 3 || nk > (int64_t)chain * split)) continue;
       const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
       if (ctas > 1e8) continue;
       const double fixed = 1.8 + rows * (bn == 64 ? 1.9 : 3.4);
