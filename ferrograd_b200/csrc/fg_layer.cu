@@ -42,15 +42,15 @@ __global__ void __launch_bounds__(256) k_linear_empty(const Epilogue e) {
 // next four steps before it multiplies.  The warp's sums meet by shuffles in a
 // fixed order.  (A tensor-core tile of so few rows first fills and drains
 // accumulators, and joins its k-ranges across CTAs: 1 x 4096 x 4096 bf16, the
-// weight from HBM, 11.6 us against 8.3 us here, 4.0 TB/s: 33 MB are too few for
+// weight from HBM, 12.5 us against 8.7 us here, 3.9 TB/s: 33 MB are too few for
 // the copy rate.)  VEC: every row starts on a 16-byte boundary; without it
 // elements are read one by one, still in neighbouring lanes.
 // ---------------------------------------------------------------------------
 constexpr int kRowsMax = 8;
 
 // For MR rows of x: the weight's rows a warp takes, and the steps it has in
-// flight.  One 16-bit row of 4096 by itself is 1 x 4096 x 4096 from HBM in 8.3 us,
-// two together 11.6; two f32 rows 15.5, one 16.2.
+// flight.  One 16-bit row of 4096 by itself is 1 x 4096 x 4096 from HBM in 8.7 us, two
+// together 12.3; f32 rows by two take 26 us for four rows of x, one by one 38.
 template <typename T, int MR>
 struct RowsShape {
   static constexpr int rows = sizeof(T) == 2 ? 1 : 2;
@@ -116,7 +116,10 @@ __global__ void __launch_bounds__(256)
   for (int c = 0; c < R; c++) wp[c] = w + min(n0 + c, e.N - 1) * wr;
   float acc[MR][R] = {};
   using Raw = typename RawOf<T, VEC>::type;
+  // The weight passes once and x is read by every warp: the one leaves L1 first.
+  // (8 x 4096 -> 4096 f32 32 us, with ordinary loads 42; 2 rows in bf16 10.3, 12.4.)
   auto read = [](const T *p) { return *reinterpret_cast<const Raw *>(p); };
+  auto pass = [](const T *p) { return __ldcs(reinterpret_cast<const Raw *>(p)); };
   auto step = [&](int64_t k, const Raw(&rw)[R]) {
     float b[R][V];
 #pragma unroll
@@ -141,14 +144,14 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int c = 0; c < R; c++) r[u][c] = read(wp[c] + k + u * S);
+      for (int c = 0; c < R; c++) r[u][c] = pass(wp[c] + k + u * S);
 #pragma unroll
     for (int u = 0; u < U; u++) step(k + u * S, r[u]);
   }
   for (; k + V <= K; k += S) {
     Raw r[R];
 #pragma unroll
-    for (int c = 0; c < R; c++) r[c] = read(wp[c] + k);
+    for (int c = 0; c < R; c++) r[c] = pass(wp[c] + k);
     step(k, r);
   }
   if (VEC && k < K)  // the row's last elements, fewer than V (one lane has them)
