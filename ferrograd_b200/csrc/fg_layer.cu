@@ -57,12 +57,13 @@ struct RowsShape {
   static constexpr int steps = MR <= 4 ? 4 : 2;
 };
 
-// Rows up to which it beats the tensor cores' few-row tiles (4096 x 4096): in
-// f32 8 (22 us against 56, which has to split the weight into planes first),
-// in 16 bits 2, or 4 where the weight would have to be copied to be aligned.
-static int rows_limit(int dtype, bool aligned) {
-  return dtype == FG_F32 ? kRowsMax : aligned ? 2 : 4;
-}
+// Rows up to which it is used instead of the tensor cores' few-row tiles.  In f32 8,
+// as those have to split the weight into planes first (8 x 4096 -> 4096 32 us against 62;
+// off 16-byte rows 50, 68), in 16 bits 2 (10.2, 12.4; off 16-byte rows, where the
+// tiles need a copy of the weight, 22.4, 28.3 -- but 46, 28.5 for three).  Measured at
+// 4096 x 4096.  A small layer gains more (2 x 256 -> 256 1.8, 4.5); a long row into few
+// outputs loses, as its warps are few: 2 x 8192 -> 128 bf16 12.9, 7.8; 8 in f32 51, 22.
+static int rows_limit(int dtype) { return dtype == FG_F32 ? kRowsMax : 2; }
 
 // What a lane reads at once: 16 bytes, or one element.
 template <typename T, bool VEC>
@@ -182,14 +183,11 @@ static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaSt
     return launch_early(kern, dim3(grid), 256, st, x, g->x_row, w, g->w_row, g->K, e);
   };
   if (g->M == 1) return vec ? go(k_linear_rows<T, 1, true>) : go(k_linear_rows<T, 1, false>);
-  if (g->M == 2) return vec ? go(k_linear_rows<T, 2, true>) : go(k_linear_rows<T, 2, false>);
-  // 16-bit rows of 16-byte reads end at two, others at four (rows_limit)
-  if constexpr (sizeof(T) == 2) {
-    return go(k_linear_rows<T, 4, false>);
-  } else {
-    if (g->M <= 4) return vec ? go(k_linear_rows<T, 4, true>) : go(k_linear_rows<T, 4, false>);
-    return vec ? go(k_linear_rows<T, 8, true>) : go(k_linear_rows<T, 8, false>);
+  if constexpr (sizeof(T) == 4) {  // 16-bit types end at two rows (rows_limit)
+    if (g->M > 4) return vec ? go(k_linear_rows<T, 8, true>) : go(k_linear_rows<T, 8, false>);
+    if (g->M > 2) return vec ? go(k_linear_rows<T, 4, true>) : go(k_linear_rows<T, 4, false>);
   }
+  return vec ? go(k_linear_rows<T, 2, true>) : go(k_linear_rows<T, 2, false>);
 }
 
 // ---------------------------------------------------------------------------
@@ -502,7 +500,7 @@ static LinearPlan plan_linear(const fg_linear_args *g) {
   if (g->M == 0 || g->N == 0 || g->K == 0) return p;
   const int es = elem_size(g->dtype);
   p.vec = rows16(g->x, g->M == 1 ? 0 : g->x_row, es) && rows16(g->w, g->w_row, es);
-  p.rows = g->M <= rows_limit(g->dtype, p.vec) && (g->x_col == 1 || g->K == 1) &&
+  p.rows = g->M <= rows_limit(g->dtype) && (g->x_col == 1 || g->K == 1) &&
            (g->w_col == 1 || g->K == 1);
   if (p.rows) return p;
   p.x = resolve_operand(g->dtype, {g->x, g->x_row, g->x_col}, g->M, g->K, &p.jobs, &p.bytes);

@@ -1,7 +1,11 @@
 """The layer products' shared-memory layout over every form and row count, and what
 their kernels may not use."""
+import ctypes
 import os
 import subprocess
+
+from ferrograd_b200 import _lib
+from test_layer_cpu import linear_args
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -26,3 +30,18 @@ def test_no_constant_loads_in_kernels_that_start_early():
             lines = [line.split("//")[0] for line in f]
         for word in ("__ldg", "__restrict__", "ld.global.nc"):
             assert not any(word in line for line in lines), (name, word)
+
+
+def test_unaligned_rows_go_where_they_are_faster():
+    """Three and four 16-bit rows off 16-byte boundaries take the tensor cores, whose
+    copy of the weight shows as workspace (4 x 4095 -> 4096: 28.5 us, 46 row by row)."""
+    L = _lib.lib()
+    need = ctypes.c_size_t()
+    for rows, staged in ((1, False), (2, False), (3, True), (4, True), (5, True)):
+        a = linear_args(M=rows, N=64, K=33, x_row=33, w_row=33, ld_out=64)
+        assert L.fg_linear_workspace(ctypes.byref(a), ctypes.byref(need)) == 0
+        assert (need.value > 0) == staged
+    for rows, staged in ((8, False), (9, True)):
+        a = linear_args(dtype=_lib.F32, M=rows)
+        assert L.fg_linear_workspace(ctypes.byref(a), ctypes.byref(need)) == 0
+        assert (need.value > 0) == staged
