@@ -940,11 +940,6 @@ static int run_two(Problems<true> &ps, int64_t ctas, int sms, cudaStream_t st) {
   return launch<T, PLANES, 1, 64, PLANES == 3, false, true>(ps, (int)ctas, ring, st);
 }
 
-static int k_blocks(int K, int planes) {
-  const int bk = planes == 3 ? 32 : 64;
-  return (int)((K + (int64_t)bk - 1) / bk);
-}
-
 static int make_problem(Problem *pr, int dtype, const Operand &a, const Operand &b, int K,
                         const Epilogue &e, const Form &f, unsigned int *err) {
   const int planes = dtype == FG_F32 ? 3 : 1, bk = planes == 3 ? 32 : 64;
@@ -973,7 +968,8 @@ int run_tensor_product(int dtype, const Product &x, cudaStream_t st) {
   if (!ctx) return set_error(FG_ERR_CUDA, "no CUDA device context");
   const int sms = ctx->num_sms ? ctx->num_sms : 148;
   const int planes = dtype == FG_F32 ? 3 : 1;
-  const Form f = pick_form(x.e.M, x.e.N, x.K, planes, chain_blocks(planes, dtype != FG_F16), sms);
+  const Form f =
+      pick_form({x.e.M, x.e.N, x.K}, planes, chain_blocks(planes, dtype != FG_F16), sms);
   Problems<false> ps = {};
   int rc = make_problem(&ps.at[0], dtype, x.a, x.b, x.K, x.e, f, ctx->d_err);
   if (rc) return rc;
@@ -987,36 +983,31 @@ int run_tensor_product(int dtype, const Product &x, cudaStream_t st) {
   }
 }
 
-// Two independent products (a gradient's dx and dw): in one launch where each
-// alone would leave SMs idle and the 64-wide tiles of both fit them twice over.
+// Two independent products, in one launch where that is cheaper.
 int run_tensor_products(int dtype, const Product &x, const Product &y, cudaStream_t st) {
   DevCtx *ctx = ctx_current();
   if (!ctx) return set_error(FG_ERR_CUDA, "no CUDA device context");
   const int sms = ctx->num_sms ? ctx->num_sms : 148;
   const int planes = dtype == FG_F32 ? 3 : 1;
-  const int nkx = k_blocks(x.K, planes), nky = k_blocks(y.K, planes);
-  const int64_t tiles = tiles_of(x.e, 128, 64) + tiles_of(y.e, 128, 64);
-  int split = 1;  // as far as both have k-blocks and the CTAs one turn
-  while (split < 8 && 2 * split <= nkx && 2 * split <= nky && tiles * 2 * split <= sms) split *= 2;
-  const int chain = chain_blocks(planes, dtype != FG_F16);
-  const bool one_chain = planes == 3 || (nkx <= chain * split && nky <= chain * split);
-  if (!one_chain || tiles > 2 * sms) {
+  Form f;
+  if (!joint_form({x.e.M, x.e.N, x.K}, {y.e.M, y.e.N, y.K}, planes,
+                  chain_blocks(planes, dtype != FG_F16), sms, &f)) {
     int rc = run_tensor_product(dtype, x, st);
     return rc ? rc : run_tensor_product(dtype, y, st);
   }
-  const Form f{false, 128, 64, split};
+  const int64_t tx = tiles_of(x.e, 128, 64) * f.split, ctas = tx + tiles_of(y.e, 128, 64) * f.split;
   Problems<true> ps = {};
-  ps.ctas = (int)(tiles_of(x.e, 128, 64) * split);
+  ps.ctas = (int)tx;
   int rc = make_problem(&ps.at[0], dtype, x.a, x.b, x.K, x.e, f, ctx->d_err);
   if (rc) return rc;
   if ((rc = make_problem(&ps.at[1], dtype, y.a, y.b, y.K, y.e, f, ctx->d_err))) return rc;
   switch (dtype) {
     case FG_F32:
-      return run_two<float, 3>(ps, tiles * split, sms, st);
+      return run_two<float, 3>(ps, ctas, sms, st);
     case FG_BF16:
-      return run_two<__nv_bfloat16, 1>(ps, tiles * split, sms, st);
+      return run_two<__nv_bfloat16, 1>(ps, ctas, sms, st);
     default:
-      return run_two<__half, 1>(ps, tiles * split, sms, st);
+      return run_two<__half, 1>(ps, ctas, sms, st);
   }
 }
 

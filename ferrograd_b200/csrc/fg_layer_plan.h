@@ -32,7 +32,17 @@ constexpr int block_warps(int cg, bool run) {
 struct Form {
   bool pair;
   int bm, bn, split;
+  double cost;  // estimated, in microseconds
 };
+// A product's rows, columns and depth.
+struct Extent {
+  int M, N, K;
+};
+inline int k_blocks(int K, int planes) {
+  const int bk = planes == 3 ? 32 : 64;
+  return (int)((K + (int64_t)bk - 1) / bk);
+}
+inline double mma_steps(int K, int planes) { return K / 16.0 * (planes == 3 ? 6.0 : 1.0); }
 
 // Shared memory a CTA must ask for so that the CTAs that fit on an SM never
 // need more than its 512 TMEM columns between them: an allocation that had to
@@ -107,20 +117,18 @@ inline SharedPlan lay_out(const SharedShape &s, size_t ring_cap) {
 // part.  It picks the fastest form or one within 10% of it on all 17 (24 x 8192 x
 // 2048 f16: 64 wide, k over 8 CTAs, 10.2 against 22.7 unsplit and 42.4 by pairs;
 // 1024 x 4096 x 4096 bf16: pairs, 27.6 against 35.1 and 48.3).
-inline Form pick_form(int M, int N, int K, int planes, int chain, int sms) {
-  const double steps = K / 16.0 * (planes == 3 ? 6.0 : 1.0);
-  Form best{true, 256, 256, 1};
-  const double pairs = ceil(M / 256.0) * ceil(N / 256.0);
-  double cost = ceil(pairs / (sms / 2)) * steps * 0.07 + 6.8;
-  const int bk = planes == 3 ? 32 : 64;
-  const int nk = (int)((K + (int64_t)bk - 1) / bk);
-  const double rows = M < 128 ? M / 128.0 : 1.0;
+inline Form pick_form(const Extent &e, int planes, int chain, int sms) {
+  const double steps = mma_steps(e.K, planes);
+  const double pairs = ceil(e.M / 256.0) * ceil(e.N / 256.0);
+  Form best{true, 256, 256, 1, ceil(pairs / (sms / 2)) * steps * 0.07 + 6.8};
+  const int nk = k_blocks(e.K, planes);
+  const double rows = e.M < 128 ? e.M / 128.0 : 1.0;
   for (int bn = 64; bn <= 128; bn *= 2)
     // (128-wide CTAs take one chain of 16-bit products, and run one to an SM, so
     // that not enough clusters of 8 fit)
     for (int split = 1; split <= (bn == 64 ? 8 : 4) && split <= nk; split *= 2) {
       if (bn == 128 && (planes == 3 || nk > (int64_t)chain * split)) continue;
-      const double ctas = ceil(M / 128.0) * ceil((double)N / bn) * split;
+      const double ctas = ceil(e.M / 128.0) * ceil((double)e.N / bn) * split;
       if (ctas > 1e8) continue;
       const double fixed = 1.8 + rows * (bn == 64 ? 1.9 : 3.4);
       const double join = split > 1 ? 0.7 + rows * (bn == 64 ? 1.1 : 3.1) : 0.0;
@@ -128,12 +136,40 @@ inline Form pick_form(int M, int N, int K, int planes, int chain, int sms) {
           split > 1 || bn == 128 ? ceil(ctas / sms) : ctas > sms ? ctas / sms : 1.0;
       const double turns = bn == 64 ? ceil(ctas / (2.0 * sms)) : per_sm;
       const double c = 1.5 + join + turns * fixed + per_sm * steps / split * 0.038;
-      if (c < cost) {
-        cost = c;
-        best = Form{false, 128, bn, split};
-      }
+      if (c < best.cost) best = Form{false, 128, bn, split, c};
     }
   return best;
+}
+
+// Two independent products (a gradient's dx and dw) as 64-wide split tiles in one
+// launch, with one split for both, as far as both have k-blocks and the CTAs one
+// turn: whether that is possible, and cheaper than a launch for each in its own form.
+// The longer product's CTAs bound it, or the SMs' share of all.  Of 31 gradients
+// timed both ways (16-bit and f32, 64 to 16384 rows, widths 64 to 8192) the estimates'
+// difference is within 5 us of the measured one for 25, and the slower way is picked for
+// three, by 1 to 4 us of 22 to 29.  256 x 784 -> 128 f32 takes 15.0 us in one launch and 21.0
+// in two, 512 x 1024 -> 1024 bf16 16.2 and 20.7; 8192 x 128 -> 128 bf16 34.7 and 21.5, 16384 x
+// 128 -> 64 f32 260 and 58: its dw, deep and of two tiles, is split no further than dx allows.
+inline bool joint_form(const Extent &x, const Extent &y, int planes, int chain, int sms, Form *f) {
+  auto tiles_of = [](const Extent &e) {
+    return (e.M + (int64_t)127) / 128 * ((e.N + (int64_t)63) / 64);
+  };
+  const int64_t tx = tiles_of(x), ty = tiles_of(y), tiles = tx + ty;
+  const int nkx = k_blocks(x.K, planes), nky = k_blocks(y.K, planes);
+  if (tiles > 2 * sms) return false;
+  int split = 1;
+  while (split < 8 && 2 * split <= nkx && 2 * split <= nky && tiles * 2 * split <= sms) split *= 2;
+  if (planes == 1 && (nkx > chain * split || nky > chain * split)) return false;
+  const double cx = mma_steps(x.K, planes) / split * 0.038;
+  const double cy = mma_steps(y.K, planes) / split * 0.038;
+  const double share = (double)split * (tx * cx + ty * cy) / sms;
+  const double longer = cx > cy ? cx : cy;
+  const int m = x.M > y.M ? x.M : y.M;
+  const double rows = m < 128 ? m / 128.0 : 1.0;
+  const double cost = 1.5 + (split > 1 ? 0.7 + rows * 1.1 : 0.0) + 1.8 + rows * 1.9 +
+                      (longer > share ? longer : share);
+  *f = Form{false, 128, 64, split, cost};
+  return cost < pick_form(x, planes, chain, sms).cost + pick_form(y, planes, chain, sms).cost;
 }
 
 }  // namespace layer
