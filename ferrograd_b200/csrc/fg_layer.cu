@@ -290,15 +290,25 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 #pragma unroll
   for (int i = 0; i < 8; i++) red[ty][tx * 8 + i] = sum[i];
   __syncthreads();
-  const int c = blockIdx.x * (TX * 8) + threadIdx.x;
+  // a tree of TY terms, eight at a time
+  constexpr int C = TX * 8;
+  auto eight = [&](int r, int col8) {
+    float t[8];
 #pragma unroll
-  for (int half = TY / 2; half > 0; half /= 2) {  // a tree: TY terms, log2 TY roundings
-    for (int i = threadIdx.x; i < half * TX * 8; i += 256)
-      red[i / (TX * 8)][i % (TX * 8)] += red[i / (TX * 8) + half][i % (TX * 8)];
+    for (int i = 0; i < 8; i++) t[i] = red[r + i][col8];
+    return ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+  };
+  static_assert(TY * C == 8 * 256, "every thread has eight terms of a column");
+  float s = eight(threadIdx.x / C * 8, threadIdx.x % C);
+  if (TY > 8) {
     __syncthreads();
+    red[threadIdx.x / C][threadIdx.x % C] = s;
+    __syncthreads();
+    if (threadIdx.x < C) s = eight(0, threadIdx.x);
   }
-  if (threadIdx.x < TX * 8 && c < N) {
-    const float s = red[0][threadIdx.x] * by.after;
+  const int c = blockIdx.x * C + threadIdx.x;
+  if (threadIdx.x < C && c < N) {
+    s *= by.after;
     if (gridDim.y == 1)
       db[c] = from_f32<T>(s);
     else
