@@ -197,10 +197,11 @@ static int run_rows(const fg_linear_args *g, const Epilogue &e, bool vec, cudaSt
 // (DzScale): without dropout's scale the 16-bit types hold dy itself where no
 // slope multiplies it, and f16 does not overflow.
 // It reads dy and pre once and writes dz once: 1.6 GB at 16384 x 16384 bf16, GELU,
-// 246 us at the copy rate, measured 391 us: with the slope's exponential and the
-// conversions 36 instructions an element, the issue slots bound it, not HBM.  A
-// thread keeps its eight columns down the rows, so the column sums need no
-// exchange until the end, and asks for the next rows before it computes.
+// 246 us at the copy rate, measured 305 us, with dropout 400: the slope's exponential
+// and the conversions are 37 instructions an element, the mask's 5 more, and the issue
+// slots, 74% of them taken, bound it, not HBM.  A thread keeps its eight columns down
+// the rows, so the column sums need no exchange until the end, and asks for the next
+// rows before it computes.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void store_dz(void *dz, int64_t at, int64_t, const float (&v)[8]) {
@@ -349,8 +350,9 @@ __global__ void __launch_bounds__(1024)
 // ---------------------------------------------------------------------------
 // out = residual + D(x): eight columns of a row a step, one Philox call for them.
 // Bound by HBM, with the issue slots close behind: 16384 x 16384 bf16 with a
-// residual in 271 us, 5.9 TB/s or 0.91 of a copy's rate (an addition of the two
-// arrays alone takes 236 us).  A thread asks for all its groups before it draws.
+// residual in 266 us, 6.1 TB/s or 0.93 of a copy's rate (an addition of the two
+// arrays alone takes 236 us).  Rows off 16-byte boundaries go element by element: 4001 x
+// 4097 bf16 39 us, 4001 x 4096 17.  A thread asks for all its groups before it draws.
 // ---------------------------------------------------------------------------
 // Groups of eight columns a thread takes, 256 groups apart.
 template <typename T>
@@ -588,9 +590,8 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
   return run_tensor_product(g->dtype, {p.x, p.w, g->K, e}, st);
 }
 
-// How k_layer_dz is cut: blocks of 256 columns for large arrays (16384 x 16384
-// bf16: 391 us), of 32 columns x 64 rows for small ones; rows a
-// block such that there are several waves of blocks and a thread adds no more than
+// How k_layer_dz is cut: blocks of 256 columns for large arrays, of 32 columns x 64
+// rows for small ones; rows a block such that there are several waves of blocks and a thread adds no more than
 // 16 rows one after another for an f32 sum (64 for a 16-bit one), and one block for
 // all rows where eight passes do (then it writes db itself and a launch is saved).
 // f32 db is off by 2^-23 of random sums' norm then; with 128 chains added in

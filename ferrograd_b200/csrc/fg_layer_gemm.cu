@@ -25,12 +25,13 @@
 //         for few rows or few tiles.
 //
 // Large products are bound by the tensor cores, and those by power: 8192 x 4096 x
-// 8192 bf16 without an epilogue runs at 1720 TFLOP/s (95% of cycles with an MMA),
-// with GELU, dropout and pre at 1550 (89%); 16384 x 4096 x 16384 with them in 1.76 ms,
-// 1250.  Operands of either order feed the MMAs alike (1688 for two MN-major).
-// f32: 8192 x 4096 x 4096 in 1.31 ms, six products of it 1260.  Small ones are
-// bound by latencies: 24 x 8192 x 2048 f16 takes 10.2 us, of which the cluster's
-// join and the epilogue are 3.
+// 8192 bf16 without an epilogue takes 344 us, 1600 TFLOP/s (96% of cycles with an MMA),
+// with GELU, dropout and pre 375 us, 1470 (90%); 16384 x 4096 x 16384 with them 1.5 ms
+// in short runs, 1.77 ms, 1240 TFLOP/s, in long ones.  Operands of either order feed the
+// MMAs alike (the gradient's dx and dw of the first, the latter MN-major twice, 334 us).
+// f32: 8192 x 4096 x 4096 in 1.32 ms, six products of it 1250 TFLOP/s.  Small ones are
+// bound by latencies: 24 x 8192 x 2048 f16 takes 11 us with the weight in L2 (14 from
+// HBM), of which the cluster's join and the epilogue are 3.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>

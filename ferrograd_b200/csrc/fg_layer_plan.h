@@ -114,8 +114,8 @@ inline SharedPlan lay_out(const SharedShape &s, size_t ring_cap) {
 // width; around them a pair spends 6.8, a lone CTA 1.8 and for 128 rows another
 // 1.9 (64 wide) or 3.4; joining a cluster's sums costs 0.7 and for 128 rows
 // another 1.1 or 3.1.  64-wide CTAs run two to an SM and hide each other's fixed
-// part.  It picks the fastest form or one within 10% of it on all 17 (24 x 8192 x
-// 2048 f16: 64 wide, k over 8 CTAs, 10.2 against 22.7 unsplit and 42.4 by pairs;
+// part.  It picks the fastest form or one within 10% of it on all 17, operands in L2 (24 x
+// 8192 x 2048 f16: 64 wide, k over 8 CTAs, 10.2 against 22.7 unsplit and 42.4 by pairs;
 // 1024 x 4096 x 4096 bf16: pairs, 27.6 against 35.1 and 48.3).
 inline Form pick_form(const Extent &e, int planes, int chain, int sms) {
   const double steps = mma_steps(e.K, planes);

@@ -167,7 +167,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     kept as [K, N] is passed as its transpose); ``bias`` [N]; ``residual``
     [M, N].  ``act`` is one of ``ACTIVATIONS``.  With ``save_pre`` returns
     ``(out, pre)``, ``pre`` being the pre-activations ``linear_grad`` needs
-    for an activation.  ``out`` may be the residual.
+    for an activation.  ``out`` may be the residual.  No autograd graph is
+    recorded, whatever the arguments require.
 
     ``stream`` is a ``cudaStream_t`` as an integer (None: torch's current
     stream).  On another stream than the current one the call allocates its

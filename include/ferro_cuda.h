@@ -203,8 +203,8 @@ int fg_gemm_3xtf32(int M, int N, int K, const float *d_a, const float *d_a_lo, i
  * f32, bf16 or f16 (one dtype a call); every sum, activation and mask is
  * computed in f32 and each output is rounded once, except where stated.
  * Strides and pitches are in elements, of either sign for inputs; addresses are
- * multiples of the element's size; sizes of 0 are allowed (an empty sum is 0).  Work is enqueued on `stream` and nothing
- * is kept from one call to the next. */
+ * multiples of the element's size; sizes of 0 are allowed (an empty sum is 0).
+ * Work is enqueued on `stream` and nothing is kept from one call to the next. */
 enum fg_act {
   FG_ACT_NONE = 0,
   FG_ACT_RELU = 1,      /* (0 < z) ? z : 0 */
