@@ -148,7 +148,7 @@ struct Problems {
 // At 64 bytes of operands in and 64 out a cycle, the MMAs of 16-bit operands
 // leave next to nothing of shared memory's 128, and a warp's 16-byte global
 // accesses to 32 rows cost it 32 passes; a TMA block costs 8 to write and 8 to
-// read.  It needs rows on 16-byte boundaries.
+// read.  It needs rows on 16-byte boundaries that end on one.
 template <typename T, int PLANES, int CG, int BN, bool RUN, bool IO, bool TWO>
 __global__ void __launch_bounds__(Block<CG, RUN>::threads, CG == 1 && !RUN ? 2 : 1)
     k_layer_product(const __grid_constant__ Problems<TWO> ps) {
@@ -910,7 +910,9 @@ static int run_form(const Form &f, Problems<false> &ps, int sms, cudaStream_t st
     // warps' two blocks of 2 KB; f32: four of 48 KB beside eight of 4 KB
     constexpr bool kLong = PLANES == 3;
     const size_t ring = (kLong ? 192 : 160) * 1024;
-    if (e.vec && (!e.residual || e.ldr >= e.N)) {  // (a tensor map's rows may not repeat)
+    // (a tensor map's rows may not repeat, and a TMA store fills up a row's last 16
+    // bytes: beyond N it would write zeros over what lies there)
+    if (e.vec && (int64_t)e.N * sizeof(T) % 16 == 0 && (!e.residual || e.ldr >= e.N)) {
       int rc = make_io_map<T>(&maps.out, e.out, e.M, e.N, e.ldo);
       if (!rc && e.pre) rc = make_io_map<T>(&maps.pre, e.pre, e.M, e.N, e.ldp);
       if (!rc && e.residual) rc = make_io_map<T>(&maps.residual, e.residual, e.M, e.N, e.ldr);

@@ -114,8 +114,9 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *m
       : "memory");
 }
 
-// 2-D tiled TMA store from this CTA's shared memory (elements outside the
-// tensor are not written), tracked by the thread's bulk groups.
+// 2-D tiled TMA store from this CTA's shared memory, tracked by the thread's bulk
+// groups.  Rows outside the tensor are not written; of a row, whole 16-byte pieces
+// are: where it ends inside one, the rest is set to 0.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *smem_src, int x,
                                              int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::

@@ -431,3 +431,77 @@ def test_long_sums_hardly_drift(dtype, m, n, k):
     ref = x.double() @ w.double().t()
     mean = float(((got.double() - ref) / ref).mean())
     assert abs(mean) <= (2.0 ** -13 if dtype == "bf16" else 2.0 ** -15)
+
+
+# ---- nothing is written beside an output ------------------------------------------------------
+
+
+GUARD = -77.0
+
+
+def guarded(rows, cols, dt, pitch):
+    """[rows, cols] inside a buffer of GUARD, and a check that the rest still is."""
+    buf = torch.full((rows, pitch), GUARD, dtype=dt, device="cuda")
+
+    def intact():
+        return bool((buf[:, cols:] == GUARD).all())
+
+    return buf[:, :cols], intact
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [3, 40, 300, 2560])
+@pytest.mark.parametrize("less", range(9))
+def test_columns_beside_the_outputs_stay(dtype, m, less):
+    """Outputs that are the first columns of wider, aligned rows: every width modulo 8,
+    in every form of the product.  What lies beside them is somebody else's."""
+    dt, L, k, n = TYPES[dtype], kernels._lib.lib(), 72, 2304 - less
+    code = {"f32": kernels._lib.F32, "bf16": kernels._lib.BF16, "f16": kernels._lib.F16}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    new = lambda r, c: torch.randn((r, c), device="cuda").to(dt)  # noqa: E731
+    ws = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    x, w, r = new(m, k), new(n, k), new(m, 2320)[:, :n]
+    (out, out_ok), (pre, pre_ok) = guarded(m, n, dt, 2320), guarded(m, n, dt, 2336)
+    a = kernels._lib.LinearArgsC(
+        dtype=code, M=m, N=n, K=k, x=x.data_ptr(), x_row=k, x_col=1, w=w.data_ptr(), w_row=k, w_col=1,
+        residual=r.data_ptr(), ld_residual=2320, act=kernels._lib.ACT_RELU, pre=pre.data_ptr(),
+        ld_pre=2336, out=out.data_ptr(), ld_out=2320, workspace=ws.data_ptr(),
+        workspace_bytes=ws.numel())
+    assert L.fg_linear(ctypes.byref(a), stream) == 0
+    want = kernels.linear(x, w, act="relu", residual=r, save_pre=True)
+    assert torch.equal(out, want[0]) and torch.equal(pre, want[1])
+    assert out_ok() and pre_ok()
+    # dx [m, n] and dw [k, n] of a layer with n inputs
+    x, w, dy = new(m, n), new(k, n), new(m, k)
+    (dx, dx_ok), (dw, dw_ok) = guarded(m, n, dt, 2320), guarded(k, n, dt, 2320)
+    g = kernels._lib.LinearGradArgsC(
+        dtype=code, M=m, N=k, K=n, dy=dy.data_ptr(), dy_row=k, dy_col=1, x=x.data_ptr(), x_row=n,
+        x_col=1, w=w.data_ptr(), w_row=n, w_col=1, dx_residual=r.data_ptr(), ld_dx_residual=2320,
+        dx=dx.data_ptr(), ld_dx=2320, dw=dw.data_ptr(), ld_dw=2320, workspace=ws.data_ptr(),
+        workspace_bytes=ws.numel())
+    assert L.fg_linear_grad(ctypes.byref(g), stream) == 0
+    want = kernels.linear_grad(dy, x, w, dx_residual=r, need_db=False)
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+    assert dx_ok() and dw_ok()
+    y, y_ok = guarded(m, n, dt, 2320)
+    kernels.dropout(r, kernels.Dropout(0.5, 1), out=y)
+    assert y_ok()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_wide_gradients_leave_the_columns_beside_them(dtype):
+    """dw in the pair form too."""
+    dt, L = TYPES[dtype], kernels._lib.lib()
+    code = {"f32": kernels._lib.F32, "bf16": kernels._lib.BF16, "f16": kernels._lib.F16}[dtype]
+    m, n, k = 128, 2560, 2301
+    new = lambda r, c: torch.randn((r, c), device="cuda").to(dt)  # noqa: E731
+    dy, x, w = new(m, n), new(m, k), new(n, k)
+    ws = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    dw, ok = guarded(n, k, dt, 2304)
+    g = kernels._lib.LinearGradArgsC(
+        dtype=code, M=m, N=n, K=k, dy=dy.data_ptr(), dy_row=n, dy_col=1, x=x.data_ptr(), x_row=k,
+        x_col=1, w=w.data_ptr(), w_row=k, w_col=1, dw=dw.data_ptr(), ld_dw=2304,
+        workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    assert L.fg_linear_grad(ctypes.byref(g), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(dw, kernels.linear_grad(dy, x, w, need_dx=False, need_db=False)[1])
+    assert ok()
