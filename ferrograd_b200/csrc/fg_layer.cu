@@ -591,11 +591,11 @@ static int linear(const fg_linear_args *g, cudaStream_t st) {
 }
 
 // How k_layer_dz is cut: blocks of 256 columns for large arrays, of 32 columns x 64
-// rows for small ones; rows a block such that there are several waves of blocks and a thread adds no more than
-// 16 rows one after another for an f32 sum (64 for a 16-bit one), and one block for
-// all rows where eight passes do (then it writes db itself and a launch is saved).
-// f32 db is off by 2^-23 of random sums' norm then; with 128 chains added in
-// turn it was 2^-22.
+// rows for small ones; rows a block such that there are several waves of blocks and
+// a thread adds no more than 16 rows one after another for an f32 sum (64 for a
+// 16-bit one), and one block for all rows where eight passes do (then it writes db
+// itself and a launch is saved).  f32 db is off by 2^-23 of random sums' norm then;
+// with 128 chains added in turn it was 2^-22.
 struct DzShape {
   int vec, tx, rows, chunks;
 };
